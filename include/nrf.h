@@ -26,7 +26,7 @@ extern "C" {
 
 /* bumped whenever a struct layout or a signature changes (200: nrf_net_t carries the LayerNorm parameters); a binding
  * compares nrf_version() with the NRF_VERSION it was written against before passing structs */
-#define NRF_VERSION 230
+#define NRF_VERSION 240
 #define NRF_MAX_D 16
 
 typedef enum {
@@ -35,6 +35,9 @@ typedef enum {
     NRF_ERR_UNSUPPORTED = 2, /* shape outside what the kernels are built for */
     NRF_ERR_LAUNCH = 3       /* HIP reported an error at launch */
 } nrf_status;
+
+/* element types of the entry points that take more than f32 */
+typedef enum { NRF_F32 = 0, NRF_BF16 = 1, NRF_F16 = 2 } nrf_dtype;
 
 int nrf_version(void);
 const char *nrf_last_error_string(void);
@@ -372,6 +375,24 @@ int nrf_sample_fine(const float *z_vals, const float *weights, int64_t n_rays, i
 /* sample_pdf alone -- sampling.py:5-60.  bins [N, nb], weights [N, nb-1] -> samples [N, n_samples]. */
 int nrf_sample_pdf(const float *bins, const float *weights, int64_t n_rows, int32_t n_bins, int32_t n_samples,
                    const float *u, float *samples, void *stream);
+
+/* ---- learned codes (no counterpart in the reference: one vector per training image or frame, per hashed grid corner, ...;
+ * an encoding like A1, but learned) ----
+ * A table of n_rows rows of `dim` elements (dtype: NRF_F32, NRF_BF16 or NRF_F16), row r at table + r * table_stride elements.
+ * ids [n] int32 or int64 (ids_are_64).  dim <= 32768, n and n_rows < 2^31 - 1, n * dim < 2^33.
+ * out [n, dim] = scale * table[ids], computed in f32 and rounded once; out_dtype: the table's type, or f32.
+ * An id outside [0, n_rows) gives a row of NaN. */
+int nrf_lookup_fwd(const void *table, int64_t table_stride, int32_t dtype, int64_t n_rows, int32_t dim, const void *ids,
+                   int32_t ids_are_64, int64_t n, float scale, void *out, int32_t out_dtype, void *stream);
+
+/* grad [n_rows, dim] (dtype: the table's type) = scale * sum over the i with ids[i] == row of g_out[i]; every row is written,
+ * rows that no id names with zeros.  g_out: row i at g_out + i * g_stride elements, of the table's type or f32.  Ids outside
+ * the table and `padding_idx` (-1: none) take no part.  Sums in f32, in an order that depends on the ids and sizes alone:
+ * repeated calls agree bit for bit.  workspace: nrf_lookup_bwd_workspace_bytes (-1: unsupported), 16-byte aligned. */
+int64_t nrf_lookup_bwd_workspace_bytes(int64_t n, int64_t n_rows, int32_t dim);
+int nrf_lookup_bwd(const void *g_out, int64_t g_stride, int32_t g_dtype, const void *ids, int32_t ids_are_64, int64_t n,
+                   int64_t n_rows, int32_t dim, float scale, int64_t padding_idx, void *grad, int32_t dtype, void *workspace,
+                   void *stream);
 
 #ifdef __cplusplus
 }

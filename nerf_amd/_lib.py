@@ -30,7 +30,7 @@ class NrfEmbed(C.Structure):
 
 
 _lib = None
-ABI_VERSION = 230     # include/nrf.h NRF_VERSION
+ABI_VERSION = 240     # include/nrf.h NRF_VERSION
 
 _SIGS = {
     "nrf_version": (C.c_int, []),
@@ -119,6 +119,11 @@ _SIGS = {
     "nrf_composite_bwd": (C.c_int, [vp, vp, vp, C.c_int32, C.c_int64, C.c_int32, vp, C.c_int32, vp, vp, vp, vp, vp,
                                     vp]),
     "nrf_sample_fine": (C.c_int, [vp, vp, C.c_int64, C.c_int32, C.c_int32, vp, vp, vp, vp, vp]),
+    "nrf_lookup_fwd": (C.c_int, [vp, C.c_int64, C.c_int32, C.c_int64, C.c_int32, vp, C.c_int32, C.c_int64, C.c_float, vp,
+                                 C.c_int32, vp]),
+    "nrf_lookup_bwd_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32]),
+    "nrf_lookup_bwd": (C.c_int, [vp, C.c_int64, C.c_int32, vp, C.c_int32, C.c_int64, C.c_int64, C.c_int32, C.c_float, C.c_int64,
+                                 vp, C.c_int32, vp, vp]),
     "nrf_sample_pdf": (C.c_int, [vp, vp, C.c_int64, C.c_int32, C.c_int32, vp, vp, vp]),
 }
 

@@ -1,0 +1,605 @@
+// Code tables: out[i] = scale * table[ids[i]] and its gradient grad[v] = scale * sum of g[i] over the i with ids[i] = v.
+//
+// Forward: every output element is one load, one product, one store; HBM-bound.  The output is cut into chunks of up to 16
+// bytes, consecutive lanes on consecutive chunks, so narrow rows (two features) and wide ones take the same path.
+//
+// Gradient: the sum over equal ids is taken in a fixed order (no float atomics: results repeat bit for bit).
+//   1. a stable sort of the pairs (id, position): least significant digit first, digits of up to 11 bits.  The blocks of the
+//      first launch that do not sort write the zeros of the dense gradient meanwhile.
+//   2. the sorted list is cut into tiles of T tokens; a team of lanes owns a tile and up to 64 vectors of columns, gathers the
+//      tokens' rows and adds runs of equal ids in f32 registers.  A run inside the tile goes straight to its row of grad; one
+//      that reaches beyond an end of it leaves a partial sum (at most two per tile).
+//   3. the team whose tile a crossing run starts in adds up the run's partial sums.
+// Any distribution of ids costs the same in 2, and a run of n tokens costs n / T partial sums in 3.
+#include "nrf_types.h"
+
+using namespace nrf;
+
+namespace {
+
+constexpr int kMaxDim = 32768;
+
+// ---------------------------------------------------------------------------------------------------- forward
+constexpr int kFwdUnroll = 4;
+
+// blockDim 256; chunk = VW elements of one row; `per_row` = dim / VW; magic = ceil(2^32 / per_row)
+template <typename T, typename O, int VW, typename I>
+__global__ void __launch_bounds__(256) lookup_fwd_kernel(const T *__restrict__ table, int64_t stride, int64_t n_rows,
+                                                         const I *__restrict__ ids, int64_t chunks, uint32_t per_row,
+                                                         uint32_t magic, float scale, O *__restrict__ out) {
+    const int64_t c0 = (int64_t)blockIdx.x * (256 * kFwdUnroll);
+    const int64_t r0 = c0 / per_row;                       // block-uniform: one 64-bit division a block
+    const uint32_t rem = (uint32_t)(c0 - r0 * per_row);
+    Pack<T, VW> v[kFwdUnroll];
+    bool ok[kFwdUnroll];
+#pragma unroll
+    for (int u = 0; u < kFwdUnroll; ++u) {
+        const uint32_t local = u * 256 + threadIdx.x;
+        ok[u] = false;
+        if (c0 + local < chunks) {
+            const uint32_t off = rem + local;
+            // off < per_row + 1024 and per_row <= 32768: off * per_row < 2^32, where the product with the magic is exact
+            const uint32_t q = per_row == 1 ? off : __umulhi(off, magic);
+            const int64_t id = (int64_t)ids[r0 + q];
+            ok[u] = (uint64_t)id < (uint64_t)n_rows;
+            if (ok[u]) v[u] = *reinterpret_cast<const Pack<T, VW> *>(table + id * stride + (int64_t)(off - q * per_row) * VW);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kFwdUnroll; ++u) {
+        const int64_t c = c0 + u * 256 + threadIdx.x;
+        if (c < chunks) {
+            Pack<O, VW> o;
+#pragma unroll
+            for (int j = 0; j < VW; ++j) o.e[j] = from_f32<O>(ok[u] ? to_f32(v[u].e[j]) * scale : __uint_as_float(0x7fc00000u));
+            *reinterpret_cast<Pack<O, VW> *>(out + c * VW) = o;
+        }
+    }
+}
+
+template <typename T, typename O, int VW>
+void launch_fwd(const void *table, int64_t stride, int64_t n_rows, const void *ids, bool i64, int64_t n, int dim, float scale,
+                void *out, hipStream_t s) {
+    const uint32_t per_row = (uint32_t)(dim / VW);
+    const uint32_t magic = (uint32_t)(((1ull << 32) + per_row - 1) / per_row);
+    const int64_t chunks = n * per_row;
+    const int blocks = (int)((chunks + 256 * kFwdUnroll - 1) / (256 * kFwdUnroll));
+    if (i64)
+        lookup_fwd_kernel<T, O, VW, int64_t><<<blocks, 256, 0, s>>>((const T *)table, stride, n_rows, (const int64_t *)ids, chunks,
+                                                                    per_row, magic, scale, (O *)out);
+    else
+        lookup_fwd_kernel<T, O, VW, int32_t><<<blocks, 256, 0, s>>>((const T *)table, stride, n_rows, (const int32_t *)ids, chunks,
+                                                                    per_row, magic, scale, (O *)out);
+}
+
+template <typename T, typename O>
+void pick_fwd(int vw, const void *table, int64_t stride, int64_t n_rows, const void *ids, bool i64, int64_t n, int dim,
+              float scale, void *out, hipStream_t s) {
+    if constexpr (sizeof(T) == 2)
+        if (vw == 8) return launch_fwd<T, O, 8>(table, stride, n_rows, ids, i64, n, dim, scale, out, s);
+    if (vw >= 4) return launch_fwd<T, O, 4>(table, stride, n_rows, ids, i64, n, dim, scale, out, s);
+    if (vw == 2) return launch_fwd<T, O, 2>(table, stride, n_rows, ids, i64, n, dim, scale, out, s);
+    launch_fwd<T, O, 1>(table, stride, n_rows, ids, i64, n, dim, scale, out, s);
+}
+
+// ---------------------------------------------------------------------------------------------------- sort of (id, position)
+// Pair: x = key (the id; n_rows for tokens that take no part: ids outside the table, the padding id), y = position.
+constexpr int kItems = 16;                  // items of a thread
+constexpr int kTile = 256 * kItems;         // items of a block, many-block sort
+constexpr int kSmall = 1024 * kItems;       // most items the one-block sort takes
+constexpr int kMaxDigit = 11;               // bits of a digit, many-block sort (2048 bins)
+constexpr int kSmallDigit = 10;             // bits of a digit, one-block sort: 16 waves' counters + the pairs fit LDS
+
+template <typename I>
+__device__ __forceinline__ uint32_t key_of(I id, uint32_t n_rows, int64_t padding) {
+    const int64_t v = (int64_t)id;
+    return (uint64_t)v < (uint64_t)n_rows && v != padding ? (uint32_t)v : n_rows;
+}
+
+// Lanes of the wave that hold the same digit (inactive lanes: never counted)
+__device__ __forceinline__ uint64_t same_digit(uint32_t d, int bits, bool active) {
+    uint64_t m = __ballot(active);
+    for (int b = 0; b < bits; ++b) {
+        const bool one = (d >> b) & 1;
+        const uint64_t w = __ballot(one);
+        m &= one ? w : ~w;
+    }
+    return m;
+}
+
+__device__ __forceinline__ int lanes_below(uint64_t m) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
+
+// Rank of an item among the items of its digit that this wave saw before it; moves the wave's counter (one leader a digit).
+// The counter is read by all lanes of the digit before the leader writes it: one wave, LDS accesses in order.
+__device__ __forceinline__ uint32_t wave_rank(uint16_t *cnt, uint32_t d, int bits, bool active) {
+    const uint64_t m = same_digit(d, bits, active);
+    uint32_t r = 0;
+    if (active) {
+        const int below = lanes_below(m);
+        const uint32_t c = *(volatile uint16_t *)&cnt[d];
+        r = c + below;
+        __builtin_amdgcn_wave_barrier();
+        if (below == 0) *(volatile uint16_t *)&cnt[d] = (uint16_t)(c + __popcll(m));
+    }
+    __builtin_amdgcn_wave_barrier();
+    return r;
+}
+
+// Exclusive scan of one value a thread over the block (WAVES waves); `sums`: WAVES words of LDS.
+template <int WAVES>
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *sums) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t x = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    if (lane == 63) sums[wave] = x;
+    __syncthreads();
+    uint32_t base = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+        if (w < wave) base += sums[w];
+    __syncthreads();
+    return base + x - v;
+}
+
+// Zeros of the dense gradient, by the blocks of a launch that do not sort: block `b` of `blocks`.
+__device__ __forceinline__ void fill_zero(void *p, int64_t bytes, int b, int blocks) {
+    const int64_t step = (int64_t)blocks * blockDim.x, first = (int64_t)b * blockDim.x + threadIdx.x;
+    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        uint4 *q = reinterpret_cast<uint4 *>(p);
+        const int64_t n = bytes >> 4;
+        for (int64_t i = first; i < n; i += step) q[i] = make_uint4(0, 0, 0, 0);
+        if (first == 0)
+            for (int64_t i = n << 4; i < bytes; i += 2) *reinterpret_cast<uint16_t *>((char *)p + i) = 0;
+    } else {
+        for (int64_t i = first; i < (bytes >> 1); i += step) reinterpret_cast<uint16_t *>(p)[i] = 0;
+    }
+}
+
+// One block sorts up to kSmall pairs in LDS; a pass ranks by waves (items in order: wave, item, lane), then moves the pairs.
+struct SmallSort {
+    uint32_t key[kSmall];
+    uint16_t pos[kSmall];
+    uint16_t cnt[16][1 << kSmallDigit];
+    uint32_t sums[16];
+};
+
+template <typename I>
+__global__ void __launch_bounds__(1024) sort_small_kernel(const I *__restrict__ ids, int n, uint32_t n_rows, int64_t padding,
+                                                          int passes, int digit, uint2 *__restrict__ pairs, void *grad,
+                                                          int64_t grad_bytes) {
+    if (blockIdx.x > 0) return fill_zero(grad, grad_bytes, blockIdx.x - 1, gridDim.x - 1);
+    __shared__ SmallSort s;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int bins = 1 << digit;
+    // waves own consecutive ranges of `per` items (a multiple of 64), item k of a lane at wave * per + k * 64 + lane
+    const int rounds = (n + 1023) / 1024, per = rounds * 64;
+    uint32_t key[kItems], rank[kItems];
+    uint16_t pos[kItems];
+    for (int k = 0; k < kItems; ++k) {
+        const int i = wave * per + k * 64 + lane;
+        if (k < rounds && i < n) {
+            key[k] = key_of(ids[i], n_rows, padding);
+            pos[k] = (uint16_t)i;
+        }
+    }
+    for (int p = 0; p < passes; ++p) {
+        for (int b = tid; b < 16 * bins; b += 1024) s.cnt[b >> digit][b & (bins - 1)] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kItems; ++k)
+            if (k < rounds) {
+                const bool on = wave * per + k * 64 + lane < n;
+                rank[k] = wave_rank(s.cnt[wave], on ? (key[k] >> (p * digit)) & (bins - 1) : 0, digit, on);
+            }
+        __syncthreads();
+        // counters -> first place of (digit, wave); digits in order, waves in order inside a digit
+        uint32_t total = 0;
+        if (tid < bins)
+            for (int w = 0; w < 16; ++w) total += s.cnt[w][tid];
+        uint32_t base = block_scan<16>(total, s.sums);
+        if (tid < bins)
+            for (int w = 0; w < 16; ++w) {
+                const uint32_t c = s.cnt[w][tid];
+                s.cnt[w][tid] = (uint16_t)base;          // places are below kSmall <= 2^14
+                base += c;
+            }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kItems; ++k)
+            if (k < rounds && wave * per + k * 64 + lane < n) {
+                const uint32_t at = s.cnt[wave][(key[k] >> (p * digit)) & (bins - 1)] + rank[k];
+                s.key[at] = key[k];
+                s.pos[at] = pos[k];
+            }
+        __syncthreads();
+        if (p + 1 < passes) {
+#pragma unroll
+            for (int k = 0; k < kItems; ++k) {
+                const int i = wave * per + k * 64 + lane;
+                if (k < rounds && i < n) {
+                    key[k] = s.key[i];
+                    pos[k] = s.pos[i];
+                }
+            }
+        }
+    }
+    for (int i = tid; i < n; i += 1024) pairs[i] = make_uint2(s.key[i], s.pos[i]);
+}
+
+// Many blocks, one digit: counts[bin][block]; the blocks behind the sorting ones write zeros (first digit only).
+template <typename I, bool FIRST>
+__global__ void __launch_bounds__(256) sort_count_kernel(const I *__restrict__ ids, const uint2 *__restrict__ in, int64_t n,
+                                                         uint32_t n_rows, int64_t padding, int shift, int digit, int tiles,
+                                                         uint32_t *__restrict__ counts, void *grad, int64_t grad_bytes) {
+    if (FIRST && (int)blockIdx.x >= tiles) return fill_zero(grad, grad_bytes, blockIdx.x - tiles, gridDim.x - tiles);
+    __shared__ uint32_t cnt[1 << kMaxDigit];
+    const int bins = 1 << digit;
+    for (int b = threadIdx.x; b < bins; b += 256) cnt[b] = 0;
+    __syncthreads();
+    const int64_t i0 = (int64_t)blockIdx.x * kTile;
+#pragma unroll 4
+    for (int k = 0; k < kItems; ++k) {
+        const int64_t i = i0 + k * 256 + threadIdx.x;
+        if (i < n) {
+            const uint32_t key = FIRST ? key_of(ids[i], n_rows, padding) : in[i].x;
+            atomicAdd(&cnt[(key >> shift) & (bins - 1)], 1u);
+        }
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += 256) counts[(int64_t)b * tiles + blockIdx.x] = cnt[b];
+}
+
+// One wave a bin: counts[bin][*] -> exclusive sums over the blocks, totals[bin].
+__global__ void __launch_bounds__(256) sort_scan_kernel(uint32_t *__restrict__ counts, uint32_t *__restrict__ totals, int bins,
+                                                        int tiles) {
+    const int lane = threadIdx.x & 63, bin = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (bin >= bins) return;
+    uint32_t *c = counts + (int64_t)bin * tiles;
+    uint32_t carry = 0;
+    for (int t = 0; t < tiles; t += 64) {
+        const uint32_t v = t + lane < tiles ? c[t + lane] : 0;
+        uint32_t x = v;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t y = __shfl_up(x, d);
+            if (lane >= d) x += y;
+        }
+        if (t + lane < tiles) c[t + lane] = carry + x - v;
+        carry += __shfl(x, 63);
+    }
+    if (lane == 0) totals[bin] = carry;
+}
+
+template <typename I, bool FIRST>
+__global__ void __launch_bounds__(256) sort_scatter_kernel(const I *__restrict__ ids, const uint2 *__restrict__ in, int64_t n,
+                                                           uint32_t n_rows, int64_t padding, int shift, int digit, int tiles,
+                                                           const uint32_t *__restrict__ counts,
+                                                           const uint32_t *__restrict__ totals, uint2 *__restrict__ out) {
+    __shared__ uint32_t base[1 << kMaxDigit];
+    __shared__ uint16_t cnt[4][1 << kMaxDigit];
+    __shared__ uint32_t sums[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int bins = 1 << digit;
+    for (int b = tid; b < 4 * bins; b += 256) cnt[b >> digit][b & (bins - 1)] = 0;
+    // first place of each bin: exclusive sum of the totals, `each` consecutive bins a thread
+    const int each = (bins + 255) / 256;
+    uint32_t mine = 0;
+    for (int j = 0; j < each; ++j)
+        if (tid * each + j < bins) mine += totals[tid * each + j];
+    uint32_t at = block_scan<4>(mine, sums);
+    for (int j = 0; j < each; ++j) {
+        const int b = tid * each + j;
+        if (b < bins) {
+            base[b] = at + counts[(int64_t)b * tiles + blockIdx.x];
+            at += totals[b];
+        }
+    }
+    const int64_t i0 = (int64_t)blockIdx.x * kTile + wave * (64 * kItems);
+    uint2 pair[kItems];
+    uint32_t rank[kItems];
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+        const int64_t i = i0 + k * 64 + lane;
+        pair[k] = make_uint2(0, 0);
+        if (i < n) pair[k] = FIRST ? make_uint2(key_of(ids[i], n_rows, padding), (uint32_t)i) : in[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kItems; ++k)
+        rank[k] = wave_rank(cnt[wave], (pair[k].x >> shift) & (bins - 1), digit, i0 + k * 64 + lane < n);
+    __syncthreads();
+    for (int b = tid; b < bins; b += 256) {
+        uint32_t sum = 0;
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t c = cnt[w][b];
+            cnt[w][b] = (uint16_t)sum;
+            sum += c;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kItems; ++k)
+        if (i0 + k * 64 + lane < n) {
+            const uint32_t d = (pair[k].x >> shift) & (bins - 1);
+            out[(int64_t)base[d] + cnt[wave][d] + rank[k]] = pair[k];
+        }
+}
+
+// ---------------------------------------------------------------------------------------------------- sums over runs of equal ids
+struct SumArgs {
+    const uint2 *pairs;
+    const void *g;
+    int64_t g_stride;
+    void *grad;
+    float *head, *tail;        // [tiles][dim]: partial sum of a run that began before the tile / that begins in it and goes on
+    int64_t n;
+    uint32_t n_rows;
+    int dim, tile, lanes;      // lanes: of a team, a power of two <= 64
+    float scale;
+};
+
+constexpr int kBatch = 8;      // rows of g that a team has in flight
+
+template <typename G, typename T, int VW>
+__device__ __forceinline__ void store_row(const SumArgs &a, uint32_t key, int col, const float *acc) {
+    Pack<T, VW> o;
+#pragma unroll
+    for (int j = 0; j < VW; ++j) o.e[j] = from_f32<T>(acc[j] * a.scale);
+    *reinterpret_cast<Pack<T, VW> *>((T *)a.grad + (int64_t)key * a.dim + col) = o;
+}
+
+template <int VW>
+__device__ __forceinline__ void store_part(float *p, int64_t tile, int dim, int col, const float *acc) {
+#pragma unroll
+    for (int j = 0; j < VW; ++j) p[tile * dim + col + j] = acc[j];
+}
+
+template <typename G, typename T, int VW>
+__global__ void __launch_bounds__(256) sum_tiles_kernel(const SumArgs a) {
+    const int lane = threadIdx.x & (a.lanes - 1);
+    const int64_t t = (int64_t)blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
+    const int col = ((int)blockIdx.y * a.lanes + lane) * VW;
+    const int64_t i0 = t * a.tile;
+    if (i0 >= a.n || col >= a.dim) return;
+    const int64_t i1 = i0 + a.tile < a.n ? i0 + a.tile : a.n;
+    const G *g = (const G *)a.g + col;
+    uint32_t cur = a.pairs[i0].x;
+    if (cur >= a.n_rows) return;                           // sorted: nothing but tokens that take no part from here on
+    bool before = i0 > 0 && a.pairs[i0 - 1].x == cur;
+    float acc[VW];
+#pragma unroll
+    for (int j = 0; j < VW; ++j) acc[j] = 0.0f;
+    for (int64_t i = i0; i < i1; i += kBatch) {
+        uint2 p[kBatch];
+        Pack<G, VW> v[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) p[k] = i + k < i1 ? a.pairs[i + k] : make_uint2(~0u, 0);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+            if (p[k].x < a.n_rows) v[k] = *reinterpret_cast<const Pack<G, VW> *>(g + (int64_t)p[k].y * a.g_stride);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            if (i + k >= i1) break;
+            if (p[k].x != cur) {
+                if (before) store_part<VW>(a.head, t, a.dim, col, acc);
+                else store_row<G, T, VW>(a, cur, col, acc);
+                cur = p[k].x;
+                before = false;
+                if (cur >= a.n_rows) return;
+#pragma unroll
+                for (int j = 0; j < VW; ++j) acc[j] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < VW; ++j) acc[j] += to_f32(v[k].e[j]);
+        }
+    }
+    if (before) store_part<VW>(a.head, t, a.dim, col, acc);
+    else if (i1 < a.n && a.pairs[i1].x == cur) store_part<VW>(a.tail, t, a.dim, col, acc);
+    else store_row<G, T, VW>(a, cur, col, acc);
+}
+
+// Runs that cross tiles: the team of the tile a run starts in adds tail[tile] and head[tile + 1 ..].
+template <typename G, typename T, int VW>
+__global__ void __launch_bounds__(256) sum_join_kernel(const SumArgs a) {
+    const int lane = threadIdx.x & (a.lanes - 1);
+    const int64_t t = (int64_t)blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
+    const int col = ((int)blockIdx.y * a.lanes + lane) * VW;
+    const int64_t i0 = t * a.tile, i1 = i0 + a.tile;
+    if (i1 >= a.n || col >= a.dim) return;
+    const uint32_t cur = a.pairs[i1 - 1].x;
+    if (cur >= a.n_rows || a.pairs[i1].x != cur || (i0 > 0 && a.pairs[i0 - 1].x == cur)) return;
+    float acc[VW];
+#pragma unroll
+    for (int j = 0; j < VW; ++j) acc[j] = a.tail[t * a.dim + col + j];
+    const int64_t tiles = (a.n + a.tile - 1) / a.tile;
+    // the run's tiles are those whose first token carries its id: batches of loads, the first other id ends it
+    for (int64_t s = t + 1; s < tiles; s += kBatch) {
+        bool in[kBatch];
+        float v[kBatch][VW];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) in[k] = s + k < tiles && a.pairs[(s + k) * a.tile].x == cur;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+            if (in[k])
+#pragma unroll
+                for (int j = 0; j < VW; ++j) v[k][j] = a.head[(s + k) * a.dim + col + j];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+            if (in[k])
+#pragma unroll
+                for (int j = 0; j < VW; ++j) acc[j] += v[k][j];
+        if (!in[kBatch - 1]) break;
+    }
+    store_row<G, T, VW>(a, cur, col, acc);
+}
+
+// ---------------------------------------------------------------------------------------------------- host
+struct BwdPlan {
+    int passes, digit;         // of the sort
+    int64_t sort_tiles;        // blocks of the many-block sort (0: one block)
+    int tile;                  // tokens of a sum tile
+    int64_t sum_tiles;
+    int64_t off_a, off_b, off_counts, off_totals, off_head, off_tail, bytes;
+};
+
+BwdPlan plan_bwd(int64_t n, int64_t n_rows, int dim) {
+    BwdPlan p;
+    int bits = 1;
+    while (bits < 32 && (n_rows >> bits) != 0) ++bits;     // keys go up to n_rows itself
+    const int most = n <= kSmall ? kSmallDigit : kMaxDigit;
+    p.passes = (bits + most - 1) / most;
+    p.digit = (bits + p.passes - 1) / p.passes;
+    p.sort_tiles = n <= kSmall ? 0 : (n + kTile - 1) / kTile;
+    // enough teams to fill the chip (16 waves on each of 256 CUs), yet tiles long enough that few runs cross them
+    p.tile = 64;
+    const int64_t vectors = (dim + 3) / 4;
+    while (p.tile > kBatch && n * vectors / p.tile < 256 * 16 * 64) p.tile >>= 1;
+    p.sum_tiles = (n + p.tile - 1) / p.tile;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
+    p.off_a = take(n * 8);
+    p.off_b = p.passes > 1 && p.sort_tiles ? take(n * 8) : 0;
+    p.off_counts = take(p.sort_tiles * (4 << p.digit));
+    p.off_totals = take(p.sort_tiles ? (4 << p.digit) : 0);
+    p.off_head = take(p.sum_tiles * dim * 4);
+    p.off_tail = take(p.sum_tiles * dim * 4);
+    p.bytes = at;
+    return p;
+}
+
+template <typename I>
+const uint2 *sort_pairs(const BwdPlan &p, const I *ids, int64_t n, int64_t n_rows, int64_t padding, char *ws, void *grad,
+                        int64_t grad_bytes, hipStream_t s) {
+    const int fill = grid_for(grad_bytes, 1 << 16, 2048);       // at least 64 KB of zeros a block
+    uint2 *a = (uint2 *)(ws + p.off_a), *b = (uint2 *)(ws + p.off_b);
+    if (p.sort_tiles == 0) {
+        sort_small_kernel<I><<<1 + fill, 1024, 0, s>>>(ids, (int)n, (uint32_t)n_rows, padding, p.passes, p.digit,
+                                                                       a, grad, grad_bytes);
+        return a;
+    }
+    uint32_t *counts = (uint32_t *)(ws + p.off_counts), *totals = (uint32_t *)(ws + p.off_totals);
+    const int tiles = (int)p.sort_tiles, bins = 1 << p.digit;
+    const uint2 *in = nullptr;
+    uint2 *out = p.passes % 2 ? a : b;                          // the last pass ends in a
+    for (int d = 0; d < p.passes; ++d) {
+        if (d == 0)
+            sort_count_kernel<I, true><<<tiles + fill, 256, 0, s>>>(ids, nullptr, n, (uint32_t)n_rows, padding, 0, p.digit, tiles,
+                                                                    counts, grad, grad_bytes);
+        else
+            sort_count_kernel<I, false><<<tiles, 256, 0, s>>>(ids, in, n, (uint32_t)n_rows, padding, d * p.digit, p.digit, tiles,
+                                                              counts, nullptr, 0);
+        sort_scan_kernel<<<(bins + 3) / 4, 256, 0, s>>>(counts, totals, bins, tiles);
+        if (d == 0)
+            sort_scatter_kernel<I, true><<<tiles, 256, 0, s>>>(ids, nullptr, n, (uint32_t)n_rows, padding, 0, p.digit, tiles,
+                                                               counts, totals, out);
+        else
+            sort_scatter_kernel<I, false><<<tiles, 256, 0, s>>>(ids, in, n, (uint32_t)n_rows, padding, d * p.digit, p.digit, tiles,
+                                                                counts, totals, out);
+        in = out;
+        out = out == a ? b : a;
+    }
+    return in;
+}
+
+template <typename G, typename T, int VW>
+void launch_sums(SumArgs a, const BwdPlan &p, hipStream_t s) {
+    const int vectors = (a.dim + VW - 1) / VW;
+    a.lanes = 1;
+    while (a.lanes < 64 && a.lanes < vectors) a.lanes <<= 1;
+    const int teams = 256 / a.lanes;
+    const dim3 grid((unsigned)((p.sum_tiles + teams - 1) / teams), (unsigned)((vectors + a.lanes - 1) / a.lanes));
+    sum_tiles_kernel<G, T, VW><<<grid, 256, 0, s>>>(a);
+    sum_join_kernel<G, T, VW><<<grid, 256, 0, s>>>(a);
+}
+
+template <typename G, typename T>
+void pick_sums(int vw, const SumArgs &a, const BwdPlan &p, hipStream_t s) {
+    if constexpr (sizeof(G) == 2 && sizeof(T) == 2)
+        if (vw == 8) return launch_sums<G, T, 8>(a, p, s);
+    if (vw >= 4) return launch_sums<G, T, 4>(a, p, s);
+    if (vw == 2) return launch_sums<G, T, 2>(a, p, s);
+    launch_sums<G, T, 1>(a, p, s);
+}
+
+// the wider side's 16 bytes set the vector; both sides' addresses must be aligned to their share of it
+int common_width(int dim, int esz_a, uint64_t addr_a, int esz_b, uint64_t addr_b) {
+    const int a = vector_width(dim, esz_a, addr_a), b = vector_width(dim, esz_b, addr_b);
+    return a < b ? a : b;
+}
+
+bool pair_ok(int32_t narrow, int32_t wide) { return narrow == wide || (wide == NRF_F32 && dtype_size(narrow) == 2); }
+
+}  // namespace
+
+extern "C" int nrf_lookup_fwd(const void *table, int64_t table_stride, int32_t dtype, int64_t n_rows, int32_t dim,
+                              const void *ids, int32_t ids_are_64, int64_t n, float scale, void *out, int32_t out_dtype,
+                              void *stream) {
+    NRF_REQUIRE(n >= 0 && n_rows >= 0 && dim >= 1, "nrf_lookup_fwd: n %lld, n_rows %lld, dim %d", (long long)n, (long long)n_rows, dim);
+    NRF_REQUIRE(dtype_size(dtype) && dtype_size(out_dtype), "nrf_lookup_fwd: dtype %d, out_dtype %d", dtype, out_dtype);
+    if (!pair_ok(dtype, out_dtype))
+        return fail(NRF_ERR_UNSUPPORTED, "nrf_lookup_fwd: out must have the table's type or f32");
+    if (dim > kMaxDim || n > INT32_MAX || n_rows >= INT32_MAX || (n * dim) >> 33)
+        return fail(NRF_ERR_UNSUPPORTED, "nrf_lookup_fwd: dim at most %d, n and n_rows below 2^31, n * dim below 2^33", kMaxDim);
+    if (n == 0) return NRF_OK;
+    NRF_REQUIRE(ids && out && (table || n_rows == 0), "nrf_lookup_fwd: null pointer");
+    NRF_REQUIRE(table_stride >= dim, "nrf_lookup_fwd: table_stride %lld below dim %d", (long long)table_stride, dim);
+    const int es = dtype_size(dtype), eo = dtype_size(out_dtype);
+    const int vw = common_width(dim, es, (uint64_t)(uintptr_t)table | (uint64_t)table_stride * es, eo, (uint64_t)(uintptr_t)out);
+    hipStream_t s = as_stream(stream);
+    const bool i64 = ids_are_64 != 0;
+    if (dtype == NRF_F32) pick_fwd<float, float>(vw, table, table_stride, n_rows, ids, i64, n, dim, scale, out, s);
+    else if (dtype == NRF_BF16 && out_dtype == NRF_BF16) pick_fwd<bf16_t, bf16_t>(vw, table, table_stride, n_rows, ids, i64, n, dim, scale, out, s);
+    else if (dtype == NRF_BF16) pick_fwd<bf16_t, float>(vw, table, table_stride, n_rows, ids, i64, n, dim, scale, out, s);
+    else if (out_dtype == NRF_F16) pick_fwd<f16_t, f16_t>(vw, table, table_stride, n_rows, ids, i64, n, dim, scale, out, s);
+    else pick_fwd<f16_t, float>(vw, table, table_stride, n_rows, ids, i64, n, dim, scale, out, s);
+    return check_launch("nrf_lookup_fwd");
+}
+
+static int bwd_shape(int64_t n, int64_t n_rows, int32_t dim) {
+    NRF_REQUIRE(n >= 0 && n_rows >= 0 && dim >= 1, "nrf_lookup_bwd: n %lld, n_rows %lld, dim %d", (long long)n, (long long)n_rows, dim);
+    if (dim > kMaxDim || n > INT32_MAX || n_rows >= INT32_MAX || (n * dim) >> 33)
+        return fail(NRF_ERR_UNSUPPORTED, "nrf_lookup_bwd: dim at most %d, n and n_rows below 2^31, n * dim below 2^33", kMaxDim);
+    return NRF_OK;
+}
+
+extern "C" int64_t nrf_lookup_bwd_workspace_bytes(int64_t n, int64_t n_rows, int32_t dim) {
+    return bwd_shape(n, n_rows, dim) == NRF_OK ? plan_bwd(n, n_rows, dim).bytes : -1;
+}
+
+extern "C" int nrf_lookup_bwd(const void *g_out, int64_t g_stride, int32_t g_dtype, const void *ids, int32_t ids_are_64, int64_t n,
+                              int64_t n_rows, int32_t dim, float scale, int64_t padding_idx, void *grad, int32_t dtype,
+                              void *workspace, void *stream) {
+    if (int rc = bwd_shape(n, n_rows, dim)) return rc;
+    NRF_REQUIRE(dtype_size(dtype) && dtype_size(g_dtype), "nrf_lookup_bwd: dtype %d, g_dtype %d", dtype, g_dtype);
+    if (!pair_ok(dtype, g_dtype)) return fail(NRF_ERR_UNSUPPORTED, "nrf_lookup_bwd: g_out must have the table's type or f32");
+    if (n_rows == 0) return NRF_OK;
+    NRF_REQUIRE(grad, "nrf_lookup_bwd: null pointer");
+    NRF_REQUIRE(n == 0 || (g_out && ids && workspace), "nrf_lookup_bwd: null pointer");
+    NRF_REQUIRE(n == 0 || g_stride >= dim, "nrf_lookup_bwd: g_stride %lld below dim %d", (long long)g_stride, dim);
+    NRF_REQUIRE(((uintptr_t)workspace & 15) == 0, "nrf_lookup_bwd: workspace must be 16-byte aligned");
+    const BwdPlan p = plan_bwd(n, n_rows, dim);
+    const int eg = dtype_size(g_dtype), es = dtype_size(dtype);
+    const int64_t grad_bytes = n_rows * dim * es;
+    hipStream_t s = as_stream(stream);
+    char *ws = (char *)workspace;
+    SumArgs a;
+    a.pairs = ids_are_64 ? sort_pairs(p, (const int64_t *)ids, n, n_rows, padding_idx, ws, grad, grad_bytes, s)
+                         : sort_pairs(p, (const int32_t *)ids, n, n_rows, padding_idx, ws, grad, grad_bytes, s);
+    if (n > 0) {
+        a.g = g_out, a.g_stride = g_stride, a.grad = grad, a.head = (float *)(ws + p.off_head), a.tail = (float *)(ws + p.off_tail);
+        a.n = n, a.n_rows = (uint32_t)n_rows, a.dim = dim, a.tile = p.tile, a.lanes = 0, a.scale = scale;
+        const int vw = common_width(dim, eg, (uint64_t)(uintptr_t)g_out | (uint64_t)g_stride * eg, es, (uint64_t)(uintptr_t)grad);
+        if (g_dtype == NRF_F32 && dtype == NRF_F32) pick_sums<float, float>(vw, a, p, s);
+        else if (g_dtype == NRF_F32 && dtype == NRF_BF16) pick_sums<float, bf16_t>(vw, a, p, s);
+        else if (g_dtype == NRF_F32) pick_sums<float, f16_t>(vw, a, p, s);
+        else if (g_dtype == NRF_BF16) pick_sums<bf16_t, bf16_t>(vw, a, p, s);
+        else pick_sums<f16_t, f16_t>(vw, a, p, s);
+    }
+    return check_launch("nrf_lookup_bwd");
+}

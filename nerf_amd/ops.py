@@ -161,6 +161,93 @@ def pe_bwd(x, g_out, num_freqs, max_freq_log2, log_sampling=True, include_input=
     return g_x.reshape(x.shape)
 
 
+# ---------------------------------------------------------------- learned codes
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # nrf_dtype
+
+
+def _typed(t, name):
+    """A GPU tensor of one of the element types the library takes; no conversion."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name}: nerf_amd kernels need a GPU tensor (got device {t.device}); there is no CPU path")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return t
+
+
+def _rows(t):
+    """2-D tensor -> (tensor with unit column stride and rows that do not overlap, row stride)."""
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+def _ids(ids, device):
+    if not isinstance(ids, torch.Tensor):
+        raise TypeError("ids: expected a torch.Tensor")
+    if ids.device != device:
+        raise RuntimeError(f"ids: expected a tensor on {device}, got {ids.device}")
+    if ids.dtype != torch.int64 and ids.dtype != torch.int32:
+        raise TypeError(f"ids: expected int32 or int64, got {ids.dtype}")
+    return ids.contiguous()
+
+
+def _call(device, name, *args):
+    """lib.name(*args, stream) with `device` current, on its current stream (the tensors' device need not be the current one)."""
+    fn = getattr(_lib.lib(), name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        check(rc, name)
+
+
+def lookup_fwd(table, ids, scale=1.0, out_dtype=None):
+    """scale * table[ids]: table [V, D] f32 / bf16 / f16 (rows may be strided), ids int32 / int64 of any shape -> [*ids.shape, D]
+    in the table's type or f32.  Ids outside [0, V) give rows of NaN."""
+    _typed(table, "table")
+    if table.dim() != 2 or table.shape[1] < 1:
+        raise ValueError(f"table: expected [rows, dim >= 1], got {tuple(table.shape)}")
+    ids = _ids(ids, table.device)
+    out_dtype = table.dtype if out_dtype is None else out_dtype
+    if out_dtype != table.dtype and out_dtype != torch.float32:
+        raise TypeError(f"out_dtype: expected {table.dtype} or float32, got {out_dtype}")
+    t, stride = _rows(table)
+    V, D = t.shape
+    out = torch.empty((*ids.shape, D), device=t.device, dtype=out_dtype)
+    _call(t.device, "nrf_lookup_fwd", t.data_ptr(), stride, _DTYPES[t.dtype], V, D, ids.data_ptr(), ids.dtype == torch.int64,
+          ids.numel(), float(scale), out.data_ptr(), _DTYPES[out_dtype])
+    return out
+
+
+def lookup_bwd(g_out, ids, n_rows, scale=1.0, padding_idx=None, dtype=None):
+    """Gradient of lookup_fwd w.r.t. its table: [n_rows, D], row v = scale * the sum of g_out over ids == v, in `dtype` (default:
+    g_out's; g_out may be f32 for a 16-bit table).  Ids outside the table and `padding_idx` take no part.  Bit-reproducible."""
+    _typed(g_out, "g_out")
+    ids = _ids(ids, g_out.device)
+    if g_out.dim() < 1 or g_out.shape[:-1] != ids.shape or g_out.shape[-1] < 1:
+        raise ValueError(f"g_out: expected [*{tuple(ids.shape)}, dim >= 1], got {tuple(g_out.shape)}")
+    dtype = g_out.dtype if dtype is None else dtype
+    if dtype not in _DTYPES or (g_out.dtype != dtype and g_out.dtype != torch.float32):
+        raise TypeError(f"dtype {dtype} does not go with a gradient of {g_out.dtype}")
+    n, D, V = ids.numel(), g_out.shape[-1], int(n_rows)
+    pad = -1 if padding_idx is None else int(padding_idx)
+    if padding_idx is not None and not 0 <= pad < V:
+        raise ValueError(f"padding_idx {pad} is outside the table's {V} rows")
+    g, stride = _rows(g_out.reshape(n, D))
+    nbytes = _lib.lib().nrf_lookup_bwd_workspace_bytes(n, V, D)
+    if nbytes < 0:
+        raise RuntimeError("nrf_lookup_bwd_workspace_bytes: " + _lib.lib().nrf_last_error_string().decode())
+    grad = torch.empty((V, D), device=g.device, dtype=dtype)
+    ws = torch.empty((max(nbytes, 1),), device=g.device, dtype=torch.uint8)
+    _call(g.device, "nrf_lookup_bwd", g.data_ptr(), stride, _DTYPES[g.dtype], ids.data_ptr(), ids.dtype == torch.int64, n, V, D,
+          float(scale), pad, grad.data_ptr(), _DTYPES[dtype], ws.data_ptr())
+    return grad
+
+
 # ---------------------------------------------------------------- compositing
 def _dirs(rays_d):
     """rays_d may be a strided view into the [N, ncol] ray matrix; pass (base pointer, row stride)."""
