@@ -394,6 +394,22 @@ int nrf_lookup_bwd(const void *g_out, int64_t g_stride, int32_t g_dtype, const v
                    int64_t n_rows, int32_t dim, float scale, int64_t padding_idx, void *grad, int32_t dtype, void *workspace,
                    void *stream);
 
+/* Indices drawn from rows of logits (sample_pdf's rule for a discrete distribution; no counterpart in the reference).
+ * logits [n_rows, size] (NRF_F32, NRF_BF16 or NRF_F16), row r at logits + r * row_stride elements (0: one row for all);
+ * u [n_rows, n_draws] uniform numbers; ids [n_rows, n_draws] and the probabilities prob [n_rows, n_draws] they were drawn with.
+ * e_i = exp((x_i - max) / temperature).  In falling order of x, ties by rising index, kept are the first top_k entries
+ * (<= 0: all), of those the shortest prefix that holds top_p of their mass (>= 1: all), of those the ones with
+ * e_i >= min_p (<= 0: all); the first entry always.  A draw is the first kept index whose running mass, in the order of the
+ * index, exceeds u times the kept mass.  temperature 0: the first maximum.  Masses and sums are f64.
+ * Each of the four can be given per row (a DEVICE array of n_rows values; NULL: the scalar).
+ * -inf and NaN logits are never drawn; +inf logits share the whole mass.  id -1, prob 0: a row in which nothing can be drawn, a
+ * row whose temperature is negative or not finite or whose top_p or min_p is NaN, a u that is NaN.  u outside [0, 1] is clamped;
+ * a min_p of a row above 1 is taken as 1.  size <= 2^28, n_rows <= 2^21. */
+int nrf_sample_logits(const void *logits, int64_t row_stride, int32_t dtype, int64_t n_rows, int32_t size, int32_t n_draws,
+                      float temperature, int32_t top_k, float top_p, float min_p, const float *temperature_rows,
+                      const int32_t *top_k_rows, const float *top_p_rows, const float *min_p_rows, const float *u, int64_t *ids,
+                      float *prob, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,6 +29,43 @@ def _ptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else C.c_void_p(0)
 
 
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # nrf_dtype
+
+
+def _typed(t, name):
+    """A GPU tensor of one of the element types the library takes; no conversion."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name}: nerf_amd kernels need a GPU tensor (got device {t.device}); there is no CPU path")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return t
+
+
+def _rows(t):
+    """2-D tensor -> (tensor with unit column stride and rows that do not overlap, row stride)."""
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+def _opt(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(device, name, *args):
+    """lib.name(*args, stream) with `device` current, on its current stream (the tensors' device need not be the current one)."""
+    fn = getattr(_lib.lib(), name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        check(rc, name)
+
+
 # ---------------------------------------------------------------- rays
 def _pose_rows(c2w):
     """[>=3, >=4] pose tensor -> (tensor kept alive, row stride) with unit column stride."""
@@ -135,6 +172,52 @@ def sample_pdf(bins, weights, n_samples, u=None):
     return out.reshape(*lead, n_samples)
 
 
+def _per_row(v, name, dtype, lead, device):
+    """(scalar, per-row tensor or None) of a filter given as a number or as one value per row."""
+    if not isinstance(v, torch.Tensor):
+        return v, None
+    if v.device != device:
+        raise RuntimeError(f"{name}: expected a tensor on {device}, got {v.device}")
+    if v.shape != lead:
+        raise ValueError(f"{name}: expected one value per row {tuple(lead)}, got {tuple(v.shape)}")
+    if dtype == torch.int32 and v.dtype != torch.int32:
+        v = v.clamp(0, 2 ** 31 - 1)
+    return 0, v.to(dtype).contiguous()
+
+
+def sample_logits(logits, n_samples, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, u=None):
+    """n_samples indices drawn from each row of `logits` [..., V] (f32 / bf16 / f16) -> (ids [..., n_samples] int64,
+    prob [..., n_samples] f32, the probabilities they were drawn with).  u [..., n_samples]: the uniform numbers to draw by
+    (None: torch.rand).  temperature, top_k, top_p, min_p: numbers, or tensors with one value per row; see nrf_sample_logits."""
+    _typed(logits, "logits")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits: expected [..., V >= 1], got {tuple(logits.shape)}")
+    dev, lead, V, n = logits.device, logits.shape[:-1], logits.shape[-1], int(n_samples)
+    if n < 0:
+        raise ValueError(f"n_samples: {n}")
+    x = logits.reshape(-1, V)
+    if V > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    R = x.shape[0]
+    if u is None:
+        u = torch.rand((*lead, n), device=dev)
+    else:
+        if u.device != dev:
+            raise RuntimeError(f"u: expected a tensor on {dev}, got {u.device}")
+        if u.shape != (*lead, n):
+            raise ValueError(f"u: expected {(*lead, n)}, got {tuple(u.shape)}")
+        u = u.float().contiguous()
+    t, tv = _per_row(temperature, "temperature", torch.float32, lead, dev)
+    k, kv = _per_row(top_k, "top_k", torch.int32, lead, dev)
+    p, pv = _per_row(top_p, "top_p", torch.float32, lead, dev)
+    m, mv = _per_row(min_p, "min_p", torch.float32, lead, dev)
+    ids = torch.empty((*lead, n), device=dev, dtype=torch.int64)
+    prob = torch.empty((*lead, n), device=dev, dtype=torch.float32)
+    _call(dev, "nrf_sample_logits", x.data_ptr(), x.stride(0) if R > 1 else V, _DTYPES[x.dtype], R, V, n, t, min(max(int(k), 0), V), p, m,
+          _opt(tv), _opt(kv), _opt(pv), _opt(mv), u.data_ptr(), ids.data_ptr(), prob.data_ptr())
+    return ids, prob
+
+
 # ---------------------------------------------------------------- positional encoding
 def pe_fwd(x, num_freqs, max_freq_log2, log_sampling=True, include_input=True):
     x = _f32(x, "x")
@@ -162,27 +245,6 @@ def pe_bwd(x, g_out, num_freqs, max_freq_log2, log_sampling=True, include_input=
 
 
 # ---------------------------------------------------------------- learned codes
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # nrf_dtype
-
-
-def _typed(t, name):
-    """A GPU tensor of one of the element types the library takes; no conversion."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name}: expected a torch.Tensor")
-    if not t.is_cuda:
-        raise RuntimeError(f"{name}: nerf_amd kernels need a GPU tensor (got device {t.device}); there is no CPU path")
-    if t.dtype not in _DTYPES:
-        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
-    return t
-
-
-def _rows(t):
-    """2-D tensor -> (tensor with unit column stride and rows that do not overlap, row stride)."""
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
-
-
 def _ids(ids, device):
     if not isinstance(ids, torch.Tensor):
         raise TypeError("ids: expected a torch.Tensor")
@@ -191,18 +253,6 @@ def _ids(ids, device):
     if ids.dtype != torch.int64 and ids.dtype != torch.int32:
         raise TypeError(f"ids: expected int32 or int64, got {ids.dtype}")
     return ids.contiguous()
-
-
-def _call(device, name, *args):
-    """lib.name(*args, stream) with `device` current, on its current stream (the tensors' device need not be the current one)."""
-    fn = getattr(_lib.lib(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
-    if rc:
-        check(rc, name)
 
 
 def lookup_fwd(table, ids, scale=1.0, out_dtype=None):

@@ -1,5 +1,7 @@
 """Hierarchical sampling -- counterpart of the reference's sampling.py:5-60, on the HIP kernel
-nrf_sample_pdf (bit-exact with the reference's CPU path on identical inputs)."""
+nrf_sample_pdf (bit-exact with the reference's CPU path on identical inputs).
+
+`sample_logits` is the same rule for a discrete distribution given by logits: pixels by an error map, classes, tokens."""
 import numpy as np
 import torch
 
@@ -20,3 +22,9 @@ def sample_pdf(bins, weights, N_samples, det=False, pytest=False):
     elif not det:
         u = torch.rand(lead + [N_samples], device=bins.device)
     return ops.sample_pdf(bins, weights, N_samples, u)
+
+
+def sample_logits(logits, N_samples=1, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, u=None):
+    """Indices drawn from softmax(logits / temperature) [..., V] after top-k, top-p and min-p -> (ids, prob), both
+    [..., N_samples]; ops.sample_logits describes the filters and `u`."""
+    return ops.sample_logits(logits, N_samples, temperature, top_k, top_p, min_p, u)
