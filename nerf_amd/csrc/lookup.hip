@@ -4,9 +4,9 @@
 // bytes, consecutive lanes on consecutive chunks, so narrow rows (two features) and wide ones take the same path.
 //
 // Gradient: the sum over equal ids is taken in a fixed order (no float atomics: results repeat bit for bit).
-//   1. a stable sort of the pairs (id, position): least significant digit first, digits of up to 11 bits.  The blocks of the
+//   1. a stable sort of the pairs (id, position): least significant digit first, digits of up to 10 bits.  The blocks of the
 //      first launch that do not sort write the zeros of the dense gradient meanwhile.
-//   2. the sorted list is cut into tiles of T tokens; a team of lanes owns a tile and up to 64 vectors of columns, gathers the
+//   2. the sorted list is cut into tiles of T tokens; a team of threads owns a tile and up to 256 vectors of columns, gathers the
 //      tokens' rows and adds runs of equal ids in f32 registers.  A run inside the tile goes straight to its row of grad; one
 //      that reaches beyond an end of it leaves a partial sum (at most two per tile).
 //   3. the team whose tile a crossing run starts in adds up the run's partial sums.
@@ -31,18 +31,24 @@ __global__ void __launch_bounds__(256) lookup_fwd_kernel(const T *__restrict__ t
     const int64_t r0 = c0 / per_row;                       // block-uniform: one 64-bit division a block
     const uint32_t rem = (uint32_t)(c0 - r0 * per_row);
     Pack<T, VW> v[kFwdUnroll];
-    bool ok[kFwdUnroll];
+    int64_t id[kFwdUnroll];
+    uint32_t col[kFwdUnroll];
+    // loads without branches between them: chunks behind the last one read the last one's row, ids outside the table row 0
 #pragma unroll
     for (int u = 0; u < kFwdUnroll; ++u) {
-        const uint32_t local = u * 256 + threadIdx.x;
-        ok[u] = false;
-        if (c0 + local < chunks) {
-            const uint32_t off = rem + local;
-            // off < per_row + 1024 and per_row <= 32768: off * per_row < 2^32, where the product with the magic is exact
-            const uint32_t q = per_row == 1 ? off : __umulhi(off, magic);
-            const int64_t id = (int64_t)ids[r0 + q];
-            ok[u] = (uint64_t)id < (uint64_t)n_rows;
-            if (ok[u]) v[u] = *reinterpret_cast<const Pack<T, VW> *>(table + id * stride + (int64_t)(off - q * per_row) * VW);
+        uint32_t local = u * 256 + threadIdx.x;
+        if (c0 + local >= chunks) local = (uint32_t)(chunks - 1 - c0);
+        const uint32_t off = rem + local;
+        // off < per_row + 1024 and per_row <= 32768: off * per_row < 2^32, where the product with the magic is exact
+        const uint32_t q = per_row == 1 ? off : __umulhi(off, magic);
+        id[u] = (int64_t)ids[r0 + q];
+        col[u] = (off - q * per_row) * VW;
+    }
+    if (n_rows > 0) {
+#pragma unroll
+        for (int u = 0; u < kFwdUnroll; ++u) {
+            const int64_t r = (uint64_t)id[u] < (uint64_t)n_rows ? id[u] : 0;
+            v[u] = *reinterpret_cast<const Pack<T, VW> *>(table + r * stride + col[u]);
         }
     }
 #pragma unroll
@@ -51,7 +57,8 @@ __global__ void __launch_bounds__(256) lookup_fwd_kernel(const T *__restrict__ t
         if (c < chunks) {
             Pack<O, VW> o;
 #pragma unroll
-            for (int j = 0; j < VW; ++j) o.e[j] = from_f32<O>(ok[u] ? to_f32(v[u].e[j]) * scale : __uint_as_float(0x7fc00000u));
+            for (int j = 0; j < VW; ++j)
+                o.e[j] = from_f32<O>((uint64_t)id[u] < (uint64_t)n_rows ? to_f32(v[u].e[j]) * scale : __uint_as_float(0x7fc00000u));
             *reinterpret_cast<Pack<O, VW> *>(out + c * VW) = o;
         }
     }
@@ -84,11 +91,11 @@ void pick_fwd(int vw, const void *table, int64_t stride, int64_t n_rows, const v
 
 // ---------------------------------------------------------------------------------------------------- sort of (id, position)
 // Pair: x = key (the id; n_rows for tokens that take no part: ids outside the table, the padding id), y = position.
-constexpr int kItems = 16;                  // items of a thread
-constexpr int kTile = 256 * kItems;         // items of a block, many-block sort
+constexpr int kItems = 16;                  // most items of a thread, one-block sort
 constexpr int kSmall = 1024 * kItems;       // most items the one-block sort takes
-constexpr int kMaxDigit = 11;               // bits of a digit, many-block sort (2048 bins)
-constexpr int kSmallDigit = 10;             // bits of a digit, one-block sort: 16 waves' counters + the pairs fit LDS
+constexpr int kTileItems = 4;               // items of a thread, many-block sort: 1024 threads, two blocks fill a CU's waves
+constexpr int kTile = 1024 * kTileItems;    // items of a block
+constexpr int kMaxDigit = 10;               // bits of a digit: 16 waves' counters and the one-block sort's pairs fit LDS
 
 template <typename I>
 __device__ __forceinline__ uint32_t key_of(I id, uint32_t n_rows, int64_t padding) {
@@ -147,17 +154,14 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *sums) {
     return base + x - v;
 }
 
-// Zeros of the dense gradient, by the blocks of a launch that do not sort: block `b` of `blocks`.
-__device__ __forceinline__ void fill_zero(void *p, int64_t bytes, int b, int blocks) {
-    const int64_t step = (int64_t)blocks * blockDim.x, first = (int64_t)b * blockDim.x + threadIdx.x;
-    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-        uint4 *q = reinterpret_cast<uint4 *>(p);
-        const int64_t n = bytes >> 4;
-        for (int64_t i = first; i < n; i += step) q[i] = make_uint4(0, 0, 0, 0);
-        if (first == 0)
-            for (int64_t i = n << 4; i < bytes; i += 2) *reinterpret_cast<uint16_t *>((char *)p + i) = 0;
+// Zeros of the dense gradient, by the blocks of a launch that do not sort: kFill bytes each (blockDim 1024).
+constexpr int kFill = 1024 * 16;
+__device__ __forceinline__ void fill_zero(char *p, int64_t bytes, int b) {
+    const int64_t begin = (int64_t)b * kFill, end = begin + kFill < bytes ? begin + kFill : bytes;
+    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && end - begin == kFill) {
+        reinterpret_cast<uint4 *>(p + begin)[threadIdx.x] = make_uint4(0, 0, 0, 0);
     } else {
-        for (int64_t i = first; i < (bytes >> 1); i += step) reinterpret_cast<uint16_t *>(p)[i] = 0;
+        for (int64_t i = begin + 2 * threadIdx.x; i < end; i += 2048) *reinterpret_cast<uint16_t *>(p + i) = 0;
     }
 }
 
@@ -165,7 +169,7 @@ __device__ __forceinline__ void fill_zero(void *p, int64_t bytes, int b, int blo
 struct SmallSort {
     uint32_t key[kSmall];
     uint16_t pos[kSmall];
-    uint16_t cnt[16][1 << kSmallDigit];
+    uint16_t cnt[16][1 << kMaxDigit];
     uint32_t sums[16];
 };
 
@@ -173,7 +177,7 @@ template <typename I>
 __global__ void __launch_bounds__(1024) sort_small_kernel(const I *__restrict__ ids, int n, uint32_t n_rows, int64_t padding,
                                                           int passes, int digit, uint2 *__restrict__ pairs, void *grad,
                                                           int64_t grad_bytes) {
-    if (blockIdx.x > 0) return fill_zero(grad, grad_bytes, blockIdx.x - 1, gridDim.x - 1);
+    if (blockIdx.x > 0) return fill_zero((char *)grad, grad_bytes, blockIdx.x - 1);
     __shared__ SmallSort s;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int bins = 1 << digit;
@@ -232,103 +236,119 @@ __global__ void __launch_bounds__(1024) sort_small_kernel(const I *__restrict__ 
     for (int i = tid; i < n; i += 1024) pairs[i] = make_uint2(s.key[i], s.pos[i]);
 }
 
-// Many blocks, one digit: counts[bin][block]; the blocks behind the sorting ones write zeros (first digit only).
+// Many blocks, one digit: counts[block][bin]; the blocks behind the sorting ones write zeros (first digit only).
 template <typename I, bool FIRST>
-__global__ void __launch_bounds__(256) sort_count_kernel(const I *__restrict__ ids, const uint2 *__restrict__ in, int64_t n,
-                                                         uint32_t n_rows, int64_t padding, int shift, int digit, int tiles,
-                                                         uint32_t *__restrict__ counts, void *grad, int64_t grad_bytes) {
-    if (FIRST && (int)blockIdx.x >= tiles) return fill_zero(grad, grad_bytes, blockIdx.x - tiles, gridDim.x - tiles);
+__global__ void __launch_bounds__(1024) sort_count_kernel(const I *__restrict__ ids, const uint2 *__restrict__ in, int64_t n,
+                                                          uint32_t n_rows, int64_t padding, int shift, int digit, int tiles,
+                                                          uint32_t *__restrict__ counts, void *grad, int64_t grad_bytes) {
+    if (FIRST && (int)blockIdx.x >= tiles) return fill_zero((char *)grad, grad_bytes, blockIdx.x - tiles);
     __shared__ uint32_t cnt[1 << kMaxDigit];
     const int bins = 1 << digit;
-    for (int b = threadIdx.x; b < bins; b += 256) cnt[b] = 0;
-    __syncthreads();
-    const int64_t i0 = (int64_t)blockIdx.x * kTile;
-#pragma unroll 4
-    for (int k = 0; k < kItems; ++k) {
-        const int64_t i = i0 + k * 256 + threadIdx.x;
-        if (i < n) {
-            const uint32_t key = FIRST ? key_of(ids[i], n_rows, padding) : in[i].x;
-            atomicAdd(&cnt[(key >> shift) & (bins - 1)], 1u);
-        }
+    if ((int)threadIdx.x < bins) cnt[threadIdx.x] = 0;
+    const int64_t i0 = (int64_t)blockIdx.x * kTile + threadIdx.x;
+    uint32_t key[kTileItems];
+#pragma unroll
+    for (int k = 0; k < kTileItems; ++k) {
+        const int64_t i = i0 + k * 1024 < n ? i0 + k * 1024 : n - 1;
+        key[k] = FIRST ? key_of(ids[i], n_rows, padding) : in[i].x;
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += 256) counts[(int64_t)b * tiles + blockIdx.x] = cnt[b];
+#pragma unroll
+    for (int k = 0; k < kTileItems; ++k)
+        if (i0 + k * 1024 < n) atomicAdd(&cnt[(key[k] >> shift) & (bins - 1)], 1u);
+    __syncthreads();
+    if ((int)threadIdx.x < bins) counts[(int64_t)blockIdx.x * bins + threadIdx.x] = cnt[threadIdx.x];
 }
 
-// One wave a bin: counts[bin][*] -> exclusive sums over the blocks, totals[bin].
-__global__ void __launch_bounds__(256) sort_scan_kernel(uint32_t *__restrict__ counts, uint32_t *__restrict__ totals, int bins,
-                                                        int tiles) {
-    const int lane = threadIdx.x & 63, bin = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (bin >= bins) return;
-    uint32_t *c = counts + (int64_t)bin * tiles;
-    uint32_t carry = 0;
-    for (int t = 0; t < tiles; t += 64) {
-        const uint32_t v = t + lane < tiles ? c[t + lane] : 0;
-        uint32_t x = v;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t y = __shfl_up(x, d);
-            if (lane >= d) x += y;
-        }
-        if (t + lane < tiles) c[t + lane] = carry + x - v;
-        carry += __shfl(x, 63);
+// counts[*][bin] -> sums over the blocks before, totals[bin].  A block takes 64 bins (a lane each), its 16 waves a strip of
+// the blocks each: sums of the strips, their running sum, then the strips again.
+__global__ void __launch_bounds__(1024) sort_scan_kernel(uint32_t *__restrict__ counts, uint32_t *__restrict__ totals, int bins,
+                                                         int tiles) {
+    __shared__ uint32_t strip[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bin = blockIdx.x * 64 + lane;
+    const int per = (tiles + 15) / 16, t0 = wave * per, t1 = min(tiles, t0 + per);
+    const bool on = bin < bins;
+    uint32_t sum = 0;
+    if (on) {
+#pragma unroll 8
+        for (int t = t0; t < t1; ++t) sum += counts[(int64_t)t * bins + bin];
     }
-    if (lane == 0) totals[bin] = carry;
+    strip[wave][lane] = sum;
+    __syncthreads();
+    uint32_t run = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+        if (w == wave) run = all;
+        all += strip[w][lane];
+    }
+    if (on) {
+#pragma unroll 8
+        for (int t = t0; t < t1; ++t) {
+            const uint32_t c = counts[(int64_t)t * bins + bin];
+            counts[(int64_t)t * bins + bin] = run;
+            run += c;
+        }
+        if (wave == 0) totals[bin] = all;
+    }
 }
 
 template <typename I, bool FIRST>
-__global__ void __launch_bounds__(256) sort_scatter_kernel(const I *__restrict__ ids, const uint2 *__restrict__ in, int64_t n,
-                                                           uint32_t n_rows, int64_t padding, int shift, int digit, int tiles,
-                                                           const uint32_t *__restrict__ counts,
-                                                           const uint32_t *__restrict__ totals, uint2 *__restrict__ out) {
+__global__ void __launch_bounds__(1024) sort_scatter_kernel(const I *__restrict__ ids, const uint2 *__restrict__ in, int64_t n,
+                                                            uint32_t n_rows, int64_t padding, int shift, int digit, int tiles,
+                                                            const uint32_t *__restrict__ counts,
+                                                            const uint32_t *__restrict__ totals, uint2 *__restrict__ out) {
     __shared__ uint32_t base[1 << kMaxDigit];
-    __shared__ uint16_t cnt[4][1 << kMaxDigit];
-    __shared__ uint32_t sums[4];
+    __shared__ uint16_t cnt[16][1 << kMaxDigit], start[1 << kMaxDigit];
+    __shared__ uint2 sorted[kTile];
+    __shared__ uint32_t sums[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int bins = 1 << digit;
-    for (int b = tid; b < 4 * bins; b += 256) cnt[b >> digit][b & (bins - 1)] = 0;
-    // first place of each bin: exclusive sum of the totals, `each` consecutive bins a thread
-    const int each = (bins + 255) / 256;
+    const int64_t i0 = (int64_t)blockIdx.x * kTile + wave * (64 * kTileItems) + lane;
+    uint2 pair[kTileItems];
+#pragma unroll
+    for (int k = 0; k < kTileItems; ++k) {
+        const int64_t i = i0 + k * 64 < n ? i0 + k * 64 : n - 1;
+        pair[k] = FIRST ? make_uint2(key_of(ids[i], n_rows, padding), (uint32_t)i) : in[i];
+    }
+    const uint32_t total = tid < bins ? totals[tid] : 0, before = tid < bins ? counts[(int64_t)blockIdx.x * bins + tid] : 0;
+    for (int b = tid; b < 16 * bins; b += 1024) cnt[b >> digit][b & (bins - 1)] = 0;
+    const uint32_t first = block_scan<16>(total, sums);        // first place of bin `tid` (ends in a barrier)
+    uint32_t rank[kTileItems];
+#pragma unroll
+    for (int k = 0; k < kTileItems; ++k) rank[k] = wave_rank(cnt[wave], (pair[k].x >> shift) & (bins - 1), digit, i0 + k * 64 < n);
+    __syncthreads();
     uint32_t mine = 0;
-    for (int j = 0; j < each; ++j)
-        if (tid * each + j < bins) mine += totals[tid * each + j];
-    uint32_t at = block_scan<4>(mine, sums);
-    for (int j = 0; j < each; ++j) {
-        const int b = tid * each + j;
-        if (b < bins) {
-            base[b] = at + counts[(int64_t)b * tiles + blockIdx.x];
-            at += totals[b];
+    if (tid < bins) {
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            const uint32_t c = cnt[w][tid];
+            cnt[w][tid] = (uint16_t)mine;
+            mine += c;
         }
     }
-    const int64_t i0 = (int64_t)blockIdx.x * kTile + wave * (64 * kItems);
-    uint2 pair[kItems];
-    uint32_t rank[kItems];
-#pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-        const int64_t i = i0 + k * 64 + lane;
-        pair[k] = make_uint2(0, 0);
-        if (i < n) pair[k] = FIRST ? make_uint2(key_of(ids[i], n_rows, padding), (uint32_t)i) : in[i];
+    const uint32_t local = block_scan<16>(mine, sums);         // first place of the bin inside this block
+    if (tid < bins) {
+        start[tid] = (uint16_t)local;
+        base[tid] = first + before - local;
     }
     __syncthreads();
+    // in the order of the output through LDS: neighbouring lanes then write neighbouring places
 #pragma unroll
-    for (int k = 0; k < kItems; ++k)
-        rank[k] = wave_rank(cnt[wave], (pair[k].x >> shift) & (bins - 1), digit, i0 + k * 64 + lane < n);
-    __syncthreads();
-    for (int b = tid; b < bins; b += 256) {
-        uint32_t sum = 0;
-        for (int w = 0; w < 4; ++w) {
-            const uint32_t c = cnt[w][b];
-            cnt[w][b] = (uint16_t)sum;
-            sum += c;
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kItems; ++k)
-        if (i0 + k * 64 + lane < n) {
+    for (int k = 0; k < kTileItems; ++k)
+        if (i0 + k * 64 < n) {
             const uint32_t d = (pair[k].x >> shift) & (bins - 1);
-            out[(int64_t)base[d] + cnt[wave][d] + rank[k]] = pair[k];
+            sorted[start[d] + cnt[wave][d] + rank[k]] = pair[k];
         }
+    __syncthreads();
+    const int64_t left = n - (int64_t)blockIdx.x * kTile;
+#pragma unroll
+    for (int k = 0; k < kTileItems; ++k) {
+        const int i = k * 1024 + tid;
+        if (i < left) {
+            const uint2 v = sorted[i];
+            out[(int64_t)(base[(v.x >> shift) & (bins - 1)] + i)] = v;
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------- sums over runs of equal ids
@@ -338,9 +358,9 @@ struct SumArgs {
     int64_t g_stride;
     void *grad;
     float *head, *tail;        // [tiles][dim]: partial sum of a run that began before the tile / that begins in it and goes on
-    int64_t n;
+    int64_t n, tiles;
     uint32_t n_rows;
-    int dim, tile, lanes;      // lanes: of a team, a power of two <= 64
+    int dim, tile, lanes, chunks;      // a team of `lanes` threads covers 1 / chunks of the columns
     float scale;
 };
 
@@ -360,14 +380,30 @@ __device__ __forceinline__ void store_part(float *p, int64_t tile, int dim, int 
     for (int j = 0; j < VW; ++j) p[tile * dim + col + j] = acc[j];
 }
 
+// Where a thread of the sum kernels works: teams of `lanes` neighbouring threads (no wave boundaries needed: nothing is exchanged
+// between lanes), the column chunks of a tile in neighbouring teams.
+struct Place {
+    int64_t tile;
+    int col;           // first column of this thread
+    bool on;
+};
+template <int VW>
+__device__ __forceinline__ Place place_of(const SumArgs &a) {
+    const int teams = 256 / a.lanes, team = threadIdx.x / a.lanes;
+    const int64_t at = (int64_t)blockIdx.x * teams + team;
+    Place p;
+    p.tile = a.chunks == 1 ? at : at / a.chunks;
+    p.col = (int)(((at - p.tile * a.chunks) * a.lanes + (threadIdx.x - team * a.lanes)) * VW);
+    p.on = team < teams && p.tile < a.tiles && p.col < a.dim;
+    return p;
+}
+
 template <typename G, typename T, int VW>
 __global__ void __launch_bounds__(256) sum_tiles_kernel(const SumArgs a) {
-    const int lane = threadIdx.x & (a.lanes - 1);
-    const int64_t t = (int64_t)blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
-    const int col = ((int)blockIdx.y * a.lanes + lane) * VW;
-    const int64_t i0 = t * a.tile;
-    if (i0 >= a.n || col >= a.dim) return;
-    const int64_t i1 = i0 + a.tile < a.n ? i0 + a.tile : a.n;
+    const Place at = place_of<VW>(a);
+    if (!at.on) return;
+    const int64_t t = at.tile, i0 = t * a.tile, i1 = i0 + a.tile < a.n ? i0 + a.tile : a.n;
+    const int col = at.col;
     const G *g = (const G *)a.g + col;
     uint32_t cur = a.pairs[i0].x;
     if (cur >= a.n_rows) return;                           // sorted: nothing but tokens that take no part from here on
@@ -375,14 +411,19 @@ __global__ void __launch_bounds__(256) sum_tiles_kernel(const SumArgs a) {
     float acc[VW];
 #pragma unroll
     for (int j = 0; j < VW; ++j) acc[j] = 0.0f;
+    uint2 next[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) next[k] = a.pairs[i0 + k < i1 ? i0 + k : i1 - 1];
     for (int64_t i = i0; i < i1; i += kBatch) {
         uint2 p[kBatch];
         Pack<G, VW> v[kBatch];
+        // positions are tokens whatever their id: no branch stands between the loads; the next batch's pairs travel with the rows
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) p[k] = i + k < i1 ? a.pairs[i + k] : make_uint2(~0u, 0);
+        for (int k = 0; k < kBatch; ++k) p[k] = next[k], v[k] = *reinterpret_cast<const Pack<G, VW> *>(g + (int64_t)p[k].y * a.g_stride);
+        if (i + kBatch < i1) {
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k)
-            if (p[k].x < a.n_rows) v[k] = *reinterpret_cast<const Pack<G, VW> *>(g + (int64_t)p[k].y * a.g_stride);
+            for (int k = 0; k < kBatch; ++k) next[k] = a.pairs[i + kBatch + k < i1 ? i + kBatch + k : i1 - 1];
+        }
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
             if (i + k >= i1) break;
@@ -404,39 +445,94 @@ __global__ void __launch_bounds__(256) sum_tiles_kernel(const SumArgs a) {
     else store_row<G, T, VW>(a, cur, col, acc);
 }
 
-// Runs that cross tiles: the team of the tile a run starts in adds tail[tile] and head[tile + 1 ..].
-template <typename G, typename T, int VW>
-__global__ void __launch_bounds__(256) sum_join_kernel(const SumArgs a) {
-    const int lane = threadIdx.x & (a.lanes - 1);
-    const int64_t t = (int64_t)blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
-    const int col = ((int)blockIdx.y * a.lanes + lane) * VW;
-    const int64_t i0 = t * a.tile, i1 = i0 + a.tile;
-    if (i1 >= a.n || col >= a.dim) return;
-    const uint32_t cur = a.pairs[i1 - 1].x;
-    if (cur >= a.n_rows || a.pairs[i1].x != cur || (i0 > 0 && a.pairs[i0 - 1].x == cur)) return;
-    float acc[VW];
-#pragma unroll
-    for (int j = 0; j < VW; ++j) acc[j] = a.tail[t * a.dim + col + j];
-    const int64_t tiles = (a.n + a.tile - 1) / a.tile;
-    // the run's tiles are those whose first token carries its id: batches of loads, the first other id ends it
-    for (int64_t s = t + 1; s < tiles; s += kBatch) {
-        bool in[kBatch];
+// acc += head[s0 .. s1) in order
+template <int VW>
+__device__ __forceinline__ void add_heads(const SumArgs &a, int64_t s0, int64_t s1, int col, float *acc) {
+    for (int64_t s = s0; s < s1; s += kBatch) {
         float v[kBatch][VW];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) in[k] = s + k < tiles && a.pairs[(s + k) * a.tile].x == cur;
+        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+            for (int j = 0; j < VW; ++j) v[k][j] = a.head[(s + k < s1 ? s + k : s1 - 1) * a.dim + col + j];
 #pragma unroll
         for (int k = 0; k < kBatch; ++k)
-            if (in[k])
 #pragma unroll
-                for (int j = 0; j < VW; ++j) v[k][j] = a.head[(s + k) * a.dim + col + j];
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k)
-            if (in[k])
-#pragma unroll
-                for (int j = 0; j < VW; ++j) acc[j] += v[k][j];
-        if (!in[kBatch - 1]) break;
+            for (int j = 0; j < VW; ++j) acc[j] += s + k < s1 ? v[k][j] : 0.0f;
     }
-    store_row<G, T, VW>(a, cur, col, acc);
+}
+
+// Runs that cross tiles: the team of the tile a run starts in adds tail[tile] and head[tile + 1 ..]; where the run covers more
+// than kBatch further tiles, the block's teams take a slice of them each and the slices are added in order.
+template <typename G, typename T, int VW>
+__global__ void __launch_bounds__(256) sum_join_kernel(const SumArgs a) {
+    __shared__ int long_team[256], long_count;
+    __shared__ float part[256 * VW];
+    const Place at = place_of<VW>(a);
+    const int teams = 256 / a.lanes, team = threadIdx.x / a.lanes, lane = threadIdx.x - team * a.lanes;
+    const int64_t t = at.tile, i0 = t * a.tile, i1 = i0 + a.tile;
+    if (threadIdx.x == 0) long_count = 0;
+    __syncthreads();
+    bool owner = at.on && i1 < a.n;
+    uint32_t cur = 0;
+    if (owner) {
+        cur = a.pairs[i1 - 1].x;
+        owner = cur < a.n_rows && a.pairs[i1].x == cur && !(i0 > 0 && a.pairs[i0 - 1].x == cur);
+    }
+    if (owner) {
+        // the run's tiles are those whose first token carries its id; the first kBatch of them here
+        uint32_t key[kBatch + 1];
+#pragma unroll
+        for (int k = 0; k <= kBatch; ++k) key[k] = a.pairs[(t + 1 + k < a.tiles ? t + 1 + k : a.tiles - 1) * a.tile].x;
+        int more = 0;
+#pragma unroll
+        for (int k = 0; k <= kBatch; ++k) more += t + 1 + k < a.tiles && key[k] == cur;     // sorted: a prefix
+        if (more <= kBatch) {
+            float acc[VW];
+#pragma unroll
+            for (int j = 0; j < VW; ++j) acc[j] = a.tail[t * a.dim + at.col + j];
+            add_heads<VW>(a, t + 1, t + 1 + more, at.col, acc);
+            store_row<G, T, VW>(a, cur, at.col, acc);
+        } else if (lane == 0) {
+            long_team[atomicAdd(&long_count, 1)] = team;
+        }
+    }
+    __syncthreads();
+    // long runs, by the whole block: thread (team, lane) takes a slice of the owner's heads at the owner's columns
+    const int count = long_count;
+    for (int q = 0; q < count; ++q) {
+        const int who = long_team[q];
+        const int64_t wat = (int64_t)blockIdx.x * teams + who, wt = a.chunks == 1 ? wat : wat / a.chunks;
+        const int col = (int)(((wat - wt * a.chunks) * a.lanes + lane) * VW);
+        const uint32_t key = a.pairs[wt * a.tile + a.tile - 1].x;
+        // tiles of the run behind the first: the last one whose first token carries the id, 256 probes a round
+        int64_t lo = wt + 1, hi = a.tiles;                     // lo is one of them; hi is not
+        while (hi - lo > 1) {
+            const int64_t step = (hi - lo + 255) / 256, probe = lo + threadIdx.x * step;
+            const int in = __syncthreads_count(probe < hi && a.pairs[probe * a.tile].x == key);
+            const int64_t next = lo + in * step;
+            lo = lo + (in - 1) * step;
+            hi = next < hi ? next : hi;
+        }
+        float acc[VW];
+#pragma unroll
+        for (int j = 0; j < VW; ++j) acc[j] = 0.0f;
+        const int64_t heads = lo - wt, slice = (heads + teams - 1) / teams, s0 = wt + 1 + team * slice;
+        const int64_t s1 = s0 + slice < lo + 1 ? s0 + slice : lo + 1;
+        if (team < teams && col < a.dim && s0 < s1) add_heads<VW>(a, s0, s1, col, acc);
+#pragma unroll
+        for (int j = 0; j < VW; ++j) part[threadIdx.x * VW + j] = acc[j];
+        __syncthreads();
+        if (team == 0 && col < a.dim) {
+            float sum[VW];
+#pragma unroll
+            for (int j = 0; j < VW; ++j) sum[j] = a.tail[wt * a.dim + col + j];
+            for (int w = 0; w < teams; ++w)
+#pragma unroll
+                for (int j = 0; j < VW; ++j) sum[j] += part[(w * a.lanes + lane) * VW + j];
+            store_row<G, T, VW>(a, key, col, sum);
+        }
+        __syncthreads();
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------- host
@@ -452,14 +548,13 @@ BwdPlan plan_bwd(int64_t n, int64_t n_rows, int dim) {
     BwdPlan p;
     int bits = 1;
     while (bits < 32 && (n_rows >> bits) != 0) ++bits;     // keys go up to n_rows itself
-    const int most = n <= kSmall ? kSmallDigit : kMaxDigit;
-    p.passes = (bits + most - 1) / most;
+    p.passes = (bits + kMaxDigit - 1) / kMaxDigit;
     p.digit = (bits + p.passes - 1) / p.passes;
     p.sort_tiles = n <= kSmall ? 0 : (n + kTile - 1) / kTile;
-    // enough teams to fill the chip (16 waves on each of 256 CUs), yet tiles long enough that few runs cross them
+    // enough teams to fill the chip (8 waves on each of 256 CUs), yet tiles long enough that few runs cross them
     p.tile = 64;
     const int64_t vectors = (dim + 3) / 4;
-    while (p.tile > kBatch && n * vectors / p.tile < 256 * 16 * 64) p.tile >>= 1;
+    while (p.tile > kBatch && n * vectors / p.tile < 256 * 8 * 64) p.tile >>= 1;
     p.sum_tiles = (n + p.tile - 1) / p.tile;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
@@ -476,7 +571,7 @@ BwdPlan plan_bwd(int64_t n, int64_t n_rows, int dim) {
 template <typename I>
 const uint2 *sort_pairs(const BwdPlan &p, const I *ids, int64_t n, int64_t n_rows, int64_t padding, char *ws, void *grad,
                         int64_t grad_bytes, hipStream_t s) {
-    const int fill = grid_for(grad_bytes, 1 << 16, 2048);       // at least 64 KB of zeros a block
+    const int fill = (int)((grad_bytes + kFill - 1) / kFill);
     uint2 *a = (uint2 *)(ws + p.off_a), *b = (uint2 *)(ws + p.off_b);
     if (p.sort_tiles == 0) {
         sort_small_kernel<I><<<1 + fill, 1024, 0, s>>>(ids, (int)n, (uint32_t)n_rows, padding, p.passes, p.digit,
@@ -489,17 +584,17 @@ const uint2 *sort_pairs(const BwdPlan &p, const I *ids, int64_t n, int64_t n_row
     uint2 *out = p.passes % 2 ? a : b;                          // the last pass ends in a
     for (int d = 0; d < p.passes; ++d) {
         if (d == 0)
-            sort_count_kernel<I, true><<<tiles + fill, 256, 0, s>>>(ids, nullptr, n, (uint32_t)n_rows, padding, 0, p.digit, tiles,
+            sort_count_kernel<I, true><<<tiles + fill, 1024, 0, s>>>(ids, nullptr, n, (uint32_t)n_rows, padding, 0, p.digit, tiles,
                                                                     counts, grad, grad_bytes);
         else
-            sort_count_kernel<I, false><<<tiles, 256, 0, s>>>(ids, in, n, (uint32_t)n_rows, padding, d * p.digit, p.digit, tiles,
+            sort_count_kernel<I, false><<<tiles, 1024, 0, s>>>(ids, in, n, (uint32_t)n_rows, padding, d * p.digit, p.digit, tiles,
                                                               counts, nullptr, 0);
-        sort_scan_kernel<<<(bins + 3) / 4, 256, 0, s>>>(counts, totals, bins, tiles);
+        sort_scan_kernel<<<(bins + 63) / 64, 1024, 0, s>>>(counts, totals, bins, tiles);
         if (d == 0)
-            sort_scatter_kernel<I, true><<<tiles, 256, 0, s>>>(ids, nullptr, n, (uint32_t)n_rows, padding, 0, p.digit, tiles,
+            sort_scatter_kernel<I, true><<<tiles, 1024, 0, s>>>(ids, nullptr, n, (uint32_t)n_rows, padding, 0, p.digit, tiles,
                                                                counts, totals, out);
         else
-            sort_scatter_kernel<I, false><<<tiles, 256, 0, s>>>(ids, in, n, (uint32_t)n_rows, padding, d * p.digit, p.digit, tiles,
+            sort_scatter_kernel<I, false><<<tiles, 1024, 0, s>>>(ids, in, n, (uint32_t)n_rows, padding, d * p.digit, p.digit, tiles,
                                                                 counts, totals, out);
         in = out;
         out = out == a ? b : a;
@@ -509,13 +604,12 @@ const uint2 *sort_pairs(const BwdPlan &p, const I *ids, int64_t n, int64_t n_row
 
 template <typename G, typename T, int VW>
 void launch_sums(SumArgs a, const BwdPlan &p, hipStream_t s) {
-    const int vectors = (a.dim + VW - 1) / VW;
-    a.lanes = 1;
-    while (a.lanes < 64 && a.lanes < vectors) a.lanes <<= 1;
+    const int vectors = a.dim / VW;
+    a.chunks = (vectors + 255) / 256, a.lanes = (vectors + a.chunks - 1) / a.chunks, a.tiles = p.sum_tiles;
     const int teams = 256 / a.lanes;
-    const dim3 grid((unsigned)((p.sum_tiles + teams - 1) / teams), (unsigned)((vectors + a.lanes - 1) / a.lanes));
-    sum_tiles_kernel<G, T, VW><<<grid, 256, 0, s>>>(a);
-    sum_join_kernel<G, T, VW><<<grid, 256, 0, s>>>(a);
+    const unsigned blocks = (unsigned)((p.sum_tiles * a.chunks + teams - 1) / teams);
+    sum_tiles_kernel<G, T, VW><<<blocks, 256, 0, s>>>(a);
+    sum_join_kernel<G, T, VW><<<blocks, 256, 0, s>>>(a);
 }
 
 template <typename G, typename T>
@@ -593,7 +687,7 @@ extern "C" int nrf_lookup_bwd(const void *g_out, int64_t g_stride, int32_t g_dty
                          : sort_pairs(p, (const int32_t *)ids, n, n_rows, padding_idx, ws, grad, grad_bytes, s);
     if (n > 0) {
         a.g = g_out, a.g_stride = g_stride, a.grad = grad, a.head = (float *)(ws + p.off_head), a.tail = (float *)(ws + p.off_tail);
-        a.n = n, a.n_rows = (uint32_t)n_rows, a.dim = dim, a.tile = p.tile, a.lanes = 0, a.scale = scale;
+        a.n = n, a.n_rows = (uint32_t)n_rows, a.dim = dim, a.tile = p.tile, a.scale = scale;
         const int vw = common_width(dim, eg, (uint64_t)(uintptr_t)g_out | (uint64_t)g_stride * eg, es, (uint64_t)(uintptr_t)grad);
         if (g_dtype == NRF_F32 && dtype == NRF_F32) pick_sums<float, float>(vw, a, p, s);
         else if (g_dtype == NRF_F32 && dtype == NRF_BF16) pick_sums<float, bf16_t>(vw, a, p, s);

@@ -45,23 +45,34 @@ def _typed(t, name):
 
 def _rows(t):
     """2-D tensor -> (tensor with unit column stride and rows that do not overlap, row stride)."""
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    n, dim = t.shape
+    row, col = t.stride()
+    if (dim > 1 and col != 1) or (n > 1 and row < dim):
         t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+        row = dim
+    return t, (row if n > 1 else dim)
 
 
 def _opt(t):
     return None if t is None else t.data_ptr()
 
 
+_device_now = torch._C._cuda_getDevice                  # the same as torch.cuda.current_device() and
+_stream_of = torch._C._cuda_getCurrentRawStream         # current_stream(i).cuda_stream, without building their objects (3 us)
+_fns = {}
+
+
 def _call(device, name, *args):
     """lib.name(*args, stream) with `device` current, on its current stream (the tensors' device need not be the current one)."""
-    fn = getattr(_lib.lib(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(_lib.lib(), name)
+    index = device.index
+    if index == _device_now():
+        rc = fn(*args, _stream_of(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream_of(index))
     if rc:
         check(rc, name)
 
@@ -267,7 +278,7 @@ def lookup_fwd(table, ids, scale=1.0, out_dtype=None):
         raise TypeError(f"out_dtype: expected {table.dtype} or float32, got {out_dtype}")
     t, stride = _rows(table)
     V, D = t.shape
-    out = torch.empty((*ids.shape, D), device=t.device, dtype=out_dtype)
+    out = t.new_empty((*ids.shape, D), dtype=out_dtype)
     _call(t.device, "nrf_lookup_fwd", t.data_ptr(), stride, _DTYPES[t.dtype], V, D, ids.data_ptr(), ids.dtype == torch.int64,
           ids.numel(), float(scale), out.data_ptr(), _DTYPES[out_dtype])
     return out
