@@ -535,17 +535,95 @@ __global__ void __launch_bounds__(256) sum_join_kernel(const SumArgs a) {
     }
 }
 
+// ---------------------------------------------------------------------------------------------------- few rows, few tokens
+// One launch, no workspace: a block takes a row (and up to 256 vectors of its columns), lists the tokens that name it, in order,
+// in LDS, and adds their rows of g: teams of threads take every teams-th listed token, their sums are added in order.
+// Every block reads all ids, and one block may have to read all of g: for small sizes only (few_rows below).
+constexpr int kScanIds = 16;                           // ids of a thread per round
+constexpr int kScanRound = 256 * kScanIds;
+
+template <typename G, typename T, int VW, typename I>
+__global__ void __launch_bounds__(256) sum_rows_kernel(const SumArgs a, const I *__restrict__ ids, int64_t padding) {
+    __shared__ uint16_t list[kScanRound];
+    __shared__ uint32_t waves[4];
+    __shared__ float part[256 * VW];
+    const int teams = 256 / a.lanes, team = threadIdx.x / a.lanes, lane = threadIdx.x - team * a.lanes;
+    const int row = blockIdx.x / a.chunks, col = ((int)(blockIdx.x - row * a.chunks) * a.lanes + lane) * VW;
+    const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63, n = (int)a.n;
+    const bool works = team < teams && col < a.dim;
+    const G *g = (const G *)a.g + (works ? col : 0);
+    float acc[VW];
+#pragma unroll
+    for (int j = 0; j < VW; ++j) acc[j] = 0.0f;
+    for (int i0 = 0; i0 < n && row != padding; i0 += kScanRound) {
+        // wave w lists its quarter of the round: ids wl, wl + 64, ... of it
+        const int first = i0 + wave * (kScanRound / 4) + wl;
+        uint64_t hits[kScanIds];
+        uint32_t count = 0;
+        I id[kScanIds];
+#pragma unroll
+        for (int k = 0; k < kScanIds; ++k) id[k] = ids[first + k * 64 < n ? first + k * 64 : n - 1];
+#pragma unroll
+        for (int k = 0; k < kScanIds; ++k) {
+            hits[k] = __ballot(id[k] == (I)row && first + k * 64 < n);
+            count += __popcll(hits[k]);
+        }
+        if (wl == 0) waves[wave] = count;
+        __syncthreads();
+        uint32_t at = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            if (w == wave) at = total;
+            total += waves[w];
+        }
+#pragma unroll
+        for (int k = 0; k < kScanIds; ++k) {
+            if ((hits[k] >> wl) & 1) list[at + lanes_below(hits[k])] = (uint16_t)(first + k * 64 - i0);
+            at += __popcll(hits[k]);
+        }
+        __syncthreads();
+        if (works)
+            for (uint32_t q = team; q < total; q += kBatch * teams) {
+                Pack<G, VW> v[kBatch];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    const uint32_t e = q + k * teams < total ? q + k * teams : q;
+                    v[k] = *reinterpret_cast<const Pack<G, VW> *>(g + (int64_t)(i0 + list[e]) * a.g_stride);
+                }
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+                    for (int j = 0; j < VW; ++j) acc[j] += q + k * teams < total ? to_f32(v[k].e[j]) : 0.0f;
+            }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < VW; ++j) part[threadIdx.x * VW + j] = acc[j];
+    __syncthreads();
+    if (team == 0 && works) {
+        for (int w = 1; w < teams; ++w)
+#pragma unroll
+            for (int j = 0; j < VW; ++j) acc[j] += part[(w * a.lanes + lane) * VW + j];
+        store_row<G, T, VW>(a, row, col, acc);
+    }
+}
+
 // ---------------------------------------------------------------------------------------------------- host
 struct BwdPlan {
     int passes, digit;         // of the sort
     int64_t sort_tiles;        // blocks of the many-block sort (0: one block)
     int tile;                  // tokens of a sum tile
     int64_t sum_tiles;
-    int64_t off_a, off_b, off_counts, off_totals, off_head, off_tail, bytes;
+    int64_t off_a, off_b, off_counts, off_totals, off_head, off_tail, bytes;       // all zero: few_rows, no workspace
 };
 
+// Few rows and tokens: one block a row beats sort, sums and join (4096 tokens of 32 columns, 100 rows: FEW_US us against SORT_US), while
+// the ids are read once a row and a block may meet all of g.  The bounds keep both below a few microseconds.
+bool few_rows(int64_t n, int64_t n_rows, int dim) { return n_rows * n <= 1 << 22 && n * dim <= 1 << 17 && n_rows * dim <= 1 << 20; }
+
 BwdPlan plan_bwd(int64_t n, int64_t n_rows, int dim) {
-    BwdPlan p;
+    BwdPlan p{};
+    if (few_rows(n, n_rows, dim)) return p;
     int bits = 1;
     while (bits < 32 && (n_rows >> bits) != 0) ++bits;     // keys go up to n_rows itself
     p.passes = (bits + kMaxDigit - 1) / kMaxDigit;
@@ -603,9 +681,15 @@ const uint2 *sort_pairs(const BwdPlan &p, const I *ids, int64_t n, int64_t n_row
 }
 
 template <typename G, typename T, int VW>
-void launch_sums(SumArgs a, const BwdPlan &p, hipStream_t s) {
+void launch_sums(SumArgs a, const BwdPlan &p, const void *ids, bool i64, int64_t padding, hipStream_t s) {
     const int vectors = a.dim / VW;
     a.chunks = (vectors + 255) / 256, a.lanes = (vectors + a.chunks - 1) / a.chunks, a.tiles = p.sum_tiles;
+    if (p.bytes == 0) {
+        const unsigned blocks = a.n_rows * a.chunks;
+        if (i64) sum_rows_kernel<G, T, VW, int64_t><<<blocks, 256, 0, s>>>(a, (const int64_t *)ids, padding);
+        else sum_rows_kernel<G, T, VW, int32_t><<<blocks, 256, 0, s>>>(a, (const int32_t *)ids, padding);
+        return;
+    }
     const int teams = 256 / a.lanes;
     const unsigned blocks = (unsigned)((p.sum_tiles * a.chunks + teams - 1) / teams);
     sum_tiles_kernel<G, T, VW><<<blocks, 256, 0, s>>>(a);
@@ -613,12 +697,12 @@ void launch_sums(SumArgs a, const BwdPlan &p, hipStream_t s) {
 }
 
 template <typename G, typename T>
-void pick_sums(int vw, const SumArgs &a, const BwdPlan &p, hipStream_t s) {
+void pick_sums(int vw, const SumArgs &a, const BwdPlan &p, const void *ids, bool i64, int64_t padding, hipStream_t s) {
     if constexpr (sizeof(G) == 2 && sizeof(T) == 2)
-        if (vw == 8) return launch_sums<G, T, 8>(a, p, s);
-    if (vw >= 4) return launch_sums<G, T, 4>(a, p, s);
-    if (vw == 2) return launch_sums<G, T, 2>(a, p, s);
-    launch_sums<G, T, 1>(a, p, s);
+        if (vw == 8) return launch_sums<G, T, 8>(a, p, ids, i64, padding, s);
+    if (vw >= 4) return launch_sums<G, T, 4>(a, p, ids, i64, padding, s);
+    if (vw == 2) return launch_sums<G, T, 2>(a, p, ids, i64, padding, s);
+    launch_sums<G, T, 1>(a, p, ids, i64, padding, s);
 }
 
 // the wider side's 16 bytes set the vector; both sides' addresses must be aligned to their share of it
@@ -673,27 +757,28 @@ extern "C" int nrf_lookup_bwd(const void *g_out, int64_t g_stride, int32_t g_dty
     NRF_REQUIRE(dtype_size(dtype) && dtype_size(g_dtype), "nrf_lookup_bwd: dtype %d, g_dtype %d", dtype, g_dtype);
     if (!pair_ok(dtype, g_dtype)) return fail(NRF_ERR_UNSUPPORTED, "nrf_lookup_bwd: g_out must have the table's type or f32");
     if (n_rows == 0) return NRF_OK;
-    NRF_REQUIRE(grad, "nrf_lookup_bwd: null pointer");
-    NRF_REQUIRE(n == 0 || (g_out && ids && workspace), "nrf_lookup_bwd: null pointer");
+    const BwdPlan p = plan_bwd(n, n_rows, dim);
+    NRF_REQUIRE(grad && (n == 0 || (g_out && ids)) && (p.bytes == 0 || workspace), "nrf_lookup_bwd: null pointer");
     NRF_REQUIRE(n == 0 || g_stride >= dim, "nrf_lookup_bwd: g_stride %lld below dim %d", (long long)g_stride, dim);
     NRF_REQUIRE(((uintptr_t)workspace & 15) == 0, "nrf_lookup_bwd: workspace must be 16-byte aligned");
-    const BwdPlan p = plan_bwd(n, n_rows, dim);
     const int eg = dtype_size(g_dtype), es = dtype_size(dtype);
     const int64_t grad_bytes = n_rows * dim * es;
     hipStream_t s = as_stream(stream);
+    const bool i64 = ids_are_64 != 0;
     char *ws = (char *)workspace;
-    SumArgs a;
-    a.pairs = ids_are_64 ? sort_pairs(p, (const int64_t *)ids, n, n_rows, padding_idx, ws, grad, grad_bytes, s)
-                         : sort_pairs(p, (const int32_t *)ids, n, n_rows, padding_idx, ws, grad, grad_bytes, s);
-    if (n > 0) {
+    SumArgs a{};
+    if (p.bytes)
+        a.pairs = i64 ? sort_pairs(p, (const int64_t *)ids, n, n_rows, padding_idx, ws, grad, grad_bytes, s)
+                      : sort_pairs(p, (const int32_t *)ids, n, n_rows, padding_idx, ws, grad, grad_bytes, s);
+    if (p.bytes == 0 || n > 0) {
         a.g = g_out, a.g_stride = g_stride, a.grad = grad, a.head = (float *)(ws + p.off_head), a.tail = (float *)(ws + p.off_tail);
         a.n = n, a.n_rows = (uint32_t)n_rows, a.dim = dim, a.tile = p.tile, a.scale = scale;
         const int vw = common_width(dim, eg, (uint64_t)(uintptr_t)g_out | (uint64_t)g_stride * eg, es, (uint64_t)(uintptr_t)grad);
-        if (g_dtype == NRF_F32 && dtype == NRF_F32) pick_sums<float, float>(vw, a, p, s);
-        else if (g_dtype == NRF_F32 && dtype == NRF_BF16) pick_sums<float, bf16_t>(vw, a, p, s);
-        else if (g_dtype == NRF_F32) pick_sums<float, f16_t>(vw, a, p, s);
-        else if (g_dtype == NRF_BF16) pick_sums<bf16_t, bf16_t>(vw, a, p, s);
-        else pick_sums<f16_t, f16_t>(vw, a, p, s);
+        if (g_dtype == NRF_F32 && dtype == NRF_F32) pick_sums<float, float>(vw, a, p, ids, i64, padding_idx, s);
+        else if (g_dtype == NRF_F32 && dtype == NRF_BF16) pick_sums<float, bf16_t>(vw, a, p, ids, i64, padding_idx, s);
+        else if (g_dtype == NRF_F32) pick_sums<float, f16_t>(vw, a, p, ids, i64, padding_idx, s);
+        else if (g_dtype == NRF_BF16) pick_sums<bf16_t, bf16_t>(vw, a, p, ids, i64, padding_idx, s);
+        else pick_sums<f16_t, f16_t>(vw, a, p, ids, i64, padding_idx, s);
     }
     return check_launch("nrf_lookup_bwd");
 }

@@ -9,18 +9,28 @@
 // 16 values of 2^(j/16) and a polynomial, about 14 f64 instructions (the library's is several times that), and entries
 // that the filters have already excluded are not evaluated.
 //
-// The cut (the last kept entry, by value and index) comes from a histogram of the row: 2048 bins of equal width below the maximum,
-// counts and masses.  Masses there are 64-bit fixed point (2^62 / V for e = 1), because integer atomics give the same
-// sums in any order.  The entries around the cut (up to 2048 of them) are then sorted in LDS.  A bin that holds more (many equal
-// values, far outliers) is split again by the bits of its values until it does not, or holds one value only.
+// The cut (the last kept entry, by value and index) is found among few entries:
+//   - top-k with k up to some 1500: the row is split into 4096 groups, and the k-th largest of the groups' maxima bounds the k-th
+//     largest entry from below.  The entries above that bound (a few more than k) go into a list in LDS.
+//   - else a histogram of the row, 2048 bins of equal width below the maximum, counts and masses.  Masses there are 64-bit
+//     fixed point (2^62 / V for e = 1), because integer atomics give the same sums in any order.  The bin of the cut, or all
+//     entries down to it, go into the list.  A bin that holds more than the list (many equal values, far outliers) is split again
+//     by the bits of its values until it does not, or holds one value only.
+// The list (up to 2048 entries) is sorted.  Where it holds everything that is kept, the draws come from it; else from the
+// masses of the row's tiles of 1024 entries.
+//
+// Three forms: short rows without a cut, a wave each; one block a row; and, for few long rows, 16 blocks a row over
+// several launches (the block that arrives last at a stage's end does what needs the whole row).
 #include "nrf_types.h"
 
 using namespace nrf;
 
 namespace {
 
-constexpr int kBins = 2048, kList = 2048, kMaxTiles = 1024;
+constexpr int kBins = 2048, kList = 2048, kGroups = 4096, kMaxTiles = 1024;
 constexpr int kMaxSize = 1 << 28, kMaxRows = 1 << 21;
+constexpr int kParts = 16;                  // blocks of a row, many-block form
+constexpr int kGroupsMaxK = 1500;           // above it the groups' bound lets more entries through than the list holds
 
 struct SampleArgs {
     const void *logits;
@@ -73,12 +83,39 @@ __device__ __forceinline__ double mass_of(const Row &w, uint32_t key) {
 }
 
 // Bin of the first histogram: equal widths below the maximum, the last bin open.  Every step is monotone in x.
-__device__ __forceinline__ int bin_of(const Row &w, float scale, uint32_t key) {
-    return (int)fminf((w.topf - value_of(key)) * scale, (float)(kBins - 1));
+__device__ __forceinline__ int bin_of(const Row &w, float scale, float x) {
+    return (int)fminf((w.topf - x) * scale, (float)(kBins - 1));
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t load_key(const T *row, int i) { return key_of(to_f32(row[i])); }
+// f(x, i, u) for the entries begin .. end of a row, 16 bytes a load (at any alignment of the elements), four loads in flight;
+// u: which of the four the entry came in (0 for the odd ones at the end).
+template <int BLOCK, int U = 4, typename T, typename F>
+__device__ __forceinline__ void for_each(const T *row, int begin, int end, F f) {
+    constexpr int E = 16 / sizeof(T);
+    struct __attribute__((packed, aligned(sizeof(T)))) Vec { T e[E]; };
+    const Vec *v = reinterpret_cast<const Vec *>(row + begin);
+    const int n = (end - begin) / E;
+    for (int j = threadIdx.x; j < n; j += BLOCK * U) {
+        Vec p[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) p[u] = v[min(j + u * BLOCK, n - 1)];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (j + u * BLOCK < n) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) f(to_f32(p[u].e[e]), begin + (j + u * BLOCK) * E + e, u);
+            }
+    }
+    const int i = begin + n * E + threadIdx.x;
+    if (i < end) f(to_f32(row[i]), i, 0);
+}
+
+// What is the same in all lanes, into scalar registers.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(uniform(__float_as_uint(v))); }
+__device__ __forceinline__ uint64_t uniform(uint64_t v) {
+    return ((uint64_t)uniform((uint32_t)(v >> 32)) << 32) | uniform((uint32_t)v);
+}
 
 // ---- block-wide helpers (BLOCK threads, all of them call)
 template <int BLOCK> struct Shared {
@@ -122,17 +159,16 @@ __device__ __forceinline__ V block_scan(V v, S *sums, V *total) {
 }
 
 template <int BLOCK>
-__device__ __forceinline__ void block_max_min(uint64_t &best, uint32_t &lo, Shared<BLOCK> &s) {
+__device__ __forceinline__ void block_max_min(float &hi, float &lo, Shared<BLOCK> &s) {
 #pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        best = max(best, (uint64_t)__shfl_xor((unsigned long long)best, d));
-        lo = min(lo, (uint32_t)__shfl_xor(lo, d));
-    }
+    for (int d = 32; d; d >>= 1) hi = fmaxf(hi, __shfl_xor(hi, d)), lo = fminf(lo, __shfl_xor(lo, d));
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (lane == 0) s.wave_u[wave] = best, s.wave_a[wave] = lo;
+    float *w_hi = reinterpret_cast<float *>(s.wave_a), *w_lo = reinterpret_cast<float *>(s.wave_u);
+    if (lane == 0) w_hi[wave] = hi, w_lo[wave] = lo;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < BLOCK / 64; ++w) best = max(best, s.wave_u[w]), lo = min(lo, s.wave_a[w]);
+    for (int w = 0; w < BLOCK / 64; ++w) hi = fmaxf(hi, w_hi[w]), lo = fminf(lo, w_lo[w]);
+    hi = uniform(hi), lo = uniform(lo);
     __syncthreads();
 }
 
@@ -200,52 +236,64 @@ struct RowState {
     Filter f;
     bool valid, use_p;      // use_p: top-p leaves something out, if anything does
     float t, scale;         // scale: bins of the first histogram
-    int shift, first;       // first: the lowest index of the maximum
+    int shift;
+    __device__ __forceinline__ bool plain() const { return !valid || t == 0.0f; }
 };
 
-// best: the largest key and, in the low half, ~(its lowest index); lo: the smallest key that can be drawn.
-__device__ __forceinline__ RowState row_state(const SampleArgs &a, int r, uint64_t best, uint32_t lo, const double *tab) {
+// top, low: the largest and the smallest logit (NaN aside)
+__device__ __forceinline__ RowState row_state(const SampleArgs &a, int r, float top, float low, const double *tab) {
     RowState o;
     const float p = a.top_p_v ? a.top_p_v[r] : a.top_p, m = a.min_p_v ? a.min_p_v[r] : a.min_p;
     const int k = a.top_k_v ? a.top_k_v[r] : a.top_k;
     o.t = a.temperature_v ? a.temperature_v[r] : a.temperature;
-    const uint32_t hi = (uint32_t)(best >> 32);
-    o.valid = hi != 0 && o.t >= 0.0f && o.t < __builtin_inff() && p == p && m == m;
-    o.first = (int)~(uint32_t)best;
-    o.w.topf = value_of(hi), o.w.top = o.w.topf, o.w.top_key = hi, o.w.tab = tab;
-    o.w.flat = o.t == 0.0f || o.w.topf == __builtin_inff();
+    top += 0.0f;                                           // -0 as +0
+    o.valid = top > -__builtin_inff() && o.t >= 0.0f && o.t < __builtin_inff() && p == p && m == m;
+    o.w.topf = top, o.w.top = top, o.w.top_key = key_of(top), o.w.tab = tab;
+    o.w.flat = o.t == 0.0f || top == __builtin_inff();
     o.w.inv_t = o.w.flat ? 0.0 : 1.0 / (double)o.t;
     o.f.k = k <= 0 || k > a.size ? a.size : k;
     o.f.p = p, o.f.m = fmin((double)m, 1.0);
     o.use_p = p < 1.0f;
     o.f.cut = o.f.k < a.size || o.use_p;
     o.f.key = 0, o.f.idx = a.size;
-    o.scale = fminf((float)kBins / fminf(o.w.topf - value_of(lo), 64.0f * o.t), 1e30f);
+    // 64 temperatures reach masses of 1e-28; top-k, which does not look at masses, gets some room where they are narrow
+    o.scale = fminf((float)kBins / fminf(top - low, fmaxf(64.0f * o.t, 16.0f)), 1e30f);
     o.shift = 62;
     for (int v = a.size; v > 0; v >>= 1) --o.shift;
     return o;
 }
 
-template <typename T>
-__device__ __forceinline__ void scan_max_min(const T *row, int begin, int end, uint64_t &best, uint32_t &lo) {
-    for (int i = begin + threadIdx.x; i < end; i += blockDim.x) {
-        const uint32_t key = load_key(row, i);
-        const uint64_t c = ((uint64_t)key << 32) | (uint32_t)~i;
-        if (key) best = max(best, c), lo = min(lo, key);
-    }
+// Lowest index in begin .. end that holds x (size where none does)
+template <int BLOCK, typename T>
+__device__ int find_value(Shared<BLOCK> &s, const T *row, int begin, int end, float x, int size) {
+    int at = size;
+    for_each<BLOCK>(row, begin, end, [&](float v, int i, int) { at = v == x ? min(at, i) : at; });
+#pragma unroll
+    for (int d = 32; d; d >>= 1) at = min(at, __shfl_xor(at, d));
+    if ((threadIdx.x & 63) == 0) s.wave_a[threadIdx.x >> 6] = at;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < BLOCK / 64; ++w) at = min(at, (int)s.wave_a[w]);
+    __syncthreads();
+    return at;
 }
 
-template <typename T>
-__device__ __forceinline__ void add_to_histogram(Histogram &h, const RowState &o, const T *row, int begin, int end) {
-    for (int i = begin + threadIdx.x; i < end; i += blockDim.x) {
-        const uint32_t key = load_key(row, i);
-        if (key) {
-            const int b = bin_of(o.w, o.scale, key);
-            atomicAdd(&h.cnt[b], 1u);
-            if (o.use_p)      // masses only where top-p asks for them
-                atomicAdd((unsigned long long *)&h.mass[b], (unsigned long long)fixed(mass_of(o.w, key), o.shift));
-        }
+template <int BLOCK, typename T>
+__device__ __forceinline__ void add_to_histogram(Histogram &h, const RowState &o, const T *row, int begin, int end, bool masses) {
+    if (!masses) {
+        for_each<BLOCK>(row, begin, end, [&](float x, int, int) {
+            if (key_of(x)) atomicAdd(&h.cnt[bin_of(o.w, o.scale, x)], 1u);
+        });
+        return;
     }
+    for_each<BLOCK, 1>(row, begin, end, [&](float x, int, int) {
+        const uint32_t key = key_of(x);
+        if (key) {
+            const int b = bin_of(o.w, o.scale, x);
+            atomicAdd(&h.cnt[b], 1u);
+            atomicAdd((unsigned long long *)&h.mass[b], (unsigned long long)fixed(mass_of(o.w, key), o.shift));
+        }
+    });
 }
 
 // ---- the cut
@@ -272,7 +320,7 @@ __device__ int cut_list(Shared<BLOCK> &s, const RowState &o, Filter &f, int n, A
             if (i0 + j == last - 1) s.found[0] = b;
         }
         __syncthreads();
-        *mass_at = s.found[0];
+        *mass_at = uniform(s.found[0]);
         __syncthreads();
         if (p >= 0.0) want = p * (double)*mass_at;                     // top-p of the mass found here
     }
@@ -284,7 +332,8 @@ __device__ int cut_list(Shared<BLOCK> &s, const RowState &o, Filter &f, int n, A
         before += e[j];
     }
     block_scan<BLOCK, uint32_t>(mine, s.wave_a, &kept);
-    const uint64_t c = s.list[kept > 0 ? kept - 1 : 0];
+    kept = uniform(kept);
+    const uint64_t c = uniform(s.list[kept > 0 ? kept - 1 : 0]);
     f.key = ~(uint32_t)(c >> 32);
     f.idx = (int)(uint32_t)c;
     __syncthreads();
@@ -313,8 +362,8 @@ __device__ int find_bin(Shared<BLOCK> &s, const Histogram &h, bool by_count, uin
         cb += c[j], mb += m[j];
     }
     __syncthreads();
-    const int bin = (int)s.found[0];
-    if (bin < kBins) above.cnt = (uint32_t)s.found[1], above.mass = s.found[2];
+    const int bin = (int)uniform(s.found[0]);
+    if (bin < kBins) above.cnt = (uint32_t)uniform(s.found[1]), above.mass = uniform(s.found[2]);
     __syncthreads();
     return bin;
 }
@@ -336,7 +385,7 @@ __device__ Step make_step(Shared<BLOCK> &s, const Histogram &h, const RowState &
     st.above = Above{0, 0};
     st.bin = find_bin<BLOCK>(s, h, by_count, o.f.k, st.wantm, st.above);
     st.any = st.bin < kBins;
-    st.n = st.any ? h.cnt[st.bin] : 0;
+    st.n = st.any ? uniform(h.cnt[st.bin]) : 0;
     st.prefix = st.above.cnt + st.n <= (uint32_t)kList;
     st.fits = st.prefix || st.n <= (uint32_t)kList;
     st.from = st.prefix ? 0 : st.bin;
@@ -344,7 +393,7 @@ __device__ Step make_step(Shared<BLOCK> &s, const Histogram &h, const RowState &
     return st;
 }
 
-// Top-k where it leaves something out, else top-p of the whole mass.
+// Top-k where it leaves something out, else top-p of the whole mass (known if the histogram has masses).
 template <int BLOCK>
 __device__ Step first_step(Shared<BLOCK> &s, const Histogram &h, RowState &o) {
     constexpr int kPer = kBins / BLOCK;
@@ -354,26 +403,38 @@ __device__ Step first_step(Shared<BLOCK> &s, const Histogram &h, RowState &o) {
     for (int j = 0; j < kPer; ++j) c += h.cnt[threadIdx.x * kPer + j], m += h.mass[threadIdx.x * kPer + j];
     block_scan<BLOCK, uint32_t>(c, s.wave_a, &total);
     block_scan<BLOCK, unsigned long long>(m, (unsigned long long *)s.wave_u, &mass);
-    if (o.f.k > (int)total) o.f.k = (int)total;
-    if (o.f.k == (int)total && !o.use_p) {
-        Step none;
-        none.any = none.fits = none.prefix = false;
-        return none;
-    }
-    return make_step<BLOCK>(s, h, o, o.f.k < (int)total, mass);
+    total = uniform(total), mass = uniform((uint64_t)mass);
+    if (o.f.k < (int)total) return make_step<BLOCK>(s, h, o, true, 0);
+    o.f.k = (int)total;
+    if (o.use_p && mass) return make_step<BLOCK>(s, h, o, false, mass);
+    Step none{};
+    return none;
+}
+
+// Entries of the bins from .. to into list[0 ..), in any order; entries beyond `room` are counted only.
+template <int BLOCK, typename T>
+__device__ void gather(uint64_t *list, uint32_t *count, uint32_t room, const RowState &o, const T *row, int begin, int end, int from,
+                       int to) {
+    // bin_of(x) >= from and <= to, before the rounding down to whole bins; the last bin has no end
+    const float low = (float)from, high = to == kBins - 1 ? __builtin_inff() : (float)(to + 1);
+    const float top = o.w.topf, scale = o.scale;
+    for_each<BLOCK>(row, begin, end, [&](float x, int i, int) {
+        const float b = fminf((top - x) * scale, (float)(kBins - 1));
+        if (b >= low && b < high) {
+            const uint32_t key = key_of(x);
+            if (key) {
+                const uint32_t at = atomicAdd(count, 1u);
+                if (at < room) list[at] = by_value(key, i);
+            }
+        }
+    });
 }
 
 template <int BLOCK, typename T>
-__device__ void gather_list(Shared<BLOCK> &s, const RowState &o, const T *row, int size, const Step &st) {
+__device__ void gather_list(Shared<BLOCK> &s, const RowState &o, const T *row, int size, int from, int to) {
     if (threadIdx.x == 0) s.count = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < size; i += BLOCK) {
-        const uint32_t key = load_key(row, i);
-        if (key) {
-            const int b = bin_of(o.w, o.scale, key);
-            if (b >= st.from && b <= st.bin) s.list[atomicAdd(&s.count, 1u)] = by_value(key, i);
-        }
-    }
+    gather<BLOCK, T>(s.list, &s.count, kList, o, row, 0, size, from, to);
     __syncthreads();
 }
 
@@ -388,29 +449,30 @@ __device__ __forceinline__ void clear_histogram(Histogram &h) {
 template <int BLOCK, typename T>
 __device__ void cut_range(Shared<BLOCK> &s, Histogram &h, const RowState &o, Filter &f, const T *row, int size, const Step &st,
                           uint64_t *mass_at) {
-    uint64_t best = 0;
-    uint32_t lo = 0xffffffffu;
-    for (int i = threadIdx.x; i < size; i += BLOCK) {
-        const uint32_t key = load_key(row, i);
-        if (key && bin_of(o.w, o.scale, key) == st.bin) best = max(best, (uint64_t)key << 32), lo = min(lo, key);
+    uint32_t hi = 0, lo = 0xffffffffu, n = st.n;
+    {
+        float top = -__builtin_inff(), low = __builtin_inff();
+        for_each<BLOCK>(row, 0, size, [&](float x, int, int) {
+            if (key_of(x) && bin_of(o.w, o.scale, x) == st.bin) top = fmaxf(top, x), low = fminf(low, x);
+        });
+        block_max_min<BLOCK>(top, low, s);
+        hi = key_of(top), lo = key_of(low);
     }
-    block_max_min<BLOCK>(best, lo, s);
-    uint32_t hi = (uint32_t)(best >> 32), n = st.n;
     Above above = st.above;
     while (n > (uint32_t)kList && lo < hi) {
         int bits = 0;
         while (((hi - lo) >> bits) >= (uint32_t)kBins) ++bits;
         clear_histogram<BLOCK>(h);
-        for (int i = threadIdx.x; i < size; i += BLOCK) {
-            const uint32_t key = load_key(row, i);
+        for_each<BLOCK, 1>(row, 0, size, [&](float x, int, int) {
+            const uint32_t key = key_of(x);
             if (key >= lo && key <= hi) {
                 atomicAdd(&h.cnt[(hi - key) >> bits], 1u);
                 atomicAdd((unsigned long long *)&h.mass[(hi - key) >> bits], (unsigned long long)fixed(mass_of(o.w, key), o.shift));
             }
-        }
+        });
         __syncthreads();
         const int bin = min(find_bin<BLOCK>(s, h, st.by_count, f.k, st.wantm, above), kBins - 1);
-        n = h.cnt[bin];
+        n = uniform(h.cnt[bin]);
         hi -= (uint32_t)bin << bits;
         if (hi - lo > (1u << bits) - 1) lo = hi - ((1u << bits) - 1);
         __syncthreads();
@@ -418,10 +480,10 @@ __device__ void cut_range(Shared<BLOCK> &s, Histogram &h, const RowState &o, Fil
     if (n <= (uint32_t)kList) {
         if (threadIdx.x == 0) s.count = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < size; i += BLOCK) {
-            const uint32_t key = load_key(row, i);
+        for_each<BLOCK>(row, 0, size, [&](float x, int i, int) {
+            const uint32_t key = key_of(x);
             if (key >= lo && key <= hi) s.list[atomicAdd(&s.count, 1u)] = by_value(key, i);
-        }
+        });
         __syncthreads();
         sort_list<BLOCK>(s, n);
         cut_list<BLOCK>(s, o, f, n, above, st.by_count ? (int)(f.k - above.cnt) : kList + 1, !st.by_count, -1.0, st.wantm, mass_at);
@@ -442,28 +504,39 @@ __device__ void cut_range(Shared<BLOCK> &s, Histogram &h, const RowState &o, Fil
     uint32_t seen = 0;                                   // entries of that value in the chunks before
     for (int i0 = 0; i0 < size && seen < q; i0 += BLOCK) {
         const int i = i0 + threadIdx.x;
-        const uint32_t is = i < size && load_key(row, i) == hi;
+        const uint32_t is = i < size && key_of(to_f32(row[i])) == hi;
         uint32_t all;
         const uint32_t before = seen + block_scan<BLOCK, uint32_t>(is, s.wave_a, &all);
         if (is && before + 1 == q) s.found[0] = i;
         seen += all;
     }
     __syncthreads();
-    f.idx = (int)s.found[0];
+    f.idx = (int)uniform(s.found[0]);
     __syncthreads();
+}
+
+// Mass (fixed point) of the entries that top-k's cut keeps
+template <int BLOCK, typename T>
+__device__ uint64_t mass_of_first(Shared<BLOCK> &s, const RowState &o, const T *row, int size) {
+    unsigned long long mine = 0, all;
+    for_each<BLOCK, 1>(row, 0, size, [&](float x, int i, int) {
+        const uint32_t key = key_of(x);
+        if (key && o.f.keeps(key, i)) mine += fixed(mass_of(o.w, key), o.shift);
+    });
+    block_scan<BLOCK, unsigned long long>(mine, (unsigned long long *)s.wave_u, &all);
+    return uniform((uint64_t)all);
 }
 
 // Both cuts of a long row, from its histogram (used up where a bin is too full).  gathered: the entries of the first step are in
 // the list already.  Returns the number of kept entries where the list holds all of them, sorted by value; else -1.
 template <int BLOCK, typename T>
 __device__ int select_cut(Shared<BLOCK> &s, Histogram &h, RowState &o, const T *row, int size, Step st, bool gathered) {
-    const bool by_k = st.any && st.by_count;
     while (st.any) {
         uint64_t mass_at = 0;
         if (st.fits) {
-            if (!gathered) gather_list<BLOCK, T>(s, o, row, size, st);
+            if (!gathered) gather_list<BLOCK, T>(s, o, row, size, st.from, st.bin);
             gathered = false;
-            const int n = s.count;
+            const int n = uniform(s.count);
             sort_list<BLOCK>(s, n);
             int kept;
             if (st.by_count) {
@@ -476,13 +549,13 @@ __device__ int select_cut(Shared<BLOCK> &s, Histogram &h, RowState &o, const T *
             if (st.prefix) return kept;
         } else {
             cut_range<BLOCK, T>(s, h, o, o.f, row, size, st, &mass_at);
-            if (by_k && st.by_count && o.use_p) {
-                clear_histogram<BLOCK>(h);
-                add_to_histogram<T>(h, o, row, 0, size);
-                __syncthreads();
-            }
         }
         if (!(st.by_count && o.use_p)) break;
+        // top-k's list was not the whole prefix: top-p by masses, which a histogram for top-k's sake has not got
+        clear_histogram<BLOCK>(h);
+        add_to_histogram<BLOCK, T>(h, o, row, 0, size, true);
+        __syncthreads();
+        mass_at = mass_of_first<BLOCK, T>(s, o, row, size);
         st = make_step<BLOCK>(s, h, o, false, mass_at);
     }
     if (!st.any) o.f.cut = false;
@@ -542,7 +615,7 @@ template <typename T>
 __device__ __forceinline__ double tile_mass(const RowState &o, const T *row, int size, int tile, int q) {
     const int lane = threadIdx.x & 63, end = min(size, (q + 1) * tile);
     double sum = 0.0;
-    for (int i = q * tile + lane; i < end; i += 64) sum += kept_mass(o.w, o.f, load_key(row, i), i);
+    for (int i = q * tile + lane; i < end; i += 64) sum += kept_mass(o.w, o.f, key_of(to_f32(row[i])), i);
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     return sum;
@@ -583,7 +656,7 @@ __device__ void draw_from_tiles(const RowState &o, const T *row, int size, int t
     const int end = min(size, (a + 1) * tile);
     for (int i0 = a * tile; i0 < end; i0 += 64) {
         const int i = i0 + lane;
-        const double e = i < end ? kept_mass(o.w, o.f, load_key(row, i), i) : 0.0;
+        const double e = i < end ? kept_mass(o.w, o.f, key_of(to_f32(row[i])), i) : 0.0;
         double c = e;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -605,84 +678,139 @@ __device__ void draw_from_tiles(const RowState &o, const T *row, int size, int t
     }
 }
 
-// Rows without anything to draw (id -1), and T = 0 (the first maximum): true if this was one of them.
-__device__ __forceinline__ bool plain_row(const RowState &o, const float *u, int draws, int64_t *ids, float *prob, int first, int step) {
-    if (o.valid && o.t > 0.0f) return false;
+// Rows without anything to draw (id -1), and T = 0 (the first maximum).
+__device__ __forceinline__ void draw_plain(const RowState &o, int at, const float *u, int draws, int64_t *ids, float *prob, int first,
+                                           int step) {
     for (int j = first; j < draws; j += step) {
         const bool ok = o.valid && u[j] == u[j];
-        ids[j] = ok ? o.first : -1;
+        ids[j] = ok ? at : -1;
         prob[j] = ok ? 1.0f : 0.0f;
     }
-    return true;
+}
+
+// The list holds all that top-k (k <= kGroupsMaxK) can keep: both cuts and the draws from it.
+template <int BLOCK>
+__device__ void draw_top_k(Shared<BLOCK> &s, RowState &o, int n, const float *u, int draws, int64_t *ids, float *prob) {
+    uint64_t mass_at;
+    sort_list<BLOCK>(s, n);
+    const int kept = cut_list<BLOCK>(s, o, o.f, n, Above{0, 0}, min(o.f.k, n), o.use_p, o.f.p, 0.0, &mass_at);
+    list_by_index<BLOCK>(s, kept);
+    draw_from_list<BLOCK>(s, o, kept, u, draws, ids, prob);
+}
+
+template <int BLOCK, typename T>
+__device__ void draw_whole_row(Shared<BLOCK> &s, double *tiles, const RowState &o, const T *row, int size, const float *u, int draws,
+                               int64_t *ids, float *prob) {
+    const int tid = threadIdx.x, tile = tile_of(size), n_tiles = (size + tile - 1) / tile;
+    for (int q = tid >> 6; q < n_tiles; q += BLOCK / 64) {
+        const double m = tile_mass<T>(o, row, size, tile, q);
+        if ((tid & 63) == 0) tiles[q] = m;
+    }
+    __syncthreads();
+    scan_tiles<BLOCK>(s, tiles, n_tiles);
+    for (int j = tid >> 6; j < draws; j += BLOCK / 64) draw_from_tiles<T>(o, row, size, tile, tiles, n_tiles, u[j], ids + j, prob + j);
 }
 
 // ---- one block a row
-// LONG: rows beyond kList entries, by the histogram; otherwise the whole row goes into the list.
-template <typename T, int BLOCK, bool LONG>
-__global__ void __launch_bounds__(BLOCK) sample_row_kernel(const SampleArgs a) {
+template <typename T>
+struct RowIO {
+    const T *row;
+    const float *u;
+    int64_t *ids;
+    float *prob;
+    __device__ __forceinline__ RowIO(const SampleArgs &a, int r)
+        : row((const T *)a.logits + (int64_t)r * a.stride), u(a.u + (int64_t)r * a.draws), ids(a.ids + (int64_t)r * a.draws),
+          prob(a.prob + (int64_t)r * a.draws) {}
+};
+
+// Rows of up to kList entries: the whole row goes into the list.
+template <typename T>
+__global__ void __launch_bounds__(256) sample_short_kernel(const SampleArgs a) {
+    constexpr int BLOCK = 256;
     __shared__ Shared<BLOCK> s;
-    const int tid = threadIdx.x, r = blockIdx.x, size = a.size;
-    const T *row = (const T *)a.logits + (int64_t)r * a.stride;
-    const float *u = a.u + (int64_t)r * a.draws;
-    int64_t *ids = a.ids + (int64_t)r * a.draws;
-    float *prob = a.prob + (int64_t)r * a.draws;
-
-    uint64_t best = 0;
-    uint32_t lo = 0xffffffffu;
-    scan_max_min<T>(row, 0, size, best, lo);
+    const int tid = threadIdx.x, size = a.size;
+    const RowIO<T> io(a, blockIdx.x);
+    float top = -__builtin_inff(), low = __builtin_inff();
+    for_each<BLOCK>(io.row, 0, size, [&](float x, int, int) { top = fmaxf(top, x), low = fminf(low, x); });
     if (tid < 16) s.tab[tid] = exp2(tid / 16.0);
-    block_max_min<BLOCK>(best, lo, s);
-    RowState o = row_state(a, r, best, lo, s.tab);
-    if (plain_row(o, u, a.draws, ids, prob, tid, BLOCK)) return;
+    block_max_min<BLOCK>(top, low, s);
+    RowState o = row_state(a, blockIdx.x, top, low, s.tab);
+    if (o.plain()) {
+        const int at = find_value<BLOCK, T>(s, io.row, 0, size, o.w.topf, size);
+        return draw_plain(o, at, io.u, a.draws, io.ids, io.prob, tid, BLOCK);
+    }
+    if (!o.f.cut) {
+        for_each<BLOCK>(io.row, 0, size, [&](float x, int i, int) { s.list[i] = ((uint64_t)i << 32) | key_of(x); });
+        __syncthreads();
+        return draw_from_list<BLOCK>(s, o, size, io.u, a.draws, io.ids, io.prob);
+    }
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    for_each<BLOCK>(io.row, 0, size, [&](float x, int i, int) {
+        const uint32_t key = key_of(x);
+        if (key) s.list[atomicAdd(&s.count, 1u)] = by_value(key, i);
+    });
+    __syncthreads();
+    draw_top_k<BLOCK>(s, o, uniform(s.count), io.u, a.draws, io.ids, io.prob);
+}
 
-    int listed = -1;
-    if constexpr (!LONG) {
-        if (!o.f.cut) {
-            for (int i = tid; i < size; i += BLOCK) s.list[i] = ((uint64_t)i << 32) | load_key(row, i);
-            __syncthreads();
-            return draw_from_list<BLOCK>(s, o, size, u, a.draws, ids, prob);
-        }
-        if (tid == 0) s.count = 0;
-        __syncthreads();
-        for (int i = tid; i < size; i += BLOCK) {
-            const uint32_t key = load_key(row, i);
-            if (key) s.list[atomicAdd(&s.count, 1u)] = by_value(key, i);
-        }
-        __syncthreads();
-        const int n = s.count;
-        sort_list<BLOCK>(s, n);
-        uint64_t mass_at;
-        listed = cut_list<BLOCK>(s, o, o.f, n, Above{0, 0}, min(o.f.k, n), o.use_p, o.f.p, 0.0, &mass_at);
-    } else if (o.f.cut) {
-        __shared__ Histogram h;
+template <typename T>
+__global__ void __launch_bounds__(1024) sample_row_kernel(const SampleArgs a) {
+    constexpr int BLOCK = 1024;
+    __shared__ Shared<BLOCK> s;
+    __shared__ Histogram h;
+    __shared__ double tiles[kMaxTiles];
+    const int tid = threadIdx.x, size = a.size;
+    const RowIO<T> io(a, blockIdx.x);
+    float group[4] = {-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()}, low = __builtin_inff();
+    for_each<BLOCK>(io.row, 0, size, [&](float x, int, int u) { group[u] = fmaxf(group[u], x), low = fminf(low, x); });
+    if (tid < 16) s.tab[tid] = exp2(tid / 16.0);
+    float top = fmaxf(fmaxf(group[0], group[1]), fmaxf(group[2], group[3]));
+    block_max_min<BLOCK>(top, low, s);
+    RowState o = row_state(a, blockIdx.x, top, low, s.tab);
+    if (o.plain()) {
+        const int at = find_value<BLOCK, T>(s, io.row, 0, size, o.w.topf, size);
+        return draw_plain(o, at, io.u, a.draws, io.ids, io.prob, tid, BLOCK);
+    }
+    if (o.f.cut) {
+        const bool by_k = o.f.k < size;
         clear_histogram<BLOCK>(h);
-        add_to_histogram<T>(h, o, row, 0, size);
-        __syncthreads();
-        const Step st = first_step<BLOCK>(s, h, o);
-        listed = select_cut<BLOCK, T>(s, h, o, row, size, st, false);
-    }
-    if (listed > 0) {
-        list_by_index<BLOCK>(s, listed);
-        return draw_from_list<BLOCK>(s, o, listed, u, a.draws, ids, prob);
-    }
-    if constexpr (LONG) {
-        __shared__ double tiles[kMaxTiles];
-        const int tile = tile_of(size), n_tiles = (size + tile - 1) / tile;
-        for (int q = tid >> 6; q < n_tiles; q += BLOCK / 64) {
-            const double m = tile_mass<T>(o, row, size, tile, q);
-            if ((tid & 63) == 0) tiles[q] = m;
+        if (o.f.k <= kGroupsMaxK) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (group[u] > -__builtin_inff()) atomicAdd(&h.cnt[bin_of(o.w, o.scale, group[u])], 1u);
+            __syncthreads();
+            Above above{0, 0};
+            const int bin = find_bin<BLOCK>(s, h, true, o.f.k, 0.0, above);
+            if (bin < kBins) {
+                gather_list<BLOCK, T>(s, o, io.row, size, 0, bin);
+                const uint32_t n = uniform(s.count);
+                if (n <= (uint32_t)kList) return draw_top_k<BLOCK>(s, o, n, io.u, a.draws, io.ids, io.prob);
+            }
+            clear_histogram<BLOCK>(h);
         }
+        add_to_histogram<BLOCK, T>(h, o, io.row, 0, size, !by_k);
         __syncthreads();
-        scan_tiles<BLOCK>(s, tiles, n_tiles);
-        for (int j = tid >> 6; j < a.draws; j += BLOCK / 64)
-            draw_from_tiles<T>(o, row, size, tile, tiles, n_tiles, u[j], ids + j, prob + j);
+        Step st = first_step<BLOCK>(s, h, o);
+        if (by_k && !st.any && o.use_p) {          // fewer than k can be drawn: top-p of them all
+            clear_histogram<BLOCK>(h);
+            add_to_histogram<BLOCK, T>(h, o, io.row, 0, size, true);
+            __syncthreads();
+            st = first_step<BLOCK>(s, h, o);
+        }
+        const int listed = select_cut<BLOCK, T>(s, h, o, io.row, size, st, false);
+        if (listed > 0) {
+            list_by_index<BLOCK>(s, listed);
+            return draw_from_list<BLOCK>(s, o, listed, io.u, a.draws, io.ids, io.prob);
+        }
     }
+    draw_whole_row<BLOCK, T>(s, tiles, o, io.row, size, io.u, a.draws, io.ids, io.prob);
 }
 
 template <typename T>
 void launch_sample(const SampleArgs &a, hipStream_t s) {
-    if (a.size <= kList) sample_row_kernel<T, 256, false><<<a.rows, 256, 0, s>>>(a);
-    else sample_row_kernel<T, 1024, true><<<a.rows, 1024, 0, s>>>(a);
+    if (a.size <= kList) sample_short_kernel<T><<<a.rows, 256, 0, s>>>(a);
+    else sample_row_kernel<T><<<a.rows, 1024, 0, s>>>(a);
 }
 
 }  // namespace

@@ -302,10 +302,10 @@ def lookup_bwd(g_out, ids, n_rows, scale=1.0, padding_idx=None, dtype=None):
     nbytes = _lib.lib().nrf_lookup_bwd_workspace_bytes(n, V, D)
     if nbytes < 0:
         raise RuntimeError("nrf_lookup_bwd_workspace_bytes: " + _lib.lib().nrf_last_error_string().decode())
-    grad = torch.empty((V, D), device=g.device, dtype=dtype)
-    ws = torch.empty((max(nbytes, 1),), device=g.device, dtype=torch.uint8)
+    grad = g.new_empty((V, D), dtype=dtype)
+    ws = g.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     _call(g.device, "nrf_lookup_bwd", g.data_ptr(), stride, _DTYPES[g.dtype], ids.data_ptr(), ids.dtype == torch.int64, n, V, D,
-          float(scale), pad, grad.data_ptr(), _DTYPES[dtype], ws.data_ptr())
+          float(scale), pad, grad.data_ptr(), _DTYPES[dtype], _opt(ws))
     return grad
 
 
