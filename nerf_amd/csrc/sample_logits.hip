@@ -30,6 +30,7 @@ namespace {
 constexpr int kBins = 2048, kList = 2048, kGroups = 4096, kMaxTiles = 1024;
 constexpr int kMaxSize = 1 << 28, kMaxRows = 1 << 21;
 constexpr int kParts = 16;                  // blocks of a row, many-block form
+constexpr int kPartsMaxRows = 64;
 constexpr int kGroupsMaxK = 1500;           // above it the groups' bound lets more entries through than the list holds
 
 struct SampleArgs {
@@ -604,21 +605,80 @@ __device__ void draw_from_list(Shared<BLOCK> &s, const RowState &o, int n, const
     }
 }
 
-// Tiles of a row: their masses, added lane by lane, then over the wave.
+// Tiles of a row: 1024 entries, or a multiple of them where a row has more than kMaxTiles; 16 consecutive entries a lane.
 __device__ __forceinline__ int tile_of(int size) {
     int tile = 1024;
     while ((size + tile - 1) / tile > kMaxTiles) tile <<= 1;
     return tile;
 }
 
+// This lane's 16 kept masses of the 1024 entries from `base`; their sum
+template <typename T>
+__device__ __forceinline__ double lane_masses(const RowState &o, const T *row, int size, int base, double *e) {
+    constexpr int E = 16 / sizeof(T);
+    struct __attribute__((packed, aligned(sizeof(T)))) Vec { T e[E]; };
+    const int i0 = base + (threadIdx.x & 63) * 16;
+    T x[16];
+    if (i0 + 16 <= size) {
+#pragma unroll
+        for (int v = 0; v < 16 / E; ++v) {
+            const Vec p = *reinterpret_cast<const Vec *>(row + i0 + v * E);
+#pragma unroll
+            for (int j = 0; j < E; ++j) x[v * E + j] = p.e[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = i0 + j < size ? row[i0 + j] : from_f32<T>(-__builtin_inff());
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        e[j] = kept_mass(o.w, o.f, key_of(to_f32(x[j])), i0 + j);
+        sum += e[j];
+    }
+    return sum;
+}
+
+// Inclusive sums over the lanes of a wave
+__device__ __forceinline__ double wave_scan(double v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const double y = __shfl_up(v, d);
+        if (lane >= d) v += y;
+    }
+    return v;
+}
+
 template <typename T>
 __device__ __forceinline__ double tile_mass(const RowState &o, const T *row, int size, int tile, int q) {
-    const int lane = threadIdx.x & 63, end = min(size, (q + 1) * tile);
-    double sum = 0.0;
-    for (int i = q * tile + lane; i < end; i += 64) sum += kept_mass(o.w, o.f, key_of(to_f32(row[i])), i);
+    double e[16], sum = 0.0;
+    const int end = min(size, (q + 1) * tile);
+    for (int base = q * tile; base < end; base += 1024) sum += lane_masses<T>(o, row, size, base, e);
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     return sum;
+}
+
+// Of the lanes' entries (base + 16 lane + j, masses e, inclusive lane sums `cum` on top of `before`) the first whose running sum
+// exceeds `want`; where rounding leaves none, the last one with mass.  Returns whether one exceeds.
+template <int P>
+__device__ __forceinline__ bool pick_entry(const double *e, double sum, double cum, double before, double want, int base, int &at,
+                                           double &mass) {
+    const uint64_t over = __ballot(sum > 0.0 && before + cum > want), some = __ballot(sum > 0.0);
+    if (some == 0) return false;
+    const int src = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+    double run = before + (cum - sum), m = 0.0;
+    int in = 0;
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        run += e[j];
+        if (e[j] > 0.0 && !found) in = j, m = e[j], found = over != 0 && run > want;
+    }
+    at = base + src * P + __shfl(in, src);
+    mass = __shfl(m, src);
+    return over != 0;
 }
 
 // tiles[0 .. n) -> running sums
@@ -651,26 +711,13 @@ __device__ void draw_from_tiles(const RowState &o, const T *row, int size, int t
         else a = mid + 1;
     }
     while (a > 0 && tiles[a] <= tiles[a - 1]) --a;       // u = 1: back to the last tile that has mass
-    double cum = a > 0 ? tiles[a - 1] : 0.0, mass = 0.0;
+    double before = a > 0 ? tiles[a - 1] : 0.0, mass = 0.0, e[16];
     int at = 0;
     const int end = min(size, (a + 1) * tile);
-    for (int i0 = a * tile; i0 < end; i0 += 64) {
-        const int i = i0 + lane;
-        const double e = i < end ? kept_mass(o.w, o.f, key_of(to_f32(row[i])), i) : 0.0;
-        double c = e;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const double y = __shfl_up(c, d);
-            if (lane >= d) c += y;
-        }
-        const uint64_t over = __ballot(e > 0.0 && cum + c > want), some = __ballot(e > 0.0);
-        // the first that exceeds; where the sums' rounding leaves none, the last one with mass
-        if (some) {
-            const int src = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
-            at = i0 + src, mass = __shfl(e, src);
-        }
-        if (over) break;
-        cum += __shfl(c, 63);
+    for (int base = a * tile; base < end; base += 1024) {
+        const double sum = lane_masses<T>(o, row, size, base, e), cum = wave_scan(sum);
+        if (pick_entry<16>(e, sum, cum, before, want, base, at, mass)) break;
+        before += __shfl(cum, 63);
     }
     if (lane == 0) {
         *id = uj == uj ? at : -1;
@@ -723,6 +770,30 @@ struct RowIO {
           prob(a.prob + (int64_t)r * a.draws) {}
 };
 
+// A long row by its histogram, from the start.
+template <int BLOCK, typename T>
+__device__ void draw_long_row(Shared<BLOCK> &s, Histogram &h, double *tiles, RowState &o, const RowIO<T> &io, const SampleArgs &a) {
+    if (o.f.cut) {
+        const bool by_k = o.f.k < a.size;
+        clear_histogram<BLOCK>(h);
+        add_to_histogram<BLOCK, T>(h, o, io.row, 0, a.size, !by_k);
+        __syncthreads();
+        Step st = first_step<BLOCK>(s, h, o);
+        if (by_k && !st.any && o.use_p) {          // fewer than k can be drawn: top-p of them all
+            clear_histogram<BLOCK>(h);
+            add_to_histogram<BLOCK, T>(h, o, io.row, 0, a.size, true);
+            __syncthreads();
+            st = first_step<BLOCK>(s, h, o);
+        }
+        const int listed = select_cut<BLOCK, T>(s, h, o, io.row, a.size, st, false);
+        if (listed > 0) {
+            list_by_index<BLOCK>(s, listed);
+            return draw_from_list<BLOCK>(s, o, listed, io.u, a.draws, io.ids, io.prob);
+        }
+    }
+    draw_whole_row<BLOCK, T>(s, tiles, o, io.row, a.size, io.u, a.draws, io.ids, io.prob);
+}
+
 // Rows of up to kList entries: the whole row goes into the list.
 template <typename T>
 __global__ void __launch_bounds__(256) sample_short_kernel(const SampleArgs a) {
@@ -772,53 +843,353 @@ __global__ void __launch_bounds__(1024) sample_row_kernel(const SampleArgs a) {
         const int at = find_value<BLOCK, T>(s, io.row, 0, size, o.w.topf, size);
         return draw_plain(o, at, io.u, a.draws, io.ids, io.prob, tid, BLOCK);
     }
-    if (o.f.cut) {
-        const bool by_k = o.f.k < size;
+    if (o.f.cut && o.f.k <= kGroupsMaxK) {
         clear_histogram<BLOCK>(h);
-        if (o.f.k <= kGroupsMaxK) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (group[u] > -__builtin_inff()) atomicAdd(&h.cnt[bin_of(o.w, o.scale, group[u])], 1u);
-            __syncthreads();
-            Above above{0, 0};
-            const int bin = find_bin<BLOCK>(s, h, true, o.f.k, 0.0, above);
-            if (bin < kBins) {
-                gather_list<BLOCK, T>(s, o, io.row, size, 0, bin);
-                const uint32_t n = uniform(s.count);
-                if (n <= (uint32_t)kList) return draw_top_k<BLOCK>(s, o, n, io.u, a.draws, io.ids, io.prob);
-            }
-            clear_histogram<BLOCK>(h);
-        }
-        add_to_histogram<BLOCK, T>(h, o, io.row, 0, size, !by_k);
+        for (int u = 0; u < 4; ++u)
+            if (group[u] > -__builtin_inff()) atomicAdd(&h.cnt[bin_of(o.w, o.scale, group[u])], 1u);
         __syncthreads();
-        Step st = first_step<BLOCK>(s, h, o);
-        if (by_k && !st.any && o.use_p) {          // fewer than k can be drawn: top-p of them all
-            clear_histogram<BLOCK>(h);
-            add_to_histogram<BLOCK, T>(h, o, io.row, 0, size, true);
-            __syncthreads();
-            st = first_step<BLOCK>(s, h, o);
-        }
-        const int listed = select_cut<BLOCK, T>(s, h, o, io.row, size, st, false);
-        if (listed > 0) {
-            list_by_index<BLOCK>(s, listed);
-            return draw_from_list<BLOCK>(s, o, listed, io.u, a.draws, io.ids, io.prob);
+        Above above{0, 0};
+        const int bin = find_bin<BLOCK>(s, h, true, o.f.k, 0.0, above);
+        if (bin < kBins) {
+            gather_list<BLOCK, T>(s, o, io.row, size, 0, bin);
+            const uint32_t n = uniform(s.count);
+            if (n <= (uint32_t)kList) return draw_top_k<BLOCK>(s, o, n, io.u, a.draws, io.ids, io.prob);
         }
     }
-    draw_whole_row<BLOCK, T>(s, tiles, o, io.row, size, io.u, a.draws, io.ids, io.prob);
+    draw_long_row<BLOCK, T>(s, h, tiles, o, io, a);
+}
+
+// ---- short rows without a cut: a wave a row, P consecutive entries a lane (rows of up to 64 P entries)
+template <typename T, int P>
+__global__ void __launch_bounds__(256) sample_wave_kernel(const SampleArgs a) {
+    __shared__ double tab[16];
+    if (threadIdx.x < 16) tab[threadIdx.x] = exp2(threadIdx.x / 16.0);
+    __syncthreads();
+    const int lane = threadIdx.x & 63, r = blockIdx.x * 4 + (threadIdx.x >> 6), size = a.size;
+    if (r >= a.rows) return;
+    const RowIO<T> io(a, r);
+    constexpr int E = 16 / sizeof(T);
+    struct __attribute__((packed, aligned(sizeof(T)))) Vec { T e[E]; };
+    const int i0 = lane * P;
+    float x[P], top = -__builtin_inff();
+#pragma unroll
+    for (int v = 0; v < P / E; ++v) {
+        const int i = i0 + v * E;
+        if (i + E <= size) {
+            const Vec p = *reinterpret_cast<const Vec *>(io.row + i);
+#pragma unroll
+            for (int j = 0; j < E; ++j) x[v * E + j] = to_f32(p.e[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j) x[v * E + j] = i + j < size ? to_f32(io.row[i + j]) : -__builtin_inff();
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < P; ++j) top = fmaxf(top, x[j]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const RowState o = row_state(a, r, uniform(top), 0.0f, tab);
+    if (o.plain()) {
+        int at = 0;
+#pragma unroll
+        for (int j = P - 1; j >= 0; --j) at = x[j] == o.w.topf ? j : at;
+        uint64_t has = 0;
+#pragma unroll
+        for (int j = 0; j < P; ++j) has |= __ballot(x[j] == o.w.topf);
+        const int src = has ? __builtin_ctzll(has) : 0;
+        return draw_plain(o, src * P + __shfl(at, src), io.u, a.draws, io.ids, io.prob, lane, 64);
+    }
+    double e[P], sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        e[j] = kept_mass(o.w, o.f, key_of(x[j]), i0 + j);
+        sum += e[j];
+    }
+    const double cum = wave_scan(sum), total = __shfl(cum, 63);
+    for (int d = 0; d < a.draws; ++d) {
+        const float u = io.u[d];
+        int at = 0;
+        double mass = 0.0;
+        pick_entry<P>(e, sum, cum, 0.0, (double)fminf(fmaxf(u, 0.0f), 1.0f) * total, 0, at, mass);
+        if (lane == 0) {
+            io.ids[d] = u == u ? at : -1;
+            io.prob[d] = u == u ? (float)(mass / total) : 0.0f;
+        }
+    }
+}
+
+// ---- few long rows: kParts blocks a row and stage.  What a stage leaves for the next, per row:
+struct RowWork {
+    float top[kParts], low[kParts];        // of each part
+    int32_t first[kParts];                 // lowest index of the part's maximum (T = 0)
+    uint32_t count[2];                     // entries in `list`: from the groups' bound / from the histogram
+    uint32_t arrived[3];
+    uint32_t done;                         // the draws are out
+    uint32_t cut, cut_key;
+    int32_t cut_idx, k;
+    uint32_t pad[6];
+    float group[kGroups];
+    Histogram h;
+    uint64_t list[kList];
+    double tiles[kMaxTiles];
+};
+
+struct Part {
+    int begin, end;
+};
+__device__ __forceinline__ Part part_of(int size, int part) {
+    const int each = ((size + kParts - 1) / kParts + 15) / 16 * 16;
+    return Part{min(size, part * each), min(size, (part + 1) * each)};
+}
+
+__device__ __forceinline__ RowState state_of(const SampleArgs &a, int r, const RowWork &w, const double *tab) {
+    float top = w.top[0], low = w.low[0];
+    for (int i = 1; i < kParts; ++i) top = fmaxf(top, w.top[i]), low = fminf(low, w.low[i]);
+    return row_state(a, r, uniform(top), uniform(low), tab);
+}
+
+// Whether this block is the last of its row at this point: what the others wrote before is visible to it then.
+template <int BLOCK>
+__device__ __forceinline__ bool last_to_arrive(Shared<BLOCK> &s, uint32_t *counter) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) s.found[0] = atomicAdd(counter, 1u) + 1 == gridDim.x;
+    __syncthreads();
+    const bool last = uniform((uint32_t)s.found[0]);
+    __syncthreads();
+    if (last) __threadfence();
+    return last;
+}
+
+// Stage 1: maximum, minimum, groups' maxima; clears what later stages add to.
+template <typename T>
+__global__ void __launch_bounds__(1024) sample_max_kernel(const SampleArgs a, RowWork *work) {
+    constexpr int BLOCK = 1024;
+    __shared__ Shared<BLOCK> s;
+    const int tid = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
+    RowWork &w = work[r];
+    const RowIO<T> io(a, r);
+    const Part p = part_of(a.size, part);
+    float top = -__builtin_inff(), low = __builtin_inff();
+    for_each<BLOCK>(io.row, p.begin, p.end, [&](float x, int, int) { top = fmaxf(top, x), low = fminf(low, x); });
+    float g = fmaxf(top, __shfl_xor(top, 1));
+    g = fmaxf(g, __shfl_xor(g, 2));
+    constexpr int kEach = kGroups / kParts;                    // groups of a part: four threads each
+    if ((tid & 3) == 0) w.group[part * kEach + (tid >> 2)] = g;
+    for (int b = tid; b < kBins / kParts; b += BLOCK) w.h.cnt[part * (kBins / kParts) + b] = 0, w.h.mass[part * (kBins / kParts) + b] = 0;
+    block_max_min<BLOCK>(top, low, s);
+    const float t = a.temperature_v ? a.temperature_v[r] : a.temperature;
+    const int first = t == 0.0f ? find_value<BLOCK, T>(s, io.row, p.begin, p.end, top, a.size) : 0;
+    if (tid == 0) {
+        w.top[part] = top, w.low[part] = low, w.first[part] = first;
+        if (part == 0) {
+            w.count[0] = w.count[1] = w.done = w.cut = 0;
+            w.arrived[0] = w.arrived[1] = w.arrived[2] = 0;
+        }
+    }
+}
+
+// Stage 2, rows whose top-k the groups' maxima bound: the list, and by the last block the draws.  Where the list overflows, the
+// next stages see to the row, or (alone) the last block by itself.
+template <typename T>
+__global__ void __launch_bounds__(1024) sample_groups_kernel(const SampleArgs a, RowWork *work, bool alone) {
+    constexpr int BLOCK = 1024;
+    __shared__ Shared<BLOCK> s;
+    __shared__ Histogram h;
+    __shared__ double tiles[kMaxTiles];
+    const int tid = threadIdx.x, r = blockIdx.y;
+    RowWork &w = work[r];
+    const RowIO<T> io(a, r);
+    if (tid < 16) s.tab[tid] = exp2(tid / 16.0);
+    RowState o = state_of(a, r, w, s.tab);
+    if (o.plain()) {                                           // the list holds nothing: one block writes the row
+        if (blockIdx.x > 0) return;
+        int at = a.size;
+        for (int i = 0; i < kParts; ++i)
+            if (w.top[i] == o.w.topf) at = min(at, w.first[i]);
+        draw_plain(o, at, io.u, a.draws, io.ids, io.prob, tid, BLOCK);
+        if (tid == 0) w.done = 1;
+        return;
+    }
+    if (o.f.k > kGroupsMaxK && !alone) return;
+    clear_histogram<BLOCK>(h);
+#pragma unroll
+    for (int u = 0; u < kGroups / BLOCK; ++u) {
+        const float g = w.group[u * BLOCK + tid];
+        if (g > -__builtin_inff()) atomicAdd(&h.cnt[bin_of(o.w, o.scale, g)], 1u);
+    }
+    __syncthreads();
+    Above above{0, 0};
+    const int bin = find_bin<BLOCK>(s, h, true, o.f.k, 0.0, above);
+    const Part p = part_of(a.size, blockIdx.x);
+    if (bin < kBins) gather<BLOCK, T>(w.list, &w.count[0], kList, o, io.row, p.begin, p.end, 0, bin);
+    if (!last_to_arrive<BLOCK>(s, &w.arrived[0])) return;
+    const uint32_t n = uniform(w.count[0]);
+    if (bin < kBins && n <= (uint32_t)kList) {
+        for (int i = tid; i < (int)n; i += BLOCK) s.list[i] = w.list[i];
+        __syncthreads();
+        draw_top_k<BLOCK>(s, o, n, io.u, a.draws, io.ids, io.prob);
+        if (tid == 0) w.done = 1;
+    } else if (alone) {
+        draw_long_row<BLOCK, T>(s, h, tiles, o, io, a);
+    }
+}
+
+// Stage 3: the histogram.
+template <typename T>
+__global__ void __launch_bounds__(1024) sample_bins_kernel(const SampleArgs a, RowWork *work) {
+    constexpr int BLOCK = 1024;
+    __shared__ Histogram h;
+    __shared__ double tab[16];
+    const int tid = threadIdx.x, r = blockIdx.y;
+    RowWork &w = work[r];
+    if (w.done) return;
+    if (tid < 16) tab[tid] = exp2(tid / 16.0);
+    const RowState o = state_of(a, r, w, tab);
+    if (o.plain() || !o.f.cut) return;
+    clear_histogram<BLOCK>(h);
+    const RowIO<T> io(a, r);
+    const Part p = part_of(a.size, blockIdx.x);
+    add_to_histogram<BLOCK, T>(h, o, io.row, p.begin, p.end, o.use_p);
+    __syncthreads();
+    for (int b = tid; b < kBins; b += BLOCK) {
+        if (h.cnt[b]) atomicAdd(&w.h.cnt[b], h.cnt[b]);
+        if (h.mass[b]) atomicAdd((unsigned long long *)&w.h.mass[b], (unsigned long long)h.mass[b]);
+    }
+}
+
+// Stage 4: the entries around the first cut into the list; the last block finds the cut.
+template <typename T>
+__global__ void __launch_bounds__(1024) sample_cut_kernel(const SampleArgs a, RowWork *work) {
+    constexpr int BLOCK = 1024;
+    __shared__ Shared<BLOCK> s;
+    __shared__ Histogram h;
+    const int tid = threadIdx.x, r = blockIdx.y;
+    RowWork &w = work[r];
+    if (w.done) return;
+    if (tid < 16) s.tab[tid] = exp2(tid / 16.0);
+    RowState o = state_of(a, r, w, s.tab);
+    if (o.plain() || !o.f.cut) return;
+    for (int b = tid; b < kBins; b += BLOCK) h.cnt[b] = w.h.cnt[b], h.mass[b] = w.h.mass[b];
+    __syncthreads();
+    const RowIO<T> io(a, r);
+    const Part p = part_of(a.size, blockIdx.x);
+    const Step st = first_step<BLOCK>(s, h, o);
+    if (st.any && st.fits) gather<BLOCK, T>(w.list, &w.count[1], kList, o, io.row, p.begin, p.end, st.from, st.bin);
+    if (!last_to_arrive<BLOCK>(s, &w.arrived[1])) return;
+    if (st.any && st.fits) {
+        const int n = (int)uniform(w.count[1]);                // as many as the histogram counted: they fit
+        for (int i = tid; i < n; i += BLOCK) s.list[i] = w.list[i];
+        if (tid == 0) s.count = n;
+        __syncthreads();
+    }
+    const int listed = select_cut<BLOCK, T>(s, h, o, io.row, a.size, st, st.any && st.fits);
+    if (listed > 0) {
+        list_by_index<BLOCK>(s, listed);
+        draw_from_list<BLOCK>(s, o, listed, io.u, a.draws, io.ids, io.prob);
+    }
+    if (tid == 0) w.done = listed > 0, w.cut = o.f.cut, w.cut_key = o.f.key, w.cut_idx = o.f.idx;
+}
+
+// What is kept, for the stages after the cut
+__device__ __forceinline__ RowState cut_state(const SampleArgs &a, int r, const RowWork &w, const double *tab) {
+    RowState o = state_of(a, r, w, tab);
+    o.f.cut = w.cut, o.f.key = w.cut_key, o.f.idx = w.cut_idx;
+    return o;
+}
+
+// Stage 5: masses of the tiles, a wave each; by the last block their running sums.
+template <typename T>
+__global__ void __launch_bounds__(256) sample_tiles_kernel(const SampleArgs a, RowWork *work) {
+    constexpr int BLOCK = 256;
+    __shared__ Shared<BLOCK> s;
+    const int tid = threadIdx.x, r = blockIdx.y, tile = tile_of(a.size), n = (a.size + tile - 1) / tile;
+    RowWork &w = work[r];
+    if (w.done) return;
+    if (tid < 16) s.tab[tid] = exp2(tid / 16.0);
+    __syncthreads();
+    const RowState o = cut_state(a, r, w, s.tab);
+    if (o.plain()) return;
+    const int q = blockIdx.x * 4 + (tid >> 6);
+    const RowIO<T> io(a, r);
+    if (q < n) {
+        const double m = tile_mass<T>(o, io.row, a.size, tile, q);
+        if ((tid & 63) == 0) w.tiles[q] = m;
+    }
+    if (last_to_arrive<BLOCK>(s, &w.arrived[2])) scan_tiles<BLOCK>(s, w.tiles, n);
+}
+
+// Stage 6: the draws, a wave each.
+template <typename T>
+__global__ void __launch_bounds__(256) sample_draw_kernel(const SampleArgs a, const RowWork *work) {
+    __shared__ double tab[16], tiles[kMaxTiles];
+    const int tid = threadIdx.x, r = blockIdx.y, tile = tile_of(a.size), n = (a.size + tile - 1) / tile;
+    const RowWork &w = work[r];
+    if (w.done) return;
+    if (tid < 16) tab[tid] = exp2(tid / 16.0);
+    const RowState o = cut_state(a, r, w, tab);
+    const RowIO<T> io(a, r);
+    if (o.plain()) {
+        int at = a.size;
+        for (int i = 0; i < kParts; ++i)
+            if (w.top[i] == o.w.topf) at = min(at, w.first[i]);
+        return draw_plain(o, at, io.u, a.draws, io.ids, io.prob, blockIdx.x * 256 + tid, gridDim.x * 256);
+    }
+    for (int q = tid; q < n; q += 256) tiles[q] = w.tiles[q];
+    __syncthreads();
+    for (int j = blockIdx.x * 4 + (tid >> 6); j < a.draws; j += gridDim.x * 4)
+        draw_from_tiles<T>(o, io.row, a.size, tile, tiles, n, io.u[j], io.ids + j, io.prob + j);
+}
+
+// ---- host
+enum Form { kWaveForm, kShortForm, kRowForm, kPartsForm };
+
+Form form_of(int64_t rows, int size, int draws, bool may_cut) {
+    if (size <= kList) return !may_cut && draws <= 16 ? kWaveForm : kShortForm;
+    return rows <= kPartsMaxRows ? kPartsForm : kRowForm;
 }
 
 template <typename T>
-void launch_sample(const SampleArgs &a, hipStream_t s) {
-    if (a.size <= kList) sample_short_kernel<T><<<a.rows, 256, 0, s>>>(a);
-    else sample_row_kernel<T><<<a.rows, 1024, 0, s>>>(a);
+void launch_sample(const SampleArgs &a, bool may_k, bool may_p, RowWork *work, hipStream_t s) {
+    const Form form = form_of(a.rows, a.size, a.draws, may_k || may_p);
+    if (form == kWaveForm) {
+        if (a.size <= 1024) sample_wave_kernel<T, 16><<<(a.rows + 3) / 4, 256, 0, s>>>(a);
+        else sample_wave_kernel<T, 32><<<(a.rows + 3) / 4, 256, 0, s>>>(a);
+    } else if (form == kShortForm) {
+        sample_short_kernel<T><<<a.rows, 256, 0, s>>>(a);
+    } else if (form == kRowForm) {
+        sample_row_kernel<T><<<a.rows, 1024, 0, s>>>(a);
+    } else {
+        const dim3 parts(kParts, a.rows);
+        sample_max_kernel<T><<<parts, 1024, 0, s>>>(a, work);
+        // one k for all rows, within the groups' reach: nothing is left for later stages
+        const bool alone = !a.top_k_v && may_k && a.top_k <= kGroupsMaxK;
+        if (may_k) sample_groups_kernel<T><<<parts, 1024, 0, s>>>(a, work, alone);
+        if (alone) return;
+        if (may_k || may_p) {
+            sample_bins_kernel<T><<<parts, 1024, 0, s>>>(a, work);
+            sample_cut_kernel<T><<<parts, 1024, 0, s>>>(a, work);
+        }
+        int tile = 1024;
+        while ((a.size + tile - 1) / tile > kMaxTiles) tile <<= 1;
+        const int n_tiles = (a.size + tile - 1) / tile;
+        sample_tiles_kernel<T><<<dim3((n_tiles + 3) / 4, a.rows), 256, 0, s>>>(a, work);
+        const int draw_blocks = (a.draws + 3) / 4 < 1024 ? (a.draws + 3) / 4 : 1024;
+        sample_draw_kernel<T><<<dim3(draw_blocks, a.rows), 256, 0, s>>>(a, work);
+    }
 }
 
 }  // namespace
 
+extern "C" int64_t nrf_sample_logits_workspace_bytes(int64_t n_rows, int32_t size) {
+    return size > kList && n_rows <= kPartsMaxRows ? n_rows * (int64_t)sizeof(RowWork) : 0;
+}
+
 extern "C" int nrf_sample_logits(const void *logits, int64_t row_stride, int32_t dtype, int64_t n_rows, int32_t size, int32_t n_draws,
                                  float temperature, int32_t top_k, float top_p, float min_p, const float *temperature_rows,
                                  const int32_t *top_k_rows, const float *top_p_rows, const float *min_p_rows, const float *u,
-                                 int64_t *ids, float *prob, void *stream) {
+                                 int64_t *ids, float *prob, void *workspace, void *stream) {
     NRF_REQUIRE(n_rows >= 0 && size >= 1 && n_draws >= 0, "nrf_sample_logits: n_rows %lld, size %d, n_draws %d", (long long)n_rows, size, n_draws);
     NRF_REQUIRE(dtype_size(dtype), "nrf_sample_logits: dtype %d", dtype);
     NRF_REQUIRE(row_stride >= 0, "nrf_sample_logits: row_stride %lld", (long long)row_stride);
@@ -834,9 +1205,13 @@ extern "C" int nrf_sample_logits(const void *logits, int64_t row_stride, int32_t
     a.temperature_v = temperature_rows, a.top_k_v = top_k_rows, a.top_p_v = top_p_rows, a.min_p_v = min_p_rows;
     a.temperature = temperature, a.top_k = top_k, a.top_p = top_p, a.min_p = min_p;
     a.rows = (int)n_rows, a.size = size, a.draws = n_draws, a.ids = ids, a.prob = prob;
+    NRF_REQUIRE(workspace || nrf_sample_logits_workspace_bytes(n_rows, size) == 0, "nrf_sample_logits: null pointer (workspace)");
+    NRF_REQUIRE(((uintptr_t)workspace & 15) == 0, "nrf_sample_logits: workspace must be 16-byte aligned");
+    const bool may_k = top_k_rows || (top_k > 0 && top_k < size), may_p = top_p_rows || top_p < 1.0f;
+    RowWork *work = (RowWork *)workspace;
     hipStream_t s = as_stream(stream);
-    if (dtype == NRF_F32) launch_sample<float>(a, s);
-    else if (dtype == NRF_BF16) launch_sample<bf16_t>(a, s);
-    else launch_sample<f16_t>(a, s);
+    if (dtype == NRF_F32) launch_sample<float>(a, may_k, may_p, work, s);
+    else if (dtype == NRF_BF16) launch_sample<bf16_t>(a, may_k, may_p, work, s);
+    else launch_sample<f16_t>(a, may_k, may_p, work, s);
     return check_launch("nrf_sample_logits");
 }

@@ -84,7 +84,7 @@ FILTERS = [dict(), dict(k=1), dict(k=40), dict(p=0.9), dict(m=0.05), dict(k=3000
 def test_filters(kind, R, V):
     rng = np.random.RandomState(V)
     x = make(kind, R, V, rng).cuda()
-    for i, f in enumerate(FILTERS):
+    for f in FILTERS:
         u = torch.from_numpy(rng.rand(R, 5).astype(np.float32)).cuda()
         check(x, u, **f)
 
