@@ -57,6 +57,13 @@ __device__ __forceinline__ float value_of(uint32_t k) {
     return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
+// 2^(j/16)
+__constant__ double kRoots[16] = {
+    0x1.0000000000000p+0, 0x1.0b5586cf9890fp+0, 0x1.172b83c7d517bp+0, 0x1.2387a6e756238p+0, 0x1.306fe0a31b715p+0,
+    0x1.3dea64c123422p+0, 0x1.4bfdad5362a27p+0, 0x1.5ab07dd485429p+0, 0x1.6a09e667f3bcdp+0, 0x1.7a11473eb0187p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.9c49182a3f090p+0, 0x1.ae89f995ad3adp+0, 0x1.c199bdd85529cp+0, 0x1.d5818dcfba487p+0,
+    0x1.ea4afa2a490dap+0};
+
 struct Row {
     double top, inv_t;      // M and 1 / T (0 at T = 0)
     float topf;
@@ -127,6 +134,7 @@ template <int BLOCK> struct Shared {
     uint32_t wave_a[kWaves];
     uint32_t count;                    // entries in `list`
     uint64_t found[3];                 // what one thread found for all
+    uint32_t crowded, bucket[kBins];   // sort_list
     uint64_t list[kList];
     double mass[kList];
 };
@@ -135,18 +143,40 @@ struct Histogram {
     uint64_t mass[kBins];
 };
 
+// The value of the lane that DPP control CTRL names, 0 where there is none (4- and 8-byte types)
+template <int CTRL, int ROWS, typename V>
+__device__ __forceinline__ V dpp(V v) {
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+    } else {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, false);
+        return __builtin_bit_cast(V, ((uint64_t)hi << 32) | lo);
+    }
+}
+
+// Inclusive sums over the lanes of a wave: shifts inside rows of 16, then the rows' last lanes (all lanes must be active)
+template <typename V>
+__device__ __forceinline__ V wave_scan(V v) {
+    v += dpp<0x111, 0xf>(v);      // row_shr:1
+    v += dpp<0x112, 0xf>(v);      // row_shr:2
+    v += dpp<0x114, 0xf>(v);      // row_shr:4
+    v += dpp<0x118, 0xf>(v);      // row_shr:8
+    v += dpp<0x142, 0xa>(v);      // row_bcast:15 into rows 1 and 3
+    v += dpp<0x143, 0xc>(v);      // row_bcast:31 into rows 2 and 3
+    return v;
+}
+template <typename V>
+__device__ __forceinline__ V lane_before(V v) { return dpp<0x138, 0xf>(v); }      // wave_shr:1
+
 // Sum of the values of the threads before this one, in a fixed order of additions; *total = the sum of all.
 template <int BLOCK, typename V, typename S>
 __device__ __forceinline__ V block_scan(V v, S *sums, V *total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const V y = __shfl_up(v, d);
-        if (lane >= d) v += y;
-    }
+    v = wave_scan(v);
     if (lane == 63) sums[wave] = v;
-    V before = __shfl_up(v, 1);
-    if (lane == 0) before = 0;
+    const V before = lane_before(v);
     __syncthreads();
     V base = 0, all = 0;
 #pragma unroll
@@ -173,37 +203,115 @@ __device__ __forceinline__ void block_max_min(float &hi, float &lo, Shared<BLOCK
     __syncthreads();
 }
 
-// list[0 .. n) into rising order; n <= kList.  Bitonic, padded with ~0 to a power of two.
-template <int BLOCK>
-__device__ void sort_list(Shared<BLOCK> &s, int n) {
-    int size = 2;
-    while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += BLOCK) s.list[i] = ~0ull;
-    __syncthreads();
-    for (int k = 2; k <= size; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int p = threadIdx.x; p < size / 2; p += BLOCK) {
-                const int a = ((p & ~(j - 1)) << 1) | (p & (j - 1)), b = a | j;
-                const uint64_t x = s.list[a], y = s.list[b];
-                if ((x > y) == ((a & k) == 0)) s.list[a] = y, s.list[b] = x;
-            }
-            __syncthreads();
-        }
-}
-
 // Order of the entries: larger value first, then smaller index.
 __device__ __forceinline__ uint64_t by_value(uint32_t key, int i) { return ((uint64_t)~key << 32) | (uint32_t)i; }
 
+// list[0 .. n) into rising order, n <= kList.  bucket(c): 0 .. kBins - 1, rising with c.
+//   few entries: each counts the smaller ones;
+//   else: buckets (about as many as entries), each entry counting within its own;
+//   where a bucket is crowded (equal values): bitonic, 66 steps of a barrier each for 2048 entries (18 us against 4).
+template <int BLOCK, typename F>
+__device__ __forceinline__ void sort_list(Shared<BLOCK> &s, int n, F bucket) {
+    constexpr int kPer = kList / BLOCK;
+    uint64_t c[kPer];
+    if (n <= 256) {
+        static_assert(BLOCK >= 256, "one entry a thread");
+        const int i = threadIdx.x;
+        uint32_t rank = 0;
+        if (i < n) {
+            c[0] = s.list[i];
+#pragma unroll 8
+            for (int j = 0; j < n; ++j) rank += s.list[j] < c[0];
+        }
+        __syncthreads();
+        if (i < n) s.list[rank] = c[0];
+        __syncthreads();
+        return;
+    }
+    uint32_t *count = s.bucket;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) count[j * BLOCK + threadIdx.x] = 0;
+    if (threadIdx.x == 0) s.crowded = 0;
+    __syncthreads();
+    int b[kPer];
+    uint32_t at[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int i = j * BLOCK + threadIdx.x;
+        if (i < n) {
+            c[j] = s.list[i];
+            b[j] = bucket(c[j]);
+            at[j] = atomicAdd(&count[b[j]], 1u);
+            if (at[j] == 64) s.crowded = 1;
+        }
+    }
+    __syncthreads();
+    if (s.crowded) {
+        int size = 512;
+        while (size < n) size <<= 1;
+        for (int i = n + threadIdx.x; i < size; i += BLOCK) s.list[i] = ~0ull;
+        __syncthreads();
+        for (int k = 2; k <= size; k <<= 1)
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                for (int p = threadIdx.x; p < size / 2; p += BLOCK) {
+                    const int x = ((p & ~(j - 1)) << 1) | (p & (j - 1)), y = x | j;
+                    const uint64_t u = s.list[x], v = s.list[y];
+                    if ((u > v) == ((x & k) == 0)) s.list[x] = v, s.list[y] = u;
+                }
+                __syncthreads();
+            }
+        return;
+    }
+    // bucket sizes -> first places
+    uint32_t mine[kPer], run = 0, all;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) mine[j] = count[threadIdx.x * kPer + j], run += mine[j];
+    uint32_t first = block_scan<BLOCK, uint32_t>(run, s.wave_a, &all);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        count[threadIdx.x * kPer + j] = first;
+        first += mine[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+        if (j * BLOCK + (int)threadIdx.x < n) s.list[count[b[j]] + at[j]] = c[j];
+    __syncthreads();
+    uint32_t place[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+        if (j * BLOCK + (int)threadIdx.x < n) {
+            const uint32_t lo = count[b[j]], hi = b[j] + 1 < kBins ? count[b[j] + 1] : n;
+            place[j] = lo;
+            for (uint32_t q = lo; q < hi; ++q) place[j] += s.list[q] < c[j];
+        }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+        if (j * BLOCK + (int)threadIdx.x < n) s.list[place[j]] = c[j];
+    __syncthreads();
+}
+
+// The list in the order of value, largest first: entries between base and base - kBins / mul.
+template <int BLOCK>
+__device__ __forceinline__ void sort_by_value(Shared<BLOCK> &s, int n, float base, float mul) {
+    sort_list<BLOCK>(s, n, [=](uint64_t c) {
+        return (int)fminf(fmaxf((base - value_of(~(uint32_t)(c >> 32))) * mul, 0.0f), (float)(kBins - 1));
+    });
+}
+
 // Entries 0 .. n of the list from the order of value to that of the index, as (index, key).
 template <int BLOCK>
-__device__ __forceinline__ void list_by_index(Shared<BLOCK> &s, int n) {
+__device__ __forceinline__ void list_by_index(Shared<BLOCK> &s, int n, int size) {
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += BLOCK) {
         const uint64_t c = s.list[i];
         s.list[i] = (c << 32) | (uint32_t)~(uint32_t)(c >> 32);
     }
     __syncthreads();
-    sort_list<BLOCK>(s, n);
+    int shift = 0;
+    while ((size - 1) >> shift >= kBins) ++shift;
+    sort_list<BLOCK>(s, n, [=](uint64_t c) { return (int)((uint32_t)(c >> 32) >> shift); });
 }
 
 struct Filter {
@@ -266,7 +374,7 @@ __device__ __forceinline__ RowState row_state(const SampleArgs &a, int r, float 
 
 // Lowest index in begin .. end that holds x (size where none does)
 template <int BLOCK, typename T>
-__device__ int find_value(Shared<BLOCK> &s, const T *row, int begin, int end, float x, int size) {
+__device__ __forceinline__ int find_value(Shared<BLOCK> &s, const T *row, int begin, int end, float x, int size) {
     int at = size;
     for_each<BLOCK>(row, begin, end, [&](float v, int i, int) { at = v == x ? min(at, i) : at; });
 #pragma unroll
@@ -301,7 +409,7 @@ __device__ __forceinline__ void add_to_histogram(Histogram &h, const RowState &o
 // In a sorted list whose first entry has `above` before it: the last of the entries that are among the first `last` and have less
 // than `want` of mass before them (by_mass).  Returns how many entries of the list that keeps; mass_at: mass up to entry `last`.
 template <int BLOCK>
-__device__ int cut_list(Shared<BLOCK> &s, const RowState &o, Filter &f, int n, Above above, int last, bool by_mass, double p,
+__device__ __forceinline__ int cut_list(Shared<BLOCK> &s, const RowState &o, Filter &f, int n, Above above, int last, bool by_mass, double p,
                         double want, uint64_t *mass_at) {
     constexpr int kPer = kList / BLOCK;
     uint64_t e[kPer], run = 0;
@@ -342,20 +450,19 @@ __device__ int cut_list(Shared<BLOCK> &s, const RowState &o, Filter &f, int n, A
 }
 
 // The bin that takes the running count to `want` (by_count), or the running mass to `wantm`; adds what stands before it to
-// `above`.  kBins: none does.
+// `above` (masses only where the histogram has them).  kBins: none does.
 template <int BLOCK>
-__device__ int find_bin(Shared<BLOCK> &s, const Histogram &h, bool by_count, uint32_t want, double wantm, Above &above) {
+__device__ __forceinline__ int find_bin(Shared<BLOCK> &s, const Histogram &h, bool by_count, bool masses, uint32_t want, double wantm, Above &above) {
     constexpr int kPer = kBins / BLOCK;
     const int b0 = threadIdx.x * kPer;
     uint32_t c[kPer], cs = 0, call;
-    uint64_t m[kPer], ms = 0;
+    uint64_t m[kPer], ms = 0, mb = 0;
     unsigned long long mall;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) c[j] = h.cnt[b0 + j], m[j] = h.mass[b0 + j], cs += c[j], ms += m[j];
-    uint64_t cb = above.cnt + block_scan<BLOCK, uint32_t>(cs, s.wave_a, &call);
-    uint64_t mb = above.mass + block_scan<BLOCK, unsigned long long>(ms, (unsigned long long *)s.wave_u, &mall);
+    for (int j = 0; j < kPer; ++j) c[j] = h.cnt[b0 + j], m[j] = masses ? h.mass[b0 + j] : 0, cs += c[j], ms += m[j];
     if (threadIdx.x == 0) s.found[0] = kBins;
-    __syncthreads();
+    uint64_t cb = above.cnt + block_scan<BLOCK, uint32_t>(cs, s.wave_a, &call);
+    if (masses) mb = above.mass + block_scan<BLOCK, unsigned long long>(ms, (unsigned long long *)s.wave_u, &mall);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
         const bool hit = by_count ? cb < want && cb + c[j] >= want : (double)mb < wantm && (double)(mb + m[j]) >= wantm;
@@ -379,12 +486,12 @@ struct Step {
 };
 
 template <int BLOCK>
-__device__ Step make_step(Shared<BLOCK> &s, const Histogram &h, const RowState &o, bool by_count, uint64_t mass_k) {
+__device__ __forceinline__ Step make_step(Shared<BLOCK> &s, const Histogram &h, const RowState &o, bool by_count, uint64_t mass_k) {
     Step st;
     st.by_count = by_count;
     st.wantm = fmax(o.f.p * (double)mass_k, 0.5);          // top-p keeps at least the first
     st.above = Above{0, 0};
-    st.bin = find_bin<BLOCK>(s, h, by_count, o.f.k, st.wantm, st.above);
+    st.bin = find_bin<BLOCK>(s, h, by_count, true, o.f.k, st.wantm, st.above);
     st.any = st.bin < kBins;
     st.n = st.any ? uniform(h.cnt[st.bin]) : 0;
     st.prefix = st.above.cnt + st.n <= (uint32_t)kList;
@@ -396,7 +503,7 @@ __device__ Step make_step(Shared<BLOCK> &s, const Histogram &h, const RowState &
 
 // Top-k where it leaves something out, else top-p of the whole mass (known if the histogram has masses).
 template <int BLOCK>
-__device__ Step first_step(Shared<BLOCK> &s, const Histogram &h, RowState &o) {
+__device__ __forceinline__ Step first_step(Shared<BLOCK> &s, const Histogram &h, RowState &o) {
     constexpr int kPer = kBins / BLOCK;
     uint32_t c = 0, total;
     unsigned long long m = 0, mass;
@@ -414,7 +521,7 @@ __device__ Step first_step(Shared<BLOCK> &s, const Histogram &h, RowState &o) {
 
 // Entries of the bins from .. to into list[0 ..), in any order; entries beyond `room` are counted only.
 template <int BLOCK, typename T>
-__device__ void gather(uint64_t *list, uint32_t *count, uint32_t room, const RowState &o, const T *row, int begin, int end, int from,
+__device__ __forceinline__ void gather(uint64_t *list, uint32_t *count, uint32_t room, const RowState &o, const T *row, int begin, int end, int from,
                        int to) {
     // bin_of(x) >= from and <= to, before the rounding down to whole bins; the last bin has no end
     const float low = (float)from, high = to == kBins - 1 ? __builtin_inff() : (float)(to + 1);
@@ -432,7 +539,7 @@ __device__ void gather(uint64_t *list, uint32_t *count, uint32_t room, const Row
 }
 
 template <int BLOCK, typename T>
-__device__ void gather_list(Shared<BLOCK> &s, const RowState &o, const T *row, int size, int from, int to) {
+__device__ __forceinline__ void gather_list(Shared<BLOCK> &s, const RowState &o, const T *row, int size, int from, int to) {
     if (threadIdx.x == 0) s.count = 0;
     __syncthreads();
     gather<BLOCK, T>(s.list, &s.count, kList, o, row, 0, size, from, to);
@@ -448,7 +555,7 @@ __device__ __forceinline__ void clear_histogram(Histogram &h) {
 // A cut inside a bin that holds more than the list: the bin's range of keys is split again (whole row per step) until the
 // entries fit, or share one value.  Uses up the histogram.
 template <int BLOCK, typename T>
-__device__ void cut_range(Shared<BLOCK> &s, Histogram &h, const RowState &o, Filter &f, const T *row, int size, const Step &st,
+__device__ __forceinline__ void cut_range(Shared<BLOCK> &s, Histogram &h, const RowState &o, Filter &f, const T *row, int size, const Step &st,
                           uint64_t *mass_at) {
     uint32_t hi = 0, lo = 0xffffffffu, n = st.n;
     {
@@ -472,7 +579,7 @@ __device__ void cut_range(Shared<BLOCK> &s, Histogram &h, const RowState &o, Fil
             }
         });
         __syncthreads();
-        const int bin = min(find_bin<BLOCK>(s, h, st.by_count, f.k, st.wantm, above), kBins - 1);
+        const int bin = min(find_bin<BLOCK>(s, h, st.by_count, true, f.k, st.wantm, above), kBins - 1);
         n = uniform(h.cnt[bin]);
         hi -= (uint32_t)bin << bits;
         if (hi - lo > (1u << bits) - 1) lo = hi - ((1u << bits) - 1);
@@ -486,7 +593,7 @@ __device__ void cut_range(Shared<BLOCK> &s, Histogram &h, const RowState &o, Fil
             if (key >= lo && key <= hi) s.list[atomicAdd(&s.count, 1u)] = by_value(key, i);
         });
         __syncthreads();
-        sort_list<BLOCK>(s, n);
+        sort_by_value<BLOCK>(s, n, value_of(hi), fminf((float)kBins / (value_of(hi) - value_of(lo)), 1e30f));
         cut_list<BLOCK>(s, o, f, n, above, st.by_count ? (int)(f.k - above.cnt) : kList + 1, !st.by_count, -1.0, st.wantm, mass_at);
         return;
     }
@@ -518,7 +625,7 @@ __device__ void cut_range(Shared<BLOCK> &s, Histogram &h, const RowState &o, Fil
 
 // Mass (fixed point) of the entries that top-k's cut keeps
 template <int BLOCK, typename T>
-__device__ uint64_t mass_of_first(Shared<BLOCK> &s, const RowState &o, const T *row, int size) {
+__device__ __forceinline__ uint64_t mass_of_first(Shared<BLOCK> &s, const RowState &o, const T *row, int size) {
     unsigned long long mine = 0, all;
     for_each<BLOCK, 1>(row, 0, size, [&](float x, int i, int) {
         const uint32_t key = key_of(x);
@@ -531,14 +638,15 @@ __device__ uint64_t mass_of_first(Shared<BLOCK> &s, const RowState &o, const T *
 // Both cuts of a long row, from its histogram (used up where a bin is too full).  gathered: the entries of the first step are in
 // the list already.  Returns the number of kept entries where the list holds all of them, sorted by value; else -1.
 template <int BLOCK, typename T>
-__device__ int select_cut(Shared<BLOCK> &s, Histogram &h, RowState &o, const T *row, int size, Step st, bool gathered) {
+__device__ __forceinline__ int select_cut(Shared<BLOCK> &s, Histogram &h, RowState &o, const T *row, int size, Step st, bool gathered) {
     while (st.any) {
         uint64_t mass_at = 0;
         if (st.fits) {
             if (!gathered) gather_list<BLOCK, T>(s, o, row, size, st.from, st.bin);
             gathered = false;
             const int n = uniform(s.count);
-            sort_list<BLOCK>(s, n);
+            // the bins from .. bin, stretched over the buckets
+            sort_by_value<BLOCK>(s, n, o.w.topf - (float)st.from / o.scale, o.scale * ((float)kBins / (float)(st.bin - st.from + 1)));
             int kept;
             if (st.by_count) {
                 // with the whole prefix in the list, top-p is decided by it too
@@ -571,7 +679,7 @@ __device__ __forceinline__ double mass_or_zero(const RowState &o, uint32_t key) 
 
 // From the list: kept entries 0 .. n by index as (index, key); a thread a draw.
 template <int BLOCK>
-__device__ void draw_from_list(Shared<BLOCK> &s, const RowState &o, int n, const float *u, int draws, int64_t *ids, float *prob) {
+__device__ __forceinline__ void draw_from_list(Shared<BLOCK> &s, const RowState &o, int n, const float *u, int draws, int64_t *ids, float *prob) {
     constexpr int kPer = kList / BLOCK;
     double e[kPer], run = 0.0, total;
     const int tid = threadIdx.x, i0 = tid * kPer;
@@ -635,19 +743,9 @@ __device__ __forceinline__ double lane_masses(const RowState &o, const T *row, i
     for (int j = 0; j < 16; ++j) {
         e[j] = kept_mass(o.w, o.f, key_of(to_f32(x[j])), i0 + j);
         sum += e[j];
+        if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // 16 exponentials interleaved need more registers than there are
     }
     return sum;
-}
-
-// Inclusive sums over the lanes of a wave
-__device__ __forceinline__ double wave_scan(double v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const double y = __shfl_up(v, d);
-        if (lane >= d) v += y;
-    }
-    return v;
 }
 
 template <typename T>
@@ -683,7 +781,7 @@ __device__ __forceinline__ bool pick_entry(const double *e, double sum, double c
 
 // tiles[0 .. n) -> running sums
 template <int BLOCK>
-__device__ void scan_tiles(Shared<BLOCK> &s, double *tiles, int n) {
+__device__ __forceinline__ void scan_tiles(Shared<BLOCK> &s, double *tiles, int n) {
     constexpr int kPer = kMaxTiles / BLOCK;
     const int q0 = threadIdx.x * kPer;
     double v[kPer], run = 0.0, total;
@@ -700,7 +798,7 @@ __device__ void scan_tiles(Shared<BLOCK> &s, double *tiles, int n) {
 
 // One draw by a wave: the tile by its running sum, then the entry.
 template <typename T>
-__device__ void draw_from_tiles(const RowState &o, const T *row, int size, int tile, const double *tiles, int n_tiles, float uj,
+__device__ __forceinline__ void draw_from_tiles(const RowState &o, const T *row, int size, int tile, const double *tiles, int n_tiles, float uj,
                                 int64_t *id, float *prob) {
     const int lane = threadIdx.x & 63;
     const double total = tiles[n_tiles - 1], want = (double)fminf(fmaxf(uj, 0.0f), 1.0f) * total;
@@ -735,18 +833,18 @@ __device__ __forceinline__ void draw_plain(const RowState &o, int at, const floa
     }
 }
 
-// The list holds all that top-k (k <= kGroupsMaxK) can keep: both cuts and the draws from it.
+// The list holds all that top-k can keep (values down to `low`): both cuts and the draws from it.
 template <int BLOCK>
-__device__ void draw_top_k(Shared<BLOCK> &s, RowState &o, int n, const float *u, int draws, int64_t *ids, float *prob) {
+__device__ __forceinline__ void draw_top_k(Shared<BLOCK> &s, RowState &o, int n, float low, int size, const float *u, int draws, int64_t *ids, float *prob) {
     uint64_t mass_at;
-    sort_list<BLOCK>(s, n);
+    sort_by_value<BLOCK>(s, n, o.w.topf, fminf((float)kBins / (o.w.topf - low), 1e30f));
     const int kept = cut_list<BLOCK>(s, o, o.f, n, Above{0, 0}, min(o.f.k, n), o.use_p, o.f.p, 0.0, &mass_at);
-    list_by_index<BLOCK>(s, kept);
+    list_by_index<BLOCK>(s, kept, size);
     draw_from_list<BLOCK>(s, o, kept, u, draws, ids, prob);
 }
 
 template <int BLOCK, typename T>
-__device__ void draw_whole_row(Shared<BLOCK> &s, double *tiles, const RowState &o, const T *row, int size, const float *u, int draws,
+__device__ __forceinline__ void draw_whole_row(Shared<BLOCK> &s, double *tiles, const RowState &o, const T *row, int size, const float *u, int draws,
                                int64_t *ids, float *prob) {
     const int tid = threadIdx.x, tile = tile_of(size), n_tiles = (size + tile - 1) / tile;
     for (int q = tid >> 6; q < n_tiles; q += BLOCK / 64) {
@@ -772,7 +870,7 @@ struct RowIO {
 
 // A long row by its histogram, from the start.
 template <int BLOCK, typename T>
-__device__ void draw_long_row(Shared<BLOCK> &s, Histogram &h, double *tiles, RowState &o, const RowIO<T> &io, const SampleArgs &a) {
+__device__ __forceinline__ void draw_long_row(Shared<BLOCK> &s, Histogram &h, double *tiles, RowState &o, const RowIO<T> &io, const SampleArgs &a) {
     if (o.f.cut) {
         const bool by_k = o.f.k < a.size;
         clear_histogram<BLOCK>(h);
@@ -787,7 +885,7 @@ __device__ void draw_long_row(Shared<BLOCK> &s, Histogram &h, double *tiles, Row
         }
         const int listed = select_cut<BLOCK, T>(s, h, o, io.row, a.size, st, false);
         if (listed > 0) {
-            list_by_index<BLOCK>(s, listed);
+            list_by_index<BLOCK>(s, listed, a.size);
             return draw_from_list<BLOCK>(s, o, listed, io.u, a.draws, io.ids, io.prob);
         }
     }
@@ -803,7 +901,7 @@ __global__ void __launch_bounds__(256) sample_short_kernel(const SampleArgs a) {
     const RowIO<T> io(a, blockIdx.x);
     float top = -__builtin_inff(), low = __builtin_inff();
     for_each<BLOCK>(io.row, 0, size, [&](float x, int, int) { top = fmaxf(top, x), low = fminf(low, x); });
-    if (tid < 16) s.tab[tid] = exp2(tid / 16.0);
+    if (tid < 16) s.tab[tid] = kRoots[tid];
     block_max_min<BLOCK>(top, low, s);
     RowState o = row_state(a, blockIdx.x, top, low, s.tab);
     if (o.plain()) {
@@ -822,7 +920,7 @@ __global__ void __launch_bounds__(256) sample_short_kernel(const SampleArgs a) {
         if (key) s.list[atomicAdd(&s.count, 1u)] = by_value(key, i);
     });
     __syncthreads();
-    draw_top_k<BLOCK>(s, o, uniform(s.count), io.u, a.draws, io.ids, io.prob);
+    draw_top_k<BLOCK>(s, o, uniform(s.count), fmaxf(low, -3e38f), size, io.u, a.draws, io.ids, io.prob);
 }
 
 template <typename T>
@@ -835,7 +933,7 @@ __global__ void __launch_bounds__(1024) sample_row_kernel(const SampleArgs a) {
     const RowIO<T> io(a, blockIdx.x);
     float group[4] = {-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()}, low = __builtin_inff();
     for_each<BLOCK>(io.row, 0, size, [&](float x, int, int u) { group[u] = fmaxf(group[u], x), low = fminf(low, x); });
-    if (tid < 16) s.tab[tid] = exp2(tid / 16.0);
+    if (tid < 16) s.tab[tid] = kRoots[tid];
     float top = fmaxf(fmaxf(group[0], group[1]), fmaxf(group[2], group[3]));
     block_max_min<BLOCK>(top, low, s);
     RowState o = row_state(a, blockIdx.x, top, low, s.tab);
@@ -850,11 +948,11 @@ __global__ void __launch_bounds__(1024) sample_row_kernel(const SampleArgs a) {
             if (group[u] > -__builtin_inff()) atomicAdd(&h.cnt[bin_of(o.w, o.scale, group[u])], 1u);
         __syncthreads();
         Above above{0, 0};
-        const int bin = find_bin<BLOCK>(s, h, true, o.f.k, 0.0, above);
+        const int bin = find_bin<BLOCK>(s, h, true, false, o.f.k, 0.0, above);
         if (bin < kBins) {
             gather_list<BLOCK, T>(s, o, io.row, size, 0, bin);
             const uint32_t n = uniform(s.count);
-            if (n <= (uint32_t)kList) return draw_top_k<BLOCK>(s, o, n, io.u, a.draws, io.ids, io.prob);
+            if (n <= (uint32_t)kList) return draw_top_k<BLOCK>(s, o, n, o.w.topf - (float)(bin + 1) / o.scale, size, io.u, a.draws, io.ids, io.prob);
         }
     }
     draw_long_row<BLOCK, T>(s, h, tiles, o, io, a);
@@ -864,7 +962,7 @@ __global__ void __launch_bounds__(1024) sample_row_kernel(const SampleArgs a) {
 template <typename T, int P>
 __global__ void __launch_bounds__(256) sample_wave_kernel(const SampleArgs a) {
     __shared__ double tab[16];
-    if (threadIdx.x < 16) tab[threadIdx.x] = exp2(threadIdx.x / 16.0);
+    if (threadIdx.x < 16) tab[threadIdx.x] = kRoots[threadIdx.x];
     __syncthreads();
     const int lane = threadIdx.x & 63, r = blockIdx.x * 4 + (threadIdx.x >> 6), size = a.size;
     if (r >= a.rows) return;
@@ -949,17 +1047,51 @@ __device__ __forceinline__ RowState state_of(const SampleArgs &a, int r, const R
     return row_state(a, r, uniform(top), uniform(low), tab);
 }
 
-// Whether this block is the last of its row at this point: what the others wrote before is visible to it then.
+// Whether this block is the last of its row at this point: what the others wrote before is visible to it then.  Every wave's
+// stores have left the compute unit before the barrier; one release (a write-back of the XCD's L2) and one acquire a block.
 template <int BLOCK>
 __device__ __forceinline__ bool last_to_arrive(Shared<BLOCK> &s, uint32_t *counter) {
-    __threadfence();
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (threadIdx.x == 0) s.found[0] = atomicAdd(counter, 1u) + 1 == gridDim.x;
+    if (threadIdx.x == 0) {
+        __threadfence();
+        s.found[0] = atomicAdd(counter, 1u) + 1 == gridDim.x;
+        __threadfence();
+    }
     __syncthreads();
     const bool last = uniform((uint32_t)s.found[0]);
     __syncthreads();
-    if (last) __threadfence();
     return last;
+}
+
+// This part's entries of the bins from .. to behind those of the other parts in the row's list (entries beyond kList: counted only).
+template <int BLOCK, typename T>
+__device__ __forceinline__ void gather_part(Shared<BLOCK> &s, const RowState &o, const T *row, Part p, int from, int to, uint64_t *list,
+                            uint32_t *count) {
+    if (threadIdx.x == 0) s.count = 0;
+    __syncthreads();
+    gather<BLOCK, T>(s.list, &s.count, kList, o, row, p.begin, p.end, from, to);
+    __syncthreads();
+    const uint32_t n = uniform(s.count);
+    if (threadIdx.x == 0) s.found[0] = n ? atomicAdd(count, n) : 0;
+    __syncthreads();
+    const uint32_t at = uniform((uint32_t)s.found[0]);
+    for (uint32_t i = threadIdx.x; i < n && i < (uint32_t)kList && at + i < (uint32_t)kList; i += BLOCK) list[at + i] = s.list[i];
+}
+
+// The row's whole list into LDS; its length
+template <int BLOCK>
+__device__ __forceinline__ uint32_t load_list(Shared<BLOCK> &s, const uint64_t *list, const uint32_t *count) {
+    uint64_t c[kList / BLOCK];                             // in flight together with the length
+#pragma unroll
+    for (int j = 0; j < kList / BLOCK; ++j) c[j] = list[j * BLOCK + threadIdx.x];
+    const uint32_t n = uniform(*count);
+#pragma unroll
+    for (int j = 0; j < kList / BLOCK; ++j) s.list[j * BLOCK + threadIdx.x] = c[j];
+    if (threadIdx.x == 0) s.count = n;
+    __syncthreads();
+    return n;
 }
 
 // Stage 1: maximum, minimum, groups' maxima; clears what later stages add to.
@@ -1001,7 +1133,10 @@ __global__ void __launch_bounds__(1024) sample_groups_kernel(const SampleArgs a,
     const int tid = threadIdx.x, r = blockIdx.y;
     RowWork &w = work[r];
     const RowIO<T> io(a, r);
-    if (tid < 16) s.tab[tid] = exp2(tid / 16.0);
+    if (tid < 16) s.tab[tid] = kRoots[tid];
+    float group[kGroups / BLOCK];
+#pragma unroll
+    for (int u = 0; u < kGroups / BLOCK; ++u) group[u] = w.group[u * BLOCK + tid];
     RowState o = state_of(a, r, w, s.tab);
     if (o.plain()) {                                           // the list holds nothing: one block writes the row
         if (blockIdx.x > 0) return;
@@ -1016,20 +1151,17 @@ __global__ void __launch_bounds__(1024) sample_groups_kernel(const SampleArgs a,
     clear_histogram<BLOCK>(h);
 #pragma unroll
     for (int u = 0; u < kGroups / BLOCK; ++u) {
-        const float g = w.group[u * BLOCK + tid];
-        if (g > -__builtin_inff()) atomicAdd(&h.cnt[bin_of(o.w, o.scale, g)], 1u);
+        if (group[u] > -__builtin_inff()) atomicAdd(&h.cnt[bin_of(o.w, o.scale, group[u])], 1u);
     }
     __syncthreads();
     Above above{0, 0};
-    const int bin = find_bin<BLOCK>(s, h, true, o.f.k, 0.0, above);
+    const int bin = find_bin<BLOCK>(s, h, true, false, o.f.k, 0.0, above);
     const Part p = part_of(a.size, blockIdx.x);
-    if (bin < kBins) gather<BLOCK, T>(w.list, &w.count[0], kList, o, io.row, p.begin, p.end, 0, bin);
+    if (bin < kBins) gather_part<BLOCK, T>(s, o, io.row, p, 0, bin, w.list, &w.count[0]);
     if (!last_to_arrive<BLOCK>(s, &w.arrived[0])) return;
-    const uint32_t n = uniform(w.count[0]);
+    const uint32_t n = load_list<BLOCK>(s, w.list, &w.count[0]);
     if (bin < kBins && n <= (uint32_t)kList) {
-        for (int i = tid; i < (int)n; i += BLOCK) s.list[i] = w.list[i];
-        __syncthreads();
-        draw_top_k<BLOCK>(s, o, n, io.u, a.draws, io.ids, io.prob);
+        draw_top_k<BLOCK>(s, o, n, o.w.topf - (float)(bin + 1) / o.scale, a.size, io.u, a.draws, io.ids, io.prob);
         if (tid == 0) w.done = 1;
     } else if (alone) {
         draw_long_row<BLOCK, T>(s, h, tiles, o, io, a);
@@ -1045,7 +1177,7 @@ __global__ void __launch_bounds__(1024) sample_bins_kernel(const SampleArgs a, R
     const int tid = threadIdx.x, r = blockIdx.y;
     RowWork &w = work[r];
     if (w.done) return;
-    if (tid < 16) tab[tid] = exp2(tid / 16.0);
+    if (tid < 16) tab[tid] = kRoots[tid];
     const RowState o = state_of(a, r, w, tab);
     if (o.plain() || !o.f.cut) return;
     clear_histogram<BLOCK>(h);
@@ -1068,7 +1200,7 @@ __global__ void __launch_bounds__(1024) sample_cut_kernel(const SampleArgs a, Ro
     const int tid = threadIdx.x, r = blockIdx.y;
     RowWork &w = work[r];
     if (w.done) return;
-    if (tid < 16) s.tab[tid] = exp2(tid / 16.0);
+    if (tid < 16) s.tab[tid] = kRoots[tid];
     RowState o = state_of(a, r, w, s.tab);
     if (o.plain() || !o.f.cut) return;
     for (int b = tid; b < kBins; b += BLOCK) h.cnt[b] = w.h.cnt[b], h.mass[b] = w.h.mass[b];
@@ -1076,17 +1208,12 @@ __global__ void __launch_bounds__(1024) sample_cut_kernel(const SampleArgs a, Ro
     const RowIO<T> io(a, r);
     const Part p = part_of(a.size, blockIdx.x);
     const Step st = first_step<BLOCK>(s, h, o);
-    if (st.any && st.fits) gather<BLOCK, T>(w.list, &w.count[1], kList, o, io.row, p.begin, p.end, st.from, st.bin);
+    if (st.any && st.fits) gather_part<BLOCK, T>(s, o, io.row, p, st.from, st.bin, w.list, &w.count[1]);
     if (!last_to_arrive<BLOCK>(s, &w.arrived[1])) return;
-    if (st.any && st.fits) {
-        const int n = (int)uniform(w.count[1]);                // as many as the histogram counted: they fit
-        for (int i = tid; i < n; i += BLOCK) s.list[i] = w.list[i];
-        if (tid == 0) s.count = n;
-        __syncthreads();
-    }
+    if (st.any && st.fits) load_list<BLOCK>(s, w.list, &w.count[1]);       // as many as the histogram counted: they fit
     const int listed = select_cut<BLOCK, T>(s, h, o, io.row, a.size, st, st.any && st.fits);
     if (listed > 0) {
-        list_by_index<BLOCK>(s, listed);
+        list_by_index<BLOCK>(s, listed, a.size);
         draw_from_list<BLOCK>(s, o, listed, io.u, a.draws, io.ids, io.prob);
     }
     if (tid == 0) w.done = listed > 0, w.cut = o.f.cut, w.cut_key = o.f.key, w.cut_idx = o.f.idx;
@@ -1107,7 +1234,7 @@ __global__ void __launch_bounds__(256) sample_tiles_kernel(const SampleArgs a, R
     const int tid = threadIdx.x, r = blockIdx.y, tile = tile_of(a.size), n = (a.size + tile - 1) / tile;
     RowWork &w = work[r];
     if (w.done) return;
-    if (tid < 16) s.tab[tid] = exp2(tid / 16.0);
+    if (tid < 16) s.tab[tid] = kRoots[tid];
     __syncthreads();
     const RowState o = cut_state(a, r, w, s.tab);
     if (o.plain()) return;
@@ -1127,7 +1254,7 @@ __global__ void __launch_bounds__(256) sample_draw_kernel(const SampleArgs a, co
     const int tid = threadIdx.x, r = blockIdx.y, tile = tile_of(a.size), n = (a.size + tile - 1) / tile;
     const RowWork &w = work[r];
     if (w.done) return;
-    if (tid < 16) tab[tid] = exp2(tid / 16.0);
+    if (tid < 16) tab[tid] = kRoots[tid];
     const RowState o = cut_state(a, r, w, tab);
     const RowIO<T> io(a, r);
     if (o.plain()) {
