@@ -67,17 +67,15 @@ __constant__ double kRoots[16] = {
 struct Row {
     double top, inv_t;      // M and 1 / T (0 at T = 0)
     float topf;
-    uint32_t top_key;
     bool flat;              // M = +inf or T = 0: mass 1 at M, 0 elsewhere
     const double *tab;      // 2^(j/16), LDS
 };
 
 // exp(y), y = (x - M) / T <= 0: y = (16 q + j) ln2 / 16 + r, |r| <= ln2 / 32, exp = 2^q tab[j] exp(r); the Taylor polynomial of
-// degree 6 leaves r^7 / 5040 < 5e-16.
-__device__ __forceinline__ double mass_of(const Row &w, uint32_t key) {
-    if (key == w.top_key) return 1.0;
-    if (w.flat || key == 0) return 0.0;
-    const double y = fmax(((double)value_of(key) - w.top) * w.inv_t, -800.0);
+// degree 6 leaves r^7 / 5040 < 5e-16.  x = M gives 1 exactly; -inf and NaN end in the clamp's 2^-1154, which is 0.
+__device__ __forceinline__ double mass_of(const Row &w, float x) {
+    if (w.flat) return x == w.topf ? 1.0 : 0.0;
+    const double y = fmax(((double)x - w.top) * w.inv_t, -800.0);
     const double n = __builtin_rint(y * (16.0 * 1.44269504088896340736));
     const double r = fma(n, -0.69314718055994530942 / 16.0, y);
     double s = fma(r, 1.0 / 720.0, 1.0 / 120.0);
@@ -324,9 +322,9 @@ struct Filter {
     __device__ __forceinline__ bool keeps(uint32_t x, int i) const { return x > key || (x == key && i <= idx); }
 };
 
-__device__ __forceinline__ double kept_mass(const Row &w, const Filter &f, uint32_t key, int i) {
-    if (key == 0 || (f.cut && !f.keeps(key, i))) return 0.0;
-    const double e = mass_of(w, key);
+__device__ __forceinline__ double kept_mass(const Row &w, const Filter &f, float x, int i) {
+    if (f.cut && !f.keeps(key_of(x), i)) return 0.0;
+    const double e = mass_of(w, x);
     return e >= f.m ? e : 0.0;
 }
 
@@ -357,7 +355,7 @@ __device__ __forceinline__ RowState row_state(const SampleArgs &a, int r, float 
     o.t = a.temperature_v ? a.temperature_v[r] : a.temperature;
     top += 0.0f;                                           // -0 as +0
     o.valid = top > -__builtin_inff() && o.t >= 0.0f && o.t < __builtin_inff() && p == p && m == m;
-    o.w.topf = top, o.w.top = top, o.w.top_key = key_of(top), o.w.tab = tab;
+    o.w.topf = top, o.w.top = top, o.w.tab = tab;
     o.w.flat = o.t == 0.0f || top == __builtin_inff();
     o.w.inv_t = o.w.flat ? 0.0 : 1.0 / (double)o.t;
     o.f.k = k <= 0 || k > a.size ? a.size : k;
@@ -400,7 +398,7 @@ __device__ __forceinline__ void add_to_histogram(Histogram &h, const RowState &o
         if (key) {
             const int b = bin_of(o.w, o.scale, x);
             atomicAdd(&h.cnt[b], 1u);
-            atomicAdd((unsigned long long *)&h.mass[b], (unsigned long long)fixed(mass_of(o.w, key), o.shift));
+            atomicAdd((unsigned long long *)&h.mass[b], (unsigned long long)fixed(mass_of(o.w, x), o.shift));
         }
     });
 }
@@ -416,7 +414,7 @@ __device__ __forceinline__ int cut_list(Shared<BLOCK> &s, const RowState &o, Fil
     const int i0 = threadIdx.x * kPer;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-        e[j] = i0 + j < n ? fixed(mass_of(o.w, ~(uint32_t)(s.list[i0 + j] >> 32)), o.shift) : 0;
+        e[j] = i0 + j < n ? fixed(mass_of(o.w, value_of(~(uint32_t)(s.list[i0 + j] >> 32))), o.shift) : 0;
         run += e[j];
     }
     unsigned long long all;
@@ -575,7 +573,7 @@ __device__ __forceinline__ void cut_range(Shared<BLOCK> &s, Histogram &h, const 
             const uint32_t key = key_of(x);
             if (key >= lo && key <= hi) {
                 atomicAdd(&h.cnt[(hi - key) >> bits], 1u);
-                atomicAdd((unsigned long long *)&h.mass[(hi - key) >> bits], (unsigned long long)fixed(mass_of(o.w, key), o.shift));
+                atomicAdd((unsigned long long *)&h.mass[(hi - key) >> bits], (unsigned long long)fixed(mass_of(o.w, x), o.shift));
             }
         });
         __syncthreads();
@@ -598,7 +596,7 @@ __device__ __forceinline__ void cut_range(Shared<BLOCK> &s, Histogram &h, const 
         return;
     }
     // one value, more than kList times: the first q of them by index
-    const uint64_t e = fixed(mass_of(o.w, hi), o.shift);
+    const uint64_t e = fixed(mass_of(o.w, value_of(hi)), o.shift);
     uint32_t q = n;
     if (st.by_count) q = f.k - above.cnt;
     else if (e > 0) {
@@ -629,7 +627,7 @@ __device__ __forceinline__ uint64_t mass_of_first(Shared<BLOCK> &s, const RowSta
     unsigned long long mine = 0, all;
     for_each<BLOCK, 1>(row, 0, size, [&](float x, int i, int) {
         const uint32_t key = key_of(x);
-        if (key && o.f.keeps(key, i)) mine += fixed(mass_of(o.w, key), o.shift);
+        if (key && o.f.keeps(key, i)) mine += fixed(mass_of(o.w, x), o.shift);
     });
     block_scan<BLOCK, unsigned long long>(mine, (unsigned long long *)s.wave_u, &all);
     return uniform((uint64_t)all);
@@ -673,7 +671,7 @@ __device__ __forceinline__ int select_cut(Shared<BLOCK> &s, Histogram &h, RowSta
 
 // ---- draws
 __device__ __forceinline__ double mass_or_zero(const RowState &o, uint32_t key) {
-    const double e = mass_of(o.w, key);
+    const double e = mass_of(o.w, value_of(key));
     return e >= o.f.m ? e : 0.0;
 }
 
@@ -741,7 +739,7 @@ __device__ __forceinline__ double lane_masses(const RowState &o, const T *row, i
     double sum = 0.0;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-        e[j] = kept_mass(o.w, o.f, key_of(to_f32(x[j])), i0 + j);
+        e[j] = kept_mass(o.w, o.f, to_f32(x[j]), i0 + j);
         sum += e[j];
         if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // 16 exponentials interleaved need more registers than there are
     }
@@ -970,7 +968,7 @@ __global__ void __launch_bounds__(256) sample_wave_kernel(const SampleArgs a) {
     constexpr int E = 16 / sizeof(T);
     struct __attribute__((packed, aligned(sizeof(T)))) Vec { T e[E]; };
     const int i0 = lane * P;
-    float x[P], top = -__builtin_inff();
+    float x[P], top = -__builtin_inff(), u = io.u[0];
 #pragma unroll
     for (int v = 0; v < P / E; ++v) {
         const int i = i0 + v * E;
@@ -1001,12 +999,12 @@ __global__ void __launch_bounds__(256) sample_wave_kernel(const SampleArgs a) {
     double e[P], sum = 0.0;
 #pragma unroll
     for (int j = 0; j < P; ++j) {
-        e[j] = kept_mass(o.w, o.f, key_of(x[j]), i0 + j);
+        e[j] = kept_mass(o.w, o.f, x[j], i0 + j);
         sum += e[j];
     }
     const double cum = wave_scan(sum), total = __shfl(cum, 63);
     for (int d = 0; d < a.draws; ++d) {
-        const float u = io.u[d];
+        if (d > 0) u = io.u[d];
         int at = 0;
         double mass = 0.0;
         pick_entry<P>(e, sum, cum, 0.0, (double)fminf(fmaxf(u, 0.0f), 1.0f) * total, 0, at, mass);
