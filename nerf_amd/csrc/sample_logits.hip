@@ -165,6 +165,24 @@ __device__ __forceinline__ V wave_scan(V v) {
     v += dpp<0x143, 0xc>(v);      // row_bcast:31 into rows 2 and 3
     return v;
 }
+__device__ __forceinline__ double last_lane(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)b, 63), hi = __builtin_amdgcn_readlane((uint32_t)(b >> 32), 63);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+// Largest of the lanes (the same moves; lanes without a source keep their own value)
+__device__ __forceinline__ float wave_max(float v) {
+#define NRF_DPP_MAX(ctrl, rows) \
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), ctrl, rows, 0xf, false)))
+    NRF_DPP_MAX(0x111, 0xf);
+    NRF_DPP_MAX(0x112, 0xf);
+    NRF_DPP_MAX(0x114, 0xf);
+    NRF_DPP_MAX(0x118, 0xf);
+    NRF_DPP_MAX(0x142, 0xa);
+    NRF_DPP_MAX(0x143, 0xc);
+#undef NRF_DPP_MAX
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
+}
 template <typename V>
 __device__ __forceinline__ V lane_before(V v) { return dpp<0x138, 0xf>(v); }      // wave_shr:1
 
@@ -189,8 +207,7 @@ __device__ __forceinline__ V block_scan(V v, S *sums, V *total) {
 
 template <int BLOCK>
 __device__ __forceinline__ void block_max_min(float &hi, float &lo, Shared<BLOCK> &s) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) hi = fmaxf(hi, __shfl_xor(hi, d)), lo = fminf(lo, __shfl_xor(lo, d));
+    hi = wave_max(hi), lo = -wave_max(-lo);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float *w_hi = reinterpret_cast<float *>(s.wave_a), *w_lo = reinterpret_cast<float *>(s.wave_u);
     if (lane == 0) w_hi[wave] = hi, w_lo[wave] = lo;
@@ -956,58 +973,83 @@ __global__ void __launch_bounds__(1024) sample_row_kernel(const SampleArgs a) {
     draw_long_row<BLOCK, T>(s, h, tiles, o, io, a);
 }
 
-// ---- short rows without a cut: a wave a row, P consecutive entries a lane (rows of up to 64 P entries)
+// Whether a chunk behind c has mass
+template <int C>
+__device__ __forceinline__ bool more_after(const double *all, int c) {
+    bool more = false;
+#pragma unroll
+    for (int k = 0; k < C; ++k) more = more || (k > c && all[k] > 0.0);
+    return more;
+}
+
+// ---- short rows without a cut: a wave a row of up to 64 P entries, in chunks of 16 bytes a lane (entry: chunk, lane, place)
 template <typename T, int P>
 __global__ void __launch_bounds__(256) sample_wave_kernel(const SampleArgs a) {
+    constexpr int E = 16 / sizeof(T), C = P / E;
     __shared__ double tab[16];
-    if (threadIdx.x < 16) tab[threadIdx.x] = kRoots[threadIdx.x];
-    __syncthreads();
-    const int lane = threadIdx.x & 63, r = blockIdx.x * 4 + (threadIdx.x >> 6), size = a.size;
-    if (r >= a.rows) return;
+    const int lane = threadIdx.x & 63, r = min((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6), a.rows - 1), size = a.size;
     const RowIO<T> io(a, r);
-    constexpr int E = 16 / sizeof(T);
     struct __attribute__((packed, aligned(sizeof(T)))) Vec { T e[E]; };
-    const int i0 = lane * P;
-    float x[P], top = -__builtin_inff(), u = io.u[0];
+    float x[C][E], top = -__builtin_inff(), u = io.u[0];
 #pragma unroll
-    for (int v = 0; v < P / E; ++v) {
-        const int i = i0 + v * E;
+    for (int c = 0; c < C; ++c) {
+        const int i = (c * 64 + lane) * E;
         if (i + E <= size) {
             const Vec p = *reinterpret_cast<const Vec *>(io.row + i);
 #pragma unroll
-            for (int j = 0; j < E; ++j) x[v * E + j] = to_f32(p.e[j]);
+            for (int j = 0; j < E; ++j) x[c][j] = to_f32(p.e[j]);
         } else {
 #pragma unroll
-            for (int j = 0; j < E; ++j) x[v * E + j] = i + j < size ? to_f32(io.row[i + j]) : -__builtin_inff();
+            for (int j = 0; j < E; ++j) x[c][j] = i + j < size ? to_f32(io.row[i + j]) : -__builtin_inff();
         }
     }
+    if (threadIdx.x < 16) tab[threadIdx.x] = kRoots[threadIdx.x];
+    __syncthreads();
+    if ((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6) >= a.rows) return;
 #pragma unroll
-    for (int j = 0; j < P; ++j) top = fmaxf(top, x[j]);
+    for (int c = 0; c < C; ++c)
 #pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    const RowState o = row_state(a, r, uniform(top), 0.0f, tab);
+        for (int j = 0; j < E; ++j) top = fmaxf(top, x[c][j]);
+    const RowState o = row_state(a, r, wave_max(top), 0.0f, tab);
     if (o.plain()) {
-        int at = 0;
+        int at = size;
 #pragma unroll
-        for (int j = P - 1; j >= 0; --j) at = x[j] == o.w.topf ? j : at;
-        uint64_t has = 0;
+        for (int c = C - 1; c >= 0; --c) {
+            const int i = (c * 64 + lane) * E;
+            int mine = E;
 #pragma unroll
-        for (int j = 0; j < P; ++j) has |= __ballot(x[j] == o.w.topf);
-        const int src = has ? __builtin_ctzll(has) : 0;
-        return draw_plain(o, src * P + __shfl(at, src), io.u, a.draws, io.ids, io.prob, lane, 64);
+            for (int j = E - 1; j >= 0; --j) mine = x[c][j] == o.w.topf ? j : mine;
+            const uint64_t has = __ballot(mine < E);
+            if (has) at = __builtin_amdgcn_readlane(i + mine, __builtin_ctzll(has));
+        }
+        return draw_plain(o, at, io.u, a.draws, io.ids, io.prob, lane, 64);
     }
-    double e[P], sum = 0.0;
+    double e[C][E], sum[C], cum[C], all[C], total = 0.0;      // per chunk: this lane's mass, with the lanes before, the wave's
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-        e[j] = kept_mass(o.w, o.f, x[j], i0 + j);
-        sum += e[j];
+    for (int c = 0; c < C; ++c) {
+        sum[c] = 0.0;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            e[c][j] = kept_mass(o.w, o.f, x[c][j], (c * 64 + lane) * E + j);
+            sum[c] += e[c][j];
+        }
+        cum[c] = wave_scan(sum[c]);
+        all[c] = last_lane(cum[c]);
+        total += all[c];
     }
-    const double cum = wave_scan(sum), total = __shfl(cum, 63);
     for (int d = 0; d < a.draws; ++d) {
         if (d > 0) u = io.u[d];
+        const double want = (double)fminf(fmaxf(u, 0.0f), 1.0f) * total;
         int at = 0;
-        double mass = 0.0;
-        pick_entry<P>(e, sum, cum, 0.0, (double)fminf(fmaxf(u, 0.0f), 1.0f) * total, 0, at, mass);
+        double mass = 0.0, before = 0.0;
+        bool found = false;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            // the chunk that exceeds; until one does, the last place with mass (all of this is wave-uniform)
+            if (!found && all[c] > 0.0 && (before + all[c] > want || c == C - 1 || !more_after<C>(all, c)))
+                found = pick_entry<E>(e[c], sum[c], cum[c], before, want, c * 64 * E, at, mass);
+            before += all[c];
+        }
         if (lane == 0) {
             io.ids[d] = u == u ? at : -1;
             io.prob[d] = u == u ? (float)(mass / total) : 0.0f;
