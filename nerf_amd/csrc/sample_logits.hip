@@ -31,6 +31,7 @@ constexpr int kBins = 2048, kList = 2048, kGroups = 4096, kMaxTiles = 1024;
 constexpr int kMaxSize = 1 << 28, kMaxRows = 1 << 21;
 constexpr int kParts = 16;                  // blocks of a row, many-block form
 constexpr int kPartsMaxRows = 64;
+constexpr int kCrowd = 160;                 // entries of a bucket from which sort_list falls back
 constexpr int kGroupsMaxK = 1500;           // above it the groups' bound lets more entries through than the list holds
 
 struct SampleArgs {
@@ -257,7 +258,7 @@ __device__ __forceinline__ void sort_list(Shared<BLOCK> &s, int n, F bucket) {
             c[j] = s.list[i];
             b[j] = bucket(c[j]);
             at[j] = atomicAdd(&count[b[j]], 1u);
-            if (at[j] == 64) s.crowded = 1;
+            if (at[j] == kCrowd) s.crowded = 1;
         }
     }
     __syncthreads();
@@ -298,6 +299,7 @@ __device__ __forceinline__ void sort_list(Shared<BLOCK> &s, int n, F bucket) {
         if (j * BLOCK + (int)threadIdx.x < n) {
             const uint32_t lo = count[b[j]], hi = b[j] + 1 < kBins ? count[b[j] + 1] : n;
             place[j] = lo;
+#pragma unroll 8
             for (uint32_t q = lo; q < hi; ++q) place[j] += s.list[q] < c[j];
         }
     __syncthreads();
@@ -534,31 +536,68 @@ __device__ __forceinline__ Step first_step(Shared<BLOCK> &s, const Histogram &h,
     return none;
 }
 
-// Entries of the bins from .. to into list[0 ..), in any order; entries beyond `room` are counted only.
-template <int BLOCK, typename T>
-__device__ __forceinline__ void gather(uint64_t *list, uint32_t *count, uint32_t room, const RowState &o, const T *row, int begin, int end, int from,
-                       int to) {
-    // bin_of(x) >= from and <= to, before the rounding down to whole bins; the last bin has no end
-    const float low = (float)from, high = to == kBins - 1 ? __builtin_inff() : (float)(to + 1);
-    const float top = o.w.topf, scale = o.scale;
-    for_each<BLOCK>(row, begin, end, [&](float x, int i, int) {
-        const float b = fminf((top - x) * scale, (float)(kBins - 1));
-        if (b >= low && b < high) {
-            const uint32_t key = key_of(x);
-            if (key) {
-                const uint32_t at = atomicAdd(count, 1u);
-                if (at < room) list[at] = by_value(key, i);
-            }
-        }
-    });
-}
+// What a list is gathered by: all entries of the bins from .. to, or (a superset of bins 0 .. to) all entries from `least` up.
+struct Reach {
+    int from, to;
+    float least;
+    __device__ __forceinline__ Reach(int f, int t) : from(f), to(t), least(0.0f) {}
+    __device__ __forceinline__ Reach(const RowState &o, int t) : from(-1), to(t) {
+        // the widths of the bins, and some roundings more; never -inf
+        const float width = (float)(t + 1) / o.scale;
+        least = t == kBins - 1 ? -3.402823466e38f : fmaxf(o.w.topf - width * 1.000001f - fabsf(o.w.topf) * 3e-7f, -3.402823466e38f);
+    }
+};
 
+// The entries of a part of a row into list[0 ..), in any order, as by_value; those beyond kList are counted only.  First a mask per
+// thread and 64 bytes, with one reservation for what is set in it, and the indices; then the values by their indices.
 template <int BLOCK, typename T>
-__device__ __forceinline__ void gather_list(Shared<BLOCK> &s, const RowState &o, const T *row, int size, int from, int to) {
+__device__ __forceinline__ uint32_t gather(Shared<BLOCK> &s, const RowState &o, const T *row, int begin, int end, const Reach &want) {
+    constexpr int E = 16 / sizeof(T), U = 4;
+    struct __attribute__((packed, aligned(sizeof(T)))) Vec { T e[E]; };
+    const Vec *v = reinterpret_cast<const Vec *>(row + begin);
+    const int nv = (end - begin) / E;
+    // before the rounding down to whole bins; the last bin has no end
+    const float low = (float)want.from, high = want.to == kBins - 1 ? __builtin_inff() : (float)(want.to + 1);
+    const auto in = [&](float x) {
+        if (want.from < 0) return x >= want.least;
+        const float b = fminf((o.w.topf - x) * o.scale, (float)(kBins - 1));
+        return b >= low && b < high && x > -__builtin_inff();
+    };
+    uint32_t *index = reinterpret_cast<uint32_t *>(s.mass);
     if (threadIdx.x == 0) s.count = 0;
     __syncthreads();
-    gather<BLOCK, T>(s.list, &s.count, kList, o, row, 0, size, from, to);
+    for (int j = threadIdx.x; j < nv; j += BLOCK * U) {
+        Vec p[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) p[u] = v[min(j + u * BLOCK, nv - 1)];
+        uint32_t mask = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) m |= in(to_f32(p[u].e[e])) ? 1u << e : 0u;
+            mask |= j + u * BLOCK < nv ? m << (u * E) : 0u;
+        }
+        if (mask) {
+            uint32_t at = atomicAdd(&s.count, (uint32_t)__popc(mask));
+            do {
+                const int bit = __builtin_ctz(mask);
+                if (at < (uint32_t)kList) index[at] = begin + (j + bit / E * BLOCK) * E + bit % E;
+                ++at;
+                mask &= mask - 1;
+            } while (mask);
+        }
+    }
+    const int i = begin + nv * E + threadIdx.x;
+    if (i < end && in(to_f32(row[i]))) {
+        const uint32_t at = atomicAdd(&s.count, 1u);
+        if (at < (uint32_t)kList) index[at] = i;
+    }
     __syncthreads();
+    const uint32_t n = uniform(s.count);
+    for (uint32_t q = threadIdx.x; q < n && q < (uint32_t)kList; q += BLOCK) s.list[q] = by_value(key_of(to_f32(row[index[q]])), index[q]);
+    __syncthreads();
+    return n;
 }
 
 template <int BLOCK>
@@ -657,9 +696,8 @@ __device__ __forceinline__ int select_cut(Shared<BLOCK> &s, Histogram &h, RowSta
     while (st.any) {
         uint64_t mass_at = 0;
         if (st.fits) {
-            if (!gathered) gather_list<BLOCK, T>(s, o, row, size, st.from, st.bin);
+            const int n = gathered ? uniform(s.count) : gather<BLOCK, T>(s, o, row, 0, size, Reach(st.from, st.bin));
             gathered = false;
-            const int n = uniform(s.count);
             // the bins from .. bin, stretched over the buckets
             sort_by_value<BLOCK>(s, n, o.w.topf - (float)st.from / o.scale, o.scale * ((float)kBins / (float)(st.bin - st.from + 1)));
             int kept;
@@ -965,8 +1003,7 @@ __global__ void __launch_bounds__(1024) sample_row_kernel(const SampleArgs a) {
         Above above{0, 0};
         const int bin = find_bin<BLOCK>(s, h, true, false, o.f.k, 0.0, above);
         if (bin < kBins) {
-            gather_list<BLOCK, T>(s, o, io.row, size, 0, bin);
-            const uint32_t n = uniform(s.count);
+            const uint32_t n = gather<BLOCK, T>(s, o, io.row, 0, size, Reach(o, bin));
             if (n <= (uint32_t)kList) return draw_top_k<BLOCK>(s, o, n, o.w.topf - (float)(bin + 1) / o.scale, size, io.u, a.draws, io.ids, io.prob);
         }
     }
@@ -1105,15 +1142,11 @@ __device__ __forceinline__ bool last_to_arrive(Shared<BLOCK> &s, uint32_t *count
     return last;
 }
 
-// This part's entries of the bins from .. to behind those of the other parts in the row's list (entries beyond kList: counted only).
+// This part's entries behind those of the other parts in the row's list (entries beyond kList: counted only).
 template <int BLOCK, typename T>
-__device__ __forceinline__ void gather_part(Shared<BLOCK> &s, const RowState &o, const T *row, Part p, int from, int to, uint64_t *list,
-                            uint32_t *count) {
-    if (threadIdx.x == 0) s.count = 0;
-    __syncthreads();
-    gather<BLOCK, T>(s.list, &s.count, kList, o, row, p.begin, p.end, from, to);
-    __syncthreads();
-    const uint32_t n = uniform(s.count);
+__device__ __forceinline__ void gather_part(Shared<BLOCK> &s, const RowState &o, const T *row, Part p, const Reach &want, uint64_t *list,
+                                            uint32_t *count) {
+    const uint32_t n = gather<BLOCK, T>(s, o, row, p.begin, p.end, want);
     if (threadIdx.x == 0) s.found[0] = n ? atomicAdd(count, n) : 0;
     __syncthreads();
     const uint32_t at = uniform((uint32_t)s.found[0]);
@@ -1197,7 +1230,7 @@ __global__ void __launch_bounds__(1024) sample_groups_kernel(const SampleArgs a,
     Above above{0, 0};
     const int bin = find_bin<BLOCK>(s, h, true, false, o.f.k, 0.0, above);
     const Part p = part_of(a.size, blockIdx.x);
-    if (bin < kBins) gather_part<BLOCK, T>(s, o, io.row, p, 0, bin, w.list, &w.count[0]);
+    if (bin < kBins) gather_part<BLOCK, T>(s, o, io.row, p, Reach(o, bin), w.list, &w.count[0]);
     if (!last_to_arrive<BLOCK>(s, &w.arrived[0])) return;
     const uint32_t n = load_list<BLOCK>(s, w.list, &w.count[0]);
     if (bin < kBins && n <= (uint32_t)kList) {
@@ -1248,7 +1281,7 @@ __global__ void __launch_bounds__(1024) sample_cut_kernel(const SampleArgs a, Ro
     const RowIO<T> io(a, r);
     const Part p = part_of(a.size, blockIdx.x);
     const Step st = first_step<BLOCK>(s, h, o);
-    if (st.any && st.fits) gather_part<BLOCK, T>(s, o, io.row, p, st.from, st.bin, w.list, &w.count[1]);
+    if (st.any && st.fits) gather_part<BLOCK, T>(s, o, io.row, p, Reach(st.from, st.bin), w.list, &w.count[1]);
     if (!last_to_arrive<BLOCK>(s, &w.arrived[1])) return;
     if (st.any && st.fits) load_list<BLOCK>(s, w.list, &w.count[1]);       // as many as the histogram counted: they fit
     const int listed = select_cut<BLOCK, T>(s, h, o, io.row, a.size, st, st.any && st.fits);
