@@ -45,9 +45,15 @@ class RayBatcher:
     def rows(self, start, stop):
         return self.perm[start:stop]
 
-    def next(self, rank=0, world=1):
+    def slots(self, rows):
+        """Which training image (index into i_train) each table row comes from: the ids of a codes.CodeTable with one code
+        per training image."""
+        return rows // (self.H * self.W)
+
+    def next(self, rank=0, world=1, return_slots=False):
         """-> (batch_rays [2, B, 3], target_s [B, 3]): train.py:183-192.  With world > 1 every rank advances the same
-        permutation and takes its contiguous slice of the global batch (identical stream, disjoint rows)."""
+        permutation and takes its contiguous slice of the global batch (identical stream, disjoint rows).
+        return_slots: also the batch's slots() [B]."""
         rows = self.perm[self.i_batch:self.i_batch + self.N_rand]
         if world > 1:
             from .parallel import slice_partition
@@ -64,6 +70,8 @@ class RayBatcher:
             self.perm = self.perm[idx]
             self.i_batch = 0
             self.epoch += 1
+        if return_slots:
+            return batch_rays, target_s, self.slots(rows)
         return batch_rays, target_s
 
 
@@ -106,3 +114,21 @@ class ImageRaySampler:
         pix = select_inds if cand is None else cand[select_inds]
         rows = pix + int(img_i) * self.H * self.W
         return ops.gather_ray_batch(rows, self.images, self.poses, self.H, self.W, self.K, f64=False)
+
+    def sample_weighted(self, img_i, N_rand, logits, precrop_frac=None, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """N_rand pixels of one image drawn, with replacement, from softmax(logits / temperature) after the filters of
+        sampling.sample_logits -- an error map's logarithm draws the pixels the network still gets wrong (no counterpart in the
+        reference).  logits: one per candidate pixel, in the order of crop_pixels() (all H*W where precrop_frac is None).
+        -> (batch_rays [2, N_rand, 3], target_s [N_rand, 3], pix [N_rand], prob [N_rand]): pix = y*W + x, prob what each was
+        drawn with (weights 1 / (n prob) make a loss unbiased).  Where nothing can be drawn, pix is -1 and the ray NaN."""
+        cand = self.crop_pixels(precrop_frac)
+        n = self.H * self.W if cand is None else cand.numel()
+        if logits.numel() != n:
+            raise ValueError(f"logits: expected one per candidate pixel ({n}), got {tuple(logits.shape)}")
+        u = None if u is None else u.reshape(1, N_rand)
+        ids, prob = ops.sample_logits(logits.reshape(1, n), N_rand, temperature, top_k, top_p, min_p, u)
+        ids, prob = ids[0], prob[0]
+        pix = ids if cand is None else torch.where(ids >= 0, cand[ids.clamp(min=0)], -1)
+        rows = torch.where(pix >= 0, pix + int(img_i) * self.H * self.W, -1)
+        rays, rgb = ops.gather_ray_batch(rows, self.images, self.poses, self.H, self.W, self.K, f64=False)
+        return rays, rgb, pix, prob

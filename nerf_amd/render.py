@@ -49,9 +49,14 @@ def _fusable(fn, embed_fn, embeddirs_fn, viewdirs):
     return True
 
 
-def run_network(inputs, viewdirs, fn, embed_fn, embeddirs_fn, netchunk=1024 * 64):
-    """inputs [..., 3] points, viewdirs [N_rays, 3] or None -> [..., out_ch]."""
-    if _fusable(fn, embed_fn, embeddirs_fn, viewdirs):
+def run_network(inputs, viewdirs, fn, embed_fn, embeddirs_fn, netchunk=1024 * 64, codes=None):
+    """inputs [..., 3] points, viewdirs [N_rays, 3] or None -> [..., out_ch].
+
+    codes [N_rays, d] (codes.CodeTable; no counterpart in the reference): one learned code per ray, appended to the embedded
+    directions, so `fn` is built with input_ch_views = d more than the direction embedder's out_dim.  Differentiable."""
+    if codes is not None and (viewdirs is None or codes.dim() != 2 or codes.shape[0] != viewdirs.shape[0]):
+        raise ValueError("codes: expected one row per ray, beside viewdirs")
+    if codes is None and _fusable(fn, embed_fn, embeddirs_fn, viewdirs):
         flat = inputs.reshape(-1, inputs.shape[-1])
         n_rays = viewdirs.shape[0] if viewdirs is not None else 1
         pts_per_ray = flat.shape[0] // n_rays if viewdirs is not None else 1
@@ -64,6 +69,9 @@ def run_network(inputs, viewdirs, fn, embed_fn, embeddirs_fn, netchunk=1024 * 64
     if viewdirs is not None:
         dirs = viewdirs[:, None].expand(inputs.shape)
         embedded = torch.cat([embedded, embeddirs_fn(torch.reshape(dirs, [-1, dirs.shape[-1]]))], -1)
+        if codes is not None:
+            per_point = codes[:, None].expand(*inputs.shape[:-1], codes.shape[-1])
+            embedded = torch.cat([embedded, per_point.reshape(-1, codes.shape[-1]).to(embedded.dtype)], -1)
     out = batchify(fn, netchunk)(embedded)
     return torch.reshape(out, list(inputs.shape[:-1]) + [out.shape[-1]])
 

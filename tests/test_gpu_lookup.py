@@ -231,3 +231,34 @@ def test_another_stream_and_a_captured_training_step():
         out, grad = step()
         for _, res in graphs:
             assert torch.equal(res[0], out) and torch.equal(res[1], grad), k
+
+
+def test_refusals():
+    from nerf_amd import ops
+    from nerf_amd.codes import lookup
+    table, ids = torch.zeros(4, 8, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    with pytest.raises(TypeError, match="int32 or int64"):
+        ops.lookup_fwd(table, ids.float())
+    with pytest.raises(RuntimeError, match="ids: expected a tensor on"):
+        ops.lookup_fwd(table, ids.cpu())
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        ops.lookup_fwd(table.double(), ids)
+    with pytest.raises(TypeError, match="out_dtype"):
+        ops.lookup_fwd(table, ids, out_dtype=torch.float16)
+    with pytest.raises(ValueError, match="dim >= 1"):
+        ops.lookup_fwd(table[0], ids)
+    with pytest.raises(RuntimeError, match="dim at most"):
+        ops.lookup_fwd(torch.zeros(1, 40000, device="cuda"), ids)
+    g = torch.zeros(3, 8, device="cuda")
+    with pytest.raises(ValueError, match="g_out: expected"):
+        ops.lookup_bwd(g[:2], ids, 4)
+    with pytest.raises(TypeError, match="does not go with"):
+        ops.lookup_bwd(g.half(), ids, 4, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="padding_idx"):
+        ops.lookup_bwd(g, ids, 4, padding_idx=4)
+    # ids changed between forward and backward: autograd's own check speaks
+    t = table.requires_grad_()
+    out = lookup(t, ids)
+    ids.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
