@@ -19,7 +19,7 @@
 // The list (up to 2048 entries) is sorted.  Where it holds everything that is kept, the draws come from it; else from the
 // masses of the row's tiles of 1024 entries.
 //
-// Three forms: short rows without a cut, a wave each; one block a row; and, for few long rows, 16 blocks a row over
+// Three forms: short rows without a cut, a wave each; one block a row; and, for few long rows, 32 blocks a row over
 // several launches (the block that arrives last at a stage's end does what needs the whole row).
 #include "nrf_types.h"
 
@@ -29,8 +29,7 @@ namespace {
 
 constexpr int kBins = 2048, kList = 2048, kGroups = 4096, kMaxTiles = 1024;
 constexpr int kMaxSize = 1 << 28, kMaxRows = 1 << 21;
-constexpr int kParts = 16;                  // blocks of a row, many-block form
-constexpr int kPartsMaxRows = 64;
+constexpr int kParts = 32;                  // blocks of a row, many-block form
 constexpr int kCrowd = 160;                 // entries of a bucket from which sort_list falls back
 constexpr int kGroupsMaxK = 1500;           // above it the groups' bound lets more entries through than the list holds
 
@@ -855,12 +854,12 @@ __device__ __forceinline__ void draw_from_tiles(const RowState &o, const T *row,
                                 int64_t *id, float *prob) {
     const int lane = threadIdx.x & 63;
     const double total = tiles[n_tiles - 1], want = (double)fminf(fmaxf(uj, 0.0f), 1.0f) * total;
-    int a = 0, b = n_tiles - 1;
-    while (a < b) {
-        const int mid = (a + b) >> 1;
-        if (tiles[mid] > want) b = mid;
-        else a = mid + 1;
-    }
+    // the first tile whose running sum exceeds `want` (else the last one): 64 probes, 16 tiles apart, then 16
+    static_assert(kMaxTiles == 64 * 16, "two steps");
+    const uint64_t far = __ballot(tiles[min(lane * 16 + 15, n_tiles - 1)] > want);
+    const int from = (far ? __builtin_ctzll(far) : 63) * 16;
+    const uint64_t near = __ballot(tiles[min(from + (lane & 15), n_tiles - 1)] > want);
+    int a = min(from + (near ? __builtin_ctzll(near) : 15), n_tiles - 1);
     while (a > 0 && tiles[a] <= tiles[a - 1]) --a;       // u = 1: back to the last tile that has mass
     double before = a > 0 ? tiles[a - 1] : 0.0, mass = 0.0, e[16];
     int at = 0;
@@ -1103,8 +1102,7 @@ struct RowWork {
     uint32_t done;                         // the draws are out
     uint32_t cut, cut_key;
     int32_t cut_idx, k;
-    uint32_t pad[6];
-    float group[kGroups];
+    alignas(256) float group[kGroups];
     Histogram h;
     uint64_t list[kList];
     double tiles[kMaxTiles];
@@ -1119,9 +1117,8 @@ __device__ __forceinline__ Part part_of(int size, int part) {
 }
 
 __device__ __forceinline__ RowState state_of(const SampleArgs &a, int r, const RowWork &w, const double *tab) {
-    float top = w.top[0], low = w.low[0];
-    for (int i = 1; i < kParts; ++i) top = fmaxf(top, w.top[i]), low = fminf(low, w.low[i]);
-    return row_state(a, r, uniform(top), uniform(low), tab);
+    const int part = threadIdx.x & (kParts - 1);               // a lane a part
+    return row_state(a, r, wave_max(w.top[part]), -wave_max(-w.low[part]), tab);
 }
 
 // Whether this block is the last of its row at this point: what the others wrote before is visible to it then.  Every wave's
@@ -1178,10 +1175,11 @@ __global__ void __launch_bounds__(1024) sample_max_kernel(const SampleArgs a, Ro
     const Part p = part_of(a.size, part);
     float top = -__builtin_inff(), low = __builtin_inff();
     for_each<BLOCK>(io.row, p.begin, p.end, [&](float x, int, int) { top = fmaxf(top, x), low = fminf(low, x); });
-    float g = fmaxf(top, __shfl_xor(top, 1));
-    g = fmaxf(g, __shfl_xor(g, 2));
-    constexpr int kEach = kGroups / kParts;                    // groups of a part: four threads each
-    if ((tid & 3) == 0) w.group[part * kEach + (tid >> 2)] = g;
+    constexpr int kEach = kGroups / kParts, kOf = BLOCK / kEach;       // groups of a part, threads of a group
+    float g = top;
+#pragma unroll
+    for (int d = 1; d < kOf; d <<= 1) g = fmaxf(g, __shfl_xor(g, d));
+    if (tid % kOf == 0) w.group[part * kEach + tid / kOf] = g;
     for (int b = tid; b < kBins / kParts; b += BLOCK) w.h.cnt[part * (kBins / kParts) + b] = 0, w.h.mass[part * (kBins / kParts) + b] = 0;
     block_max_min<BLOCK>(top, low, s);
     const float t = a.temperature_v ? a.temperature_v[r] : a.temperature;
@@ -1345,9 +1343,12 @@ __global__ void __launch_bounds__(256) sample_draw_kernel(const SampleArgs a, co
 // ---- host
 enum Form { kWaveForm, kShortForm, kRowForm, kPartsForm };
 
+// Long rows: with many of them, a block each fills the chip and is done in one launch; few of them are split.  Measured, one draw,
+// bf16, one block a row against split rows: top-k 50 131072 x 1: 19 / 18 us, 640000 x 1: 46 / 20, 640000 x 32: 55 / 50; top-p 32768 x 1:
+// 40 / 36, 32768 x 16: 41 / 51, 131072 x 16: 116 / 67, 131072 x 64: 117 / 196; no cut 131072 x 1: 45 / 19, x 16: 45 / 30, x 32: 45 / 49.
 Form form_of(int64_t rows, int size, int draws, bool may_cut) {
     if (size <= kList) return !may_cut && draws <= 16 ? kWaveForm : kShortForm;
-    return rows <= kPartsMaxRows ? kPartsForm : kRowForm;
+    return size >= 65536 && rows <= 16 ? kPartsForm : kRowForm;
 }
 
 template <typename T>
@@ -1383,7 +1384,7 @@ void launch_sample(const SampleArgs &a, bool may_k, bool may_p, RowWork *work, h
 }  // namespace
 
 extern "C" int64_t nrf_sample_logits_workspace_bytes(int64_t n_rows, int32_t size) {
-    return size > kList && n_rows <= kPartsMaxRows ? n_rows * (int64_t)sizeof(RowWork) : 0;
+    return form_of(n_rows, size, 1, true) == kPartsForm ? n_rows * (int64_t)sizeof(RowWork) : 0;
 }
 
 extern "C" int nrf_sample_logits(const void *logits, int64_t row_stride, int32_t dtype, int64_t n_rows, int32_t size, int32_t n_draws,

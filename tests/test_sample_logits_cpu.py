@@ -21,8 +21,8 @@ def call(logits=P, stride=100, dtype=0, rows=4, size=100, draws=2, t=1.0, k=0, p
     (dict(stride=-1), 1, "stride"), (dict(t=-0.5), 1, "temperature"), (dict(t=float("inf")), 1, "temperature"),
     (dict(t=float("nan")), 1, "temperature"), (dict(p=float("nan")), 1, "top_p"), (dict(m=1.5), 1, "min_p"),
     (dict(m=float("nan")), 1, "min_p"), (dict(size=2 ** 28 + 1), 2, "2^28"), (dict(rows=2 ** 21 + 1), 2, "2^21"),
-    (dict(rows=2 ** 20, draws=2 ** 11), 2, "2^31"), (dict(size=5000, ws=NULL), 1, "workspace"),
-    (dict(size=5000, ws=C.c_void_p(4100)), 1, "aligned"),
+    (dict(rows=2 ** 20, draws=2 ** 11), 2, "2^31"), (dict(size=70000, ws=NULL), 1, "workspace"),
+    (dict(size=70000, ws=C.c_void_p(4100)), 1, "aligned"),
 ])
 def test_refusals(kw, code, text):
     assert call(**kw) == code
@@ -44,5 +44,5 @@ def test_python_refuses_cpu_tensors():
 
 def test_workspace_sizes():
     f = _lib.lib().nrf_sample_logits_workspace_bytes
-    assert f(1, 2048) == 0 and f(4096, 131072) == 0 and f(0, 5000) == 0
-    assert f(2, 5000) == 2 * f(1, 640000) > 0 and f(1, 5000) % 16 == 0
+    assert f(1, 2048) == 0 and f(4096, 131072) == 0 and f(0, 70000) == 0
+    assert f(2, 70000) == 2 * f(1, 640000) > 0 and f(1, 70000) % 16 == 0
