@@ -93,8 +93,10 @@ void pick_fwd(int vw, const void *table, int64_t stride, int64_t n_rows, const v
 // Pair: x = key (the id; n_rows for tokens that take no part: ids outside the table, the padding id), y = position.
 constexpr int kItems = 16;                  // most items of a thread, one-block sort
 constexpr int kSmall = 1024 * kItems;       // most items the one-block sort takes
-constexpr int kTileItems = 4;               // items of a thread, many-block sort: 1024 threads, two blocks fill a CU's waves
-constexpr int kTile = 1024 * kTileItems;    // items of a block
+constexpr int kTileItems = 4;               // items of a thread, many-block sort: 1024 threads, two blocks fill a CU's waves ...
+constexpr int kFewItems = 2;                // ... and where few blocks have work, when the ranking's chain of items takes the time
+constexpr int kTile = 1024 * kTileItems;
+constexpr int kFewTiles = 64;               // blocks up to which each sums the counters of all (a scan launch costs 5 us)
 constexpr int kMaxDigit = 10;               // bits of a digit: 16 waves' counters and the one-block sort's pairs fit LDS
 
 template <typename I>
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(1024) sort_small_kernel(const I *__restrict__ 
 }
 
 // Many blocks, one digit: counts[block][bin]; the blocks behind the sorting ones write zeros (first digit only).
-template <typename I, bool FIRST>
+template <typename I, bool FIRST, int ITEMS>
 __global__ void __launch_bounds__(1024) sort_count_kernel(const I *__restrict__ ids, const uint2 *__restrict__ in, int64_t n,
                                                           uint32_t n_rows, int64_t padding, int shift, int digit, int tiles,
                                                           uint32_t *__restrict__ counts, void *grad, int64_t grad_bytes) {
@@ -245,16 +247,16 @@ __global__ void __launch_bounds__(1024) sort_count_kernel(const I *__restrict__ 
     __shared__ uint32_t cnt[1 << kMaxDigit];
     const int bins = 1 << digit;
     if ((int)threadIdx.x < bins) cnt[threadIdx.x] = 0;
-    const int64_t i0 = (int64_t)blockIdx.x * kTile + threadIdx.x;
-    uint32_t key[kTileItems];
+    const int64_t i0 = (int64_t)blockIdx.x * (1024 * ITEMS) + threadIdx.x;
+    uint32_t key[ITEMS];
 #pragma unroll
-    for (int k = 0; k < kTileItems; ++k) {
+    for (int k = 0; k < ITEMS; ++k) {
         const int64_t i = i0 + k * 1024 < n ? i0 + k * 1024 : n - 1;
         key[k] = FIRST ? key_of(ids[i], n_rows, padding) : in[i].x;
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kTileItems; ++k)
+    for (int k = 0; k < ITEMS; ++k)
         if (i0 + k * 1024 < n) atomicAdd(&cnt[(key[k] >> shift) & (bins - 1)], 1u);
     __syncthreads();
     if ((int)threadIdx.x < bins) counts[(int64_t)blockIdx.x * bins + threadIdx.x] = cnt[threadIdx.x];
@@ -292,30 +294,42 @@ __global__ void __launch_bounds__(1024) sort_scan_kernel(uint32_t *__restrict__ 
     }
 }
 
-template <typename I, bool FIRST>
+template <typename I, bool FIRST, int ITEMS>
 __global__ void __launch_bounds__(1024) sort_scatter_kernel(const I *__restrict__ ids, const uint2 *__restrict__ in, int64_t n,
                                                             uint32_t n_rows, int64_t padding, int shift, int digit, int tiles,
                                                             const uint32_t *__restrict__ counts,
                                                             const uint32_t *__restrict__ totals, uint2 *__restrict__ out) {
     __shared__ uint32_t base[1 << kMaxDigit];
     __shared__ uint16_t cnt[16][1 << kMaxDigit], start[1 << kMaxDigit];
-    __shared__ uint2 sorted[kTile];
+    __shared__ uint2 sorted[1024 * ITEMS];
     __shared__ uint32_t sums[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int bins = 1 << digit;
-    const int64_t i0 = (int64_t)blockIdx.x * kTile + wave * (64 * kTileItems) + lane;
-    uint2 pair[kTileItems];
+    const int64_t i0 = (int64_t)blockIdx.x * (1024 * ITEMS) + wave * (64 * ITEMS) + lane;
+    uint2 pair[ITEMS];
 #pragma unroll
-    for (int k = 0; k < kTileItems; ++k) {
+    for (int k = 0; k < ITEMS; ++k) {
         const int64_t i = i0 + k * 64 < n ? i0 + k * 64 : n - 1;
         pair[k] = FIRST ? make_uint2(key_of(ids[i], n_rows, padding), (uint32_t)i) : in[i];
     }
-    const uint32_t total = tid < bins ? totals[tid] : 0, before = tid < bins ? counts[(int64_t)blockIdx.x * bins + tid] : 0;
+    uint32_t total = 0, before = 0;
+    if (tid < bins) {
+        if (tiles <= kFewTiles) {                          // no scan launch: the blocks before, and all of them
+#pragma unroll 8
+            for (int t = 0; t < tiles; ++t) {
+                const uint32_t c = counts[t * bins + tid];
+                total += c;
+                before += t < (int)blockIdx.x ? c : 0;
+            }
+        } else {
+            total = totals[tid], before = counts[(int64_t)blockIdx.x * bins + tid];
+        }
+    }
     for (int b = tid; b < 16 * bins; b += 1024) cnt[b >> digit][b & (bins - 1)] = 0;
     const uint32_t first = block_scan<16>(total, sums);        // first place of bin `tid` (ends in a barrier)
-    uint32_t rank[kTileItems];
+    uint32_t rank[ITEMS];
 #pragma unroll
-    for (int k = 0; k < kTileItems; ++k) rank[k] = wave_rank(cnt[wave], (pair[k].x >> shift) & (bins - 1), digit, i0 + k * 64 < n);
+    for (int k = 0; k < ITEMS; ++k) rank[k] = wave_rank(cnt[wave], (pair[k].x >> shift) & (bins - 1), digit, i0 + k * 64 < n);
     __syncthreads();
     uint32_t mine = 0;
     if (tid < bins) {
@@ -334,15 +348,15 @@ __global__ void __launch_bounds__(1024) sort_scatter_kernel(const I *__restrict_
     __syncthreads();
     // in the order of the output through LDS: neighbouring lanes then write neighbouring places
 #pragma unroll
-    for (int k = 0; k < kTileItems; ++k)
+    for (int k = 0; k < ITEMS; ++k)
         if (i0 + k * 64 < n) {
             const uint32_t d = (pair[k].x >> shift) & (bins - 1);
             sorted[start[d] + cnt[wave][d] + rank[k]] = pair[k];
         }
     __syncthreads();
-    const int64_t left = n - (int64_t)blockIdx.x * kTile;
+    const int64_t left = n - (int64_t)blockIdx.x * (1024 * ITEMS);
 #pragma unroll
-    for (int k = 0; k < kTileItems; ++k) {
+    for (int k = 0; k < ITEMS; ++k) {
         const int i = k * 1024 + tid;
         if (i < left) {
             const uint2 v = sorted[i];
@@ -365,6 +379,7 @@ struct SumArgs {
 };
 
 constexpr int kBatch = 8;      // rows of g that a team has in flight
+constexpr int kAlone = 4;      // batches of partial sums that a team adds alone
 
 template <typename G, typename T, int VW>
 __device__ __forceinline__ void store_row(const SumArgs &a, uint32_t key, int col, const float *acc) {
@@ -462,7 +477,7 @@ __device__ __forceinline__ void add_heads(const SumArgs &a, int64_t s0, int64_t 
 }
 
 // Runs that cross tiles: the team of the tile a run starts in adds tail[tile] and head[tile + 1 ..]; where the run covers more
-// than kBatch further tiles, the block's teams take a slice of them each and the slices are added in order.
+// than kAlone * kBatch further tiles, the block's teams take a slice of them each and the slices are added in order.
 template <typename G, typename T, int VW>
 __global__ void __launch_bounds__(256) sum_join_kernel(const SumArgs a) {
     __shared__ int long_team[256], long_count;
@@ -479,21 +494,33 @@ __global__ void __launch_bounds__(256) sum_join_kernel(const SumArgs a) {
         owner = cur < a.n_rows && a.pairs[i1].x == cur && !(i0 > 0 && a.pairs[i0 - 1].x == cur);
     }
     if (owner) {
-        // the run's tiles are those whose first token carries its id; the first kBatch of them here
-        uint32_t key[kBatch + 1];
-#pragma unroll
-        for (int k = 0; k <= kBatch; ++k) key[k] = a.pairs[(t + 1 + k < a.tiles ? t + 1 + k : a.tiles - 1) * a.tile].x;
-        int more = 0;
-#pragma unroll
-        for (int k = 0; k <= kBatch; ++k) more += t + 1 + k < a.tiles && key[k] == cur;     // sorted: a prefix
-        if (more <= kBatch) {
+        const int64_t far = t + 1 + kAlone * kBatch;
+        if (far < a.tiles && a.pairs[far * a.tile].x == cur) {
+            if (lane == 0) long_team[atomicAdd(&long_count, 1)] = team;
+        } else {
+            // the run's tiles are those whose first token carries its id: batches, keys and sums together
             float acc[VW];
 #pragma unroll
             for (int j = 0; j < VW; ++j) acc[j] = a.tail[t * a.dim + at.col + j];
-            add_heads<VW>(a, t + 1, t + 1 + more, at.col, acc);
+            bool more = true;
+            for (int64_t q = t + 1; more && q < far; q += kBatch) {
+                uint32_t key[kBatch];
+                float v[kBatch][VW];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    const int64_t e = q + k < a.tiles ? q + k : a.tiles - 1;
+                    key[k] = a.pairs[e * a.tile].x;
+#pragma unroll
+                    for (int j = 0; j < VW; ++j) v[k][j] = a.head[e * a.dim + at.col + j];     // unwritten behind the run's end: unused
+                }
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    more = more && q + k < a.tiles && key[k] == cur;
+#pragma unroll
+                    for (int j = 0; j < VW; ++j) acc[j] = more ? acc[j] + v[k][j] : acc[j];
+                }
+            }
             store_row<G, T, VW>(a, cur, at.col, acc);
-        } else if (lane == 0) {
-            long_team[atomicAdd(&long_count, 1)] = team;
         }
     }
     __syncthreads();
@@ -535,21 +562,27 @@ __global__ void __launch_bounds__(256) sum_join_kernel(const SumArgs a) {
     }
 }
 
-// ---------------------------------------------------------------------------------------------------- few rows, few tokens
-// One launch, no workspace: a block takes a row (and up to 256 vectors of its columns), lists the tokens that name it, in order,
+// ---------------------------------------------------------------------------------------------------- few tokens
+// No sort, no workspace: a block takes a row (and up to 256 vectors of its columns), lists the tokens that name it, in order,
 // in LDS, and adds their rows of g: teams of threads take every teams-th listed token, their sums are added in order.
-// Every block reads all ids, and one block may have to read all of g: for small sizes only (few_rows below).
+// BY_TOKEN: the rows are those that the tokens name, each seen to by its first token's block (the zeros are there already);
+// otherwise all rows of the table, in one launch.
+// Every block reads all ids, and one block may have to read all of g: for small sizes only (few_tokens below).
 constexpr int kScanIds = 16;                           // ids of a thread per round
 constexpr int kScanRound = 256 * kScanIds;
 
-template <typename G, typename T, int VW, typename I>
+__global__ void __launch_bounds__(1024) zero_kernel(char *grad, int64_t bytes) { fill_zero(grad, bytes, blockIdx.x); }
+
+template <typename G, typename T, int VW, typename I, bool BY_TOKEN>
 __global__ void __launch_bounds__(256) sum_rows_kernel(const SumArgs a, const I *__restrict__ ids, int64_t padding) {
     __shared__ uint16_t list[kScanRound];
     __shared__ uint32_t waves[4];
     __shared__ float part[256 * VW];
     const int teams = 256 / a.lanes, team = threadIdx.x / a.lanes, lane = threadIdx.x - team * a.lanes;
-    const int row = blockIdx.x / a.chunks, col = ((int)(blockIdx.x - row * a.chunks) * a.lanes + lane) * VW;
+    const int which = blockIdx.x / a.chunks, col = ((int)(blockIdx.x - which * a.chunks) * a.lanes + lane) * VW;
     const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63, n = (int)a.n;
+    const int64_t row = BY_TOKEN ? (int64_t)ids[which] : which;
+    if (BY_TOKEN && ((uint64_t)row >= (uint64_t)a.n_rows || row == padding)) return;
     const bool works = team < teams && col < a.dim;
     const G *g = (const G *)a.g + (works ? col : 0);
     float acc[VW];
@@ -582,6 +615,7 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const SumArgs a, const I 
             at += __popcll(hits[k]);
         }
         __syncthreads();
+        if (BY_TOKEN && i0 == 0 && list[0] != which) return;           // an earlier token sees to the row
         if (works)
             for (uint32_t q = team; q < total; q += kBatch * teams) {
                 Pack<G, VW> v[kBatch];
@@ -604,7 +638,7 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const SumArgs a, const I 
         for (int w = 1; w < teams; ++w)
 #pragma unroll
             for (int j = 0; j < VW; ++j) acc[j] += part[(w * a.lanes + lane) * VW + j];
-        store_row<G, T, VW>(a, row, col, acc);
+        store_row<G, T, VW>(a, (uint32_t)row, col, acc);
     }
 }
 
@@ -612,23 +646,36 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const SumArgs a, const I 
 struct BwdPlan {
     int passes, digit;         // of the sort
     int64_t sort_tiles;        // blocks of the many-block sort (0: one block)
+    int sort_items;            // items of a thread in it
     int tile;                  // tokens of a sum tile
     int64_t sum_tiles;
-    int64_t off_a, off_b, off_counts, off_totals, off_head, off_tail, bytes;       // all zero: few_rows, no workspace
+    int64_t off_a, off_b, off_counts, off_totals, off_head, off_tail, bytes;       // all zero: few tokens, no workspace
 };
 
-// Few rows and tokens: one block a row beats sort, sums and join (4096 tokens of 32 columns, 100 rows: FEW_US us against SORT_US), while
-// the ids are read once a row and a block may meet all of g.  The bounds keep both below a few microseconds.
-bool few_rows(int64_t n, int64_t n_rows, int dim) { return n_rows * n <= 1 << 22 && n * dim <= 1 << 17 && n_rows * dim <= 1 << 20; }
+// Few tokens: without a sort (one or two launches against three or more).  The ids are read once a row or token, and a block may
+// meet all of g: each of its teams then 128 tokens at most, about 10 us.
+// Measured, us a call, against the sorted way: 4096 tokens x 32 over 100 rows 9.0 / 16.5, all on one row 10.2 / 17.7; 16384 x 8 over
+// 256 rows 11.7 / 31; 64 x 1024 over 1024 rows 9.2 / 16.2.
+enum Few { kNotFew, kFewRows, kFewTokens };
+Few few_tokens(int64_t n, int64_t n_rows, int dim) {
+    const int vw = dim % 4 == 0 ? 4 : dim % 2 == 0 ? 2 : 1, lanes = dim / vw < 256 ? dim / vw : 256;
+    const int chunks = (dim / vw + 255) / 256;
+    if (n > 128 * (256 / lanes)) return kNotFew;
+    if (n_rows * chunks <= 4096 && n_rows * n <= 1 << 22) return kFewRows;
+    return n <= 4096 ? kFewTokens : kNotFew;
+}
 
 BwdPlan plan_bwd(int64_t n, int64_t n_rows, int dim) {
     BwdPlan p{};
-    if (few_rows(n, n_rows, dim)) return p;
+    if (few_tokens(n, n_rows, dim) != kNotFew) return p;
     int bits = 1;
     while (bits < 32 && (n_rows >> bits) != 0) ++bits;     // keys go up to n_rows itself
     p.passes = (bits + kMaxDigit - 1) / kMaxDigit;
     p.digit = (bits + p.passes - 1) / p.passes;
-    p.sort_tiles = n <= kSmall ? 0 : (n + kTile - 1) / kTile;
+    // one block sorts a tile's worth, and more while the zeros of a large gradient hide it (65 us for 16384 tokens)
+    const bool one_block = n <= kTile || (n <= kSmall && n_rows * dim >= 1 << 28);
+    p.sort_items = n <= (int64_t)kFewTiles * 1024 * kFewItems ? kFewItems : kTileItems;
+    p.sort_tiles = one_block ? 0 : (n + 1024 * p.sort_items - 1) / (1024 * p.sort_items);
     // enough teams to fill the chip (8 waves on each of 256 CUs), yet tiles long enough that few runs cross them
     p.tile = 64;
     const int64_t vectors = (dim + 3) / 4;
@@ -646,6 +693,36 @@ BwdPlan plan_bwd(int64_t n, int64_t n_rows, int dim) {
     return p;
 }
 
+template <typename I, int ITEMS>
+const uint2 *sort_many(const BwdPlan &p, const I *ids, int64_t n, int64_t n_rows, int64_t padding, char *ws, void *grad,
+                       int64_t grad_bytes, hipStream_t s) {
+    const int fill = (int)((grad_bytes + kFill - 1) / kFill);
+    uint2 *a = (uint2 *)(ws + p.off_a), *b = (uint2 *)(ws + p.off_b);
+    uint32_t *counts = (uint32_t *)(ws + p.off_counts), *totals = (uint32_t *)(ws + p.off_totals);
+    const int tiles = (int)p.sort_tiles, bins = 1 << p.digit;
+    const uint2 *in = nullptr;
+    uint2 *out = p.passes % 2 ? a : b;                          // the last pass ends in a
+    for (int d = 0; d < p.passes; ++d) {
+        const int shift = d * p.digit;
+        if (d == 0)
+            sort_count_kernel<I, true, ITEMS><<<tiles + fill, 1024, 0, s>>>(ids, nullptr, n, (uint32_t)n_rows, padding, 0, p.digit,
+                                                                            tiles, counts, grad, grad_bytes);
+        else
+            sort_count_kernel<I, false, ITEMS><<<tiles, 1024, 0, s>>>(ids, in, n, (uint32_t)n_rows, padding, shift, p.digit, tiles,
+                                                                      counts, nullptr, 0);
+        if (tiles > kFewTiles) sort_scan_kernel<<<(bins + 63) / 64, 1024, 0, s>>>(counts, totals, bins, tiles);
+        if (d == 0)
+            sort_scatter_kernel<I, true, ITEMS><<<tiles, 1024, 0, s>>>(ids, nullptr, n, (uint32_t)n_rows, padding, 0, p.digit, tiles,
+                                                                       counts, totals, out);
+        else
+            sort_scatter_kernel<I, false, ITEMS><<<tiles, 1024, 0, s>>>(ids, in, n, (uint32_t)n_rows, padding, shift, p.digit, tiles,
+                                                                        counts, totals, out);
+        in = out;
+        out = out == a ? b : a;
+    }
+    return in;
+}
+
 template <typename I>
 const uint2 *sort_pairs(const BwdPlan &p, const I *ids, int64_t n, int64_t n_rows, int64_t padding, char *ws, void *grad,
                         int64_t grad_bytes, hipStream_t s) {
@@ -656,28 +733,8 @@ const uint2 *sort_pairs(const BwdPlan &p, const I *ids, int64_t n, int64_t n_row
                                                                        a, grad, grad_bytes);
         return a;
     }
-    uint32_t *counts = (uint32_t *)(ws + p.off_counts), *totals = (uint32_t *)(ws + p.off_totals);
-    const int tiles = (int)p.sort_tiles, bins = 1 << p.digit;
-    const uint2 *in = nullptr;
-    uint2 *out = p.passes % 2 ? a : b;                          // the last pass ends in a
-    for (int d = 0; d < p.passes; ++d) {
-        if (d == 0)
-            sort_count_kernel<I, true><<<tiles + fill, 1024, 0, s>>>(ids, nullptr, n, (uint32_t)n_rows, padding, 0, p.digit, tiles,
-                                                                    counts, grad, grad_bytes);
-        else
-            sort_count_kernel<I, false><<<tiles, 1024, 0, s>>>(ids, in, n, (uint32_t)n_rows, padding, d * p.digit, p.digit, tiles,
-                                                              counts, nullptr, 0);
-        sort_scan_kernel<<<(bins + 63) / 64, 1024, 0, s>>>(counts, totals, bins, tiles);
-        if (d == 0)
-            sort_scatter_kernel<I, true><<<tiles, 1024, 0, s>>>(ids, nullptr, n, (uint32_t)n_rows, padding, 0, p.digit, tiles,
-                                                               counts, totals, out);
-        else
-            sort_scatter_kernel<I, false><<<tiles, 1024, 0, s>>>(ids, in, n, (uint32_t)n_rows, padding, d * p.digit, p.digit, tiles,
-                                                                counts, totals, out);
-        in = out;
-        out = out == a ? b : a;
-    }
-    return in;
+    return p.sort_items == kFewItems ? sort_many<I, kFewItems>(p, ids, n, n_rows, padding, ws, grad, grad_bytes, s)
+                                     : sort_many<I, kTileItems>(p, ids, n, n_rows, padding, ws, grad, grad_bytes, s);
 }
 
 template <typename G, typename T, int VW>
@@ -685,9 +742,18 @@ void launch_sums(SumArgs a, const BwdPlan &p, const void *ids, bool i64, int64_t
     const int vectors = a.dim / VW;
     a.chunks = (vectors + 255) / 256, a.lanes = (vectors + a.chunks - 1) / a.chunks, a.tiles = p.sum_tiles;
     if (p.bytes == 0) {
-        const unsigned blocks = a.n_rows * a.chunks;
-        if (i64) sum_rows_kernel<G, T, VW, int64_t><<<blocks, 256, 0, s>>>(a, (const int64_t *)ids, padding);
-        else sum_rows_kernel<G, T, VW, int32_t><<<blocks, 256, 0, s>>>(a, (const int32_t *)ids, padding);
+        if (few_tokens(a.n, a.n_rows, a.dim) == kFewRows) {
+            const unsigned blocks = a.n_rows * a.chunks;
+            if (i64) sum_rows_kernel<G, T, VW, int64_t, false><<<blocks, 256, 0, s>>>(a, (const int64_t *)ids, padding);
+            else sum_rows_kernel<G, T, VW, int32_t, false><<<blocks, 256, 0, s>>>(a, (const int32_t *)ids, padding);
+            return;
+        }
+        const int64_t bytes = (int64_t)a.n_rows * a.dim * (int64_t)sizeof(T);
+        zero_kernel<<<(unsigned)((bytes + kFill - 1) / kFill), 1024, 0, s>>>((char *)a.grad, bytes);
+        const unsigned blocks = (unsigned)a.n * a.chunks;
+        if (blocks == 0) return;
+        if (i64) sum_rows_kernel<G, T, VW, int64_t, true><<<blocks, 256, 0, s>>>(a, (const int64_t *)ids, padding);
+        else sum_rows_kernel<G, T, VW, int32_t, true><<<blocks, 256, 0, s>>>(a, (const int32_t *)ids, padding);
         return;
     }
     const int teams = 256 / a.lanes;
@@ -741,8 +807,8 @@ extern "C" int nrf_lookup_fwd(const void *table, int64_t table_stride, int32_t d
 
 static int bwd_shape(int64_t n, int64_t n_rows, int32_t dim) {
     NRF_REQUIRE(n >= 0 && n_rows >= 0 && dim >= 1, "nrf_lookup_bwd: n %lld, n_rows %lld, dim %d", (long long)n, (long long)n_rows, dim);
-    if (dim > kMaxDim || n > INT32_MAX || n_rows >= INT32_MAX || (n * dim) >> 33)
-        return fail(NRF_ERR_UNSUPPORTED, "nrf_lookup_bwd: dim at most %d, n and n_rows below 2^31, n * dim below 2^33", kMaxDim);
+    if (dim > kMaxDim || n > INT32_MAX || n_rows >= INT32_MAX || (n * dim) >> 33 || (n_rows * dim) >> 33)
+        return fail(NRF_ERR_UNSUPPORTED, "nrf_lookup_bwd: dim at most %d, n and n_rows below 2^31, n * dim and n_rows * dim below 2^33", kMaxDim);
     return NRF_OK;
 }
 

@@ -61,7 +61,7 @@ def check_bwd(g, ids, V, scale, pad, grad):
 
 # n, V, D: one token, one column, odd sizes, rows that are not 16-byte multiples, wide rows, sizes around the sorts' borders
 SHAPES = [(1, 1, 1), (1, 7, 48), (3, 2, 5), (64, 100, 32), (65, 100, 33), (1000, 3, 27), (4097, 300, 8), (300, 70000, 4),
-          (16384, 1025, 12), (16385, 1500, 16), (20000, 5, 2), (50001, 4096, 3), (33, 1000, 4096), (40, 9, 1111), (2, 3, 32768)]
+          (900, 100000, 4), (1024, 4097, 9), (2440, 9464, 8), (4096, 50000, 3), (300001, 600000, 2), (4100, 5000, 33), (16384, 1025, 12), (16385, 1500, 16), (20000, 5, 2), (50001, 4096, 3), (33, 1000, 4096), (40, 9, 1111), (2, 3, 32768)]
 
 
 @pytest.mark.parametrize("n,V,D", SHAPES)
@@ -165,6 +165,25 @@ def test_gradient_of_many_tokens_on_few_rows():
     grad = ops.lookup_bwd(g, ids, V)
     check_bwd(g, ids, V, 1.0, None, grad)
     assert torch.equal(grad, ops.lookup_bwd(g, ids, V))
+
+
+@pytest.mark.parametrize("kind", ["zipf", "one"])
+def test_gradient_of_a_large_table(kind):
+    """2^28 elements: the sort of 16384 tokens beside the zeros; compared row by row on the GPU, in f64."""
+    from nerf_amd import ops
+    rng = np.random.RandomState(12)
+    n, V, D = 16384, 131072, 2048
+    ids = make_ids(kind, n, V, rng).cuda()
+    g = torch.from_numpy(rng.normal(size=(n, D)).astype(np.float32)).cuda().bfloat16()
+    grad = ops.lookup_bwd(g, ids, V, 0.5)
+    rows, inverse, count = torch.unique(ids, return_inverse=True, return_counts=True)
+    want = torch.zeros(len(rows), D, dtype=torch.float64, device="cuda").index_add_(0, inverse, g.double()) * 0.5
+    mass = torch.zeros(len(rows), D, dtype=torch.float64, device="cuda").index_add_(0, inverse, g.double().abs()) * 0.5
+    tol = (count[:, None] * 2.0 ** -24 * mass + 2.0 ** -8 * want.abs()) * (1 + 1e-3)
+    assert ((grad[rows].double() - want).abs() <= tol).all()
+    grad[rows] = 0
+    assert int((grad != 0).sum()) == 0
+    assert torch.equal(ops.lookup_bwd(g, ids, V, 0.5)[rows], ops.lookup_bwd(g, ids, V, 0.5)[rows])
 
 
 def test_autograd_and_differences():

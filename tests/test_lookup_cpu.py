@@ -40,6 +40,7 @@ def test_forward_refusals(kw, code, text):
     (dict(ws=C.c_void_p(4097)), 1, "aligned"), (dict(stride=7), 1, "stride"), (dict(dim=0), 1, "dim"), (dict(n=-1), 1, "n -1"),
     (dict(dtype=1, g_dtype=2), 2, "type"), (dict(dtype=0, g_dtype=1), 2, "type"), (dict(dtype=9), 1, "dtype"),
     (dict(dim=32769, stride=32769), 2, "dim at most"), (dict(n=2 ** 31), 2, "2^31"), (dict(n_rows=2 ** 31 - 1), 2, "2^31"),
+    (dict(n_rows=2 ** 30), 2, "n_rows * dim"),
 ])
 def test_gradient_refusals(kw, code, text):
     assert bwd(**kw) == code
@@ -53,10 +54,10 @@ def test_nothing_to_do_launches_nothing():
 
 def test_workspace_sizes():
     f = _lib.lib().nrf_lookup_bwd_workspace_bytes
-    assert f(0, 10, 4) >= 0 and f(4096, 100, 32) == 0          # few rows and tokens: one launch, no workspace
+    assert f(0, 10, 4) >= 0 and f(4096, 5000, 32) == 0         # few tokens: no sort, no workspace
     assert f(-1, 10, 4) == -1 and f(10, 10, 0) == -1 and f(10, 10, 32769) == -1 and f(2 ** 31, 10, 1) == -1
     # pairs of (id, position), twice for more than one pass, and two partial sums a tile: within a small multiple of the input
-    for n, rows, dim in ((4096, 5000, 32), (786432, 200, 33), (2097152, 524288, 2), (16384, 131072, 4096)):
+    for n, rows, dim in ((9000, 5000, 32), (786432, 200, 33), (2097152, 524288, 2), (16384, 131072, 4096)):
         assert n * 8 <= f(n, rows, dim) <= n * 24 + n * dim * 4 + (1 << 24)
 
 
