@@ -405,8 +405,8 @@ int nrf_lookup_bwd(const void *g_out, int64_t g_stride, int32_t g_dtype, const v
  * -inf and NaN logits are never drawn; +inf logits share the whole mass.  id -1, prob 0: a row in which nothing can be drawn, a
  * row whose temperature is negative or not finite or whose top_p or min_p is NaN, a u that is NaN.  u outside [0, 1] is clamped;
  * a min_p of a row above 1 is taken as 1.  size <= 2^28, n_rows <= 2^21.
- * workspace: nrf_sample_logits_workspace_bytes (0 for short or many rows: may be NULL then), 16-byte aligned. */
-int64_t nrf_sample_logits_workspace_bytes(int64_t n_rows, int32_t size);
+ * workspace: nrf_sample_logits_workspace_bytes (0 for short rows and for many: may be NULL then), 16-byte aligned. */
+int64_t nrf_sample_logits_workspace_bytes(int64_t n_rows, int32_t size, int32_t n_draws);
 int nrf_sample_logits(const void *logits, int64_t row_stride, int32_t dtype, int64_t n_rows, int32_t size, int32_t n_draws,
                       float temperature, int32_t top_k, float top_p, float min_p, const float *temperature_rows,
                       const int32_t *top_k_rows, const float *top_p_rows, const float *min_p_rows, const float *u, int64_t *ids,

@@ -126,7 +126,7 @@ _SIGS = {
                                  vp, C.c_int32, vp, vp]),
     "nrf_sample_logits": (C.c_int, [vp, C.c_int64, C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_float, C.c_int32, C.c_float,
                                     C.c_float, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
-    "nrf_sample_logits_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int32]),
+    "nrf_sample_logits_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int32, C.c_int32]),
     "nrf_sample_pdf": (C.c_int, [vp, vp, C.c_int64, C.c_int32, C.c_int32, vp, vp, vp]),
 }
 

@@ -653,14 +653,14 @@ struct BwdPlan {
 };
 
 // Few tokens: without a sort (one or two launches against three or more).  The ids are read once a row or token, and a block may
-// meet all of g: each of its teams then 128 tokens at most, about 10 us.
+// meet all of g: each of its teams then 256 tokens at most, about 20 us.
 // Measured, us a call, against the sorted way: 4096 tokens x 32 over 100 rows 9.0 / 16.5, all on one row 10.2 / 17.7; 16384 x 8 over
 // 256 rows 11.7 / 31; 64 x 1024 over 1024 rows 9.2 / 16.2.
 enum Few { kNotFew, kFewRows, kFewTokens };
 Few few_tokens(int64_t n, int64_t n_rows, int dim) {
     const int vw = dim % 4 == 0 ? 4 : dim % 2 == 0 ? 2 : 1, lanes = dim / vw < 256 ? dim / vw : 256;
     const int chunks = (dim / vw + 255) / 256;
-    if (n > 128 * (256 / lanes)) return kNotFew;
+    if (n > 256 * (256 / lanes)) return kNotFew;
     if (n_rows * chunks <= 4096 && n_rows * n <= 1 << 22) return kFewRows;
     return n <= 4096 ? kFewTokens : kNotFew;
 }

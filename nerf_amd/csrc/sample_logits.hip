@@ -1346,9 +1346,12 @@ enum Form { kWaveForm, kShortForm, kRowForm, kPartsForm };
 // Long rows: with many of them, a block each fills the chip and is done in one launch; few of them are split.  Measured, one draw,
 // bf16, one block a row against split rows: top-k 50 131072 x 1: 19 / 18 us, 640000 x 1: 46 / 20, 640000 x 32: 55 / 50; top-p 32768 x 1:
 // 40 / 36, 32768 x 16: 41 / 51, 131072 x 16: 116 / 67, 131072 x 64: 117 / 196; no cut 131072 x 1: 45 / 19, x 16: 45 / 30, x 32: 45 / 49.
+// One block draws 16 at a time where the list does not hold all that is kept: one row of 37446, top-p, 16 draws 50 / 38, 64: 71 / 38, 2181:
+// 972 / 40.
 Form form_of(int64_t rows, int size, int draws, bool may_cut) {
     if (size <= kList) return !may_cut && draws <= 16 ? kWaveForm : kShortForm;
-    return size >= 65536 && rows <= 16 ? kPartsForm : kRowForm;
+    if (rows <= 16) return size >= 65536 || draws > 16 ? kPartsForm : kRowForm;
+    return rows <= 64 && draws > 256 ? kPartsForm : kRowForm;
 }
 
 template <typename T>
@@ -1383,8 +1386,8 @@ void launch_sample(const SampleArgs &a, bool may_k, bool may_p, RowWork *work, h
 
 }  // namespace
 
-extern "C" int64_t nrf_sample_logits_workspace_bytes(int64_t n_rows, int32_t size) {
-    return form_of(n_rows, size, 1, true) == kPartsForm ? n_rows * (int64_t)sizeof(RowWork) : 0;
+extern "C" int64_t nrf_sample_logits_workspace_bytes(int64_t n_rows, int32_t size, int32_t n_draws) {
+    return form_of(n_rows, size, n_draws, true) == kPartsForm ? n_rows * (int64_t)sizeof(RowWork) : 0;
 }
 
 extern "C" int nrf_sample_logits(const void *logits, int64_t row_stride, int32_t dtype, int64_t n_rows, int32_t size, int32_t n_draws,
@@ -1406,7 +1409,7 @@ extern "C" int nrf_sample_logits(const void *logits, int64_t row_stride, int32_t
     a.temperature_v = temperature_rows, a.top_k_v = top_k_rows, a.top_p_v = top_p_rows, a.min_p_v = min_p_rows;
     a.temperature = temperature, a.top_k = top_k, a.top_p = top_p, a.min_p = min_p;
     a.rows = (int)n_rows, a.size = size, a.draws = n_draws, a.ids = ids, a.prob = prob;
-    NRF_REQUIRE(workspace || nrf_sample_logits_workspace_bytes(n_rows, size) == 0, "nrf_sample_logits: null pointer (workspace)");
+    NRF_REQUIRE(workspace || nrf_sample_logits_workspace_bytes(n_rows, size, n_draws) == 0, "nrf_sample_logits: null pointer (workspace)");
     NRF_REQUIRE(((uintptr_t)workspace & 15) == 0, "nrf_sample_logits: workspace must be 16-byte aligned");
     const bool may_k = top_k_rows || (top_k > 0 && top_k < size), may_p = top_p_rows || top_p < 1.0f;
     RowWork *work = (RowWork *)workspace;

@@ -223,7 +223,7 @@ def sample_logits(logits, n_samples, temperature=1.0, top_k=0, top_p=1.0, min_p=
     p, pv = _per_row(top_p, "top_p", torch.float32, lead, dev)
     m, mv = _per_row(min_p, "min_p", torch.float32, lead, dev)
     ids, prob = u.new_empty((*lead, n), dtype=torch.int64), u.new_empty((*lead, n))
-    nbytes = _lib.lib().nrf_sample_logits_workspace_bytes(R, V)
+    nbytes = _lib.lib().nrf_sample_logits_workspace_bytes(R, V, n)
     ws = u.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     _call(dev, "nrf_sample_logits", x.data_ptr(), x.stride(0) if R > 1 else V, _DTYPES[x.dtype], R, V, n, t, min(max(int(k), 0), V), p, m,
           _opt(tv), _opt(kv), _opt(pv), _opt(mv), u.data_ptr(), ids.data_ptr(), prob.data_ptr(), _opt(ws))

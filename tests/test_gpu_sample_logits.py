@@ -91,7 +91,7 @@ def test_filters(kind, R, V):
 
 @pytest.mark.parametrize("kind", ["normal", "errors", "flat", "two", "masked", "outlier", "narrow"])
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("R,V,n", [(1, 131072, 1), (2, 100003, 40), (18, 65537, 3), (200, 4099, 2)])
+@pytest.mark.parametrize("R,V,n", [(1, 131072, 1), (2, 100003, 40), (18, 65537, 3), (200, 4099, 2), (3, 2500, 300)])
 def test_long_rows(kind, dtype, R, V, n):
     rng = np.random.RandomState(V + n)
     x = make(kind, R, V, rng)
