@@ -1367,8 +1367,8 @@ void launch_sample(const SampleArgs &a, bool may_k, bool may_p, RowWork *work, h
     } else {
         const dim3 parts(kParts, a.rows);
         sample_max_kernel<T><<<parts, 1024, 0, s>>>(a, work);
-        // one k for all rows, within the groups' reach: nothing is left for later stages
-        const bool alone = !a.top_k_v && may_k && a.top_k <= kGroupsMaxK;
+        // one k for all rows, within the groups' reach: nothing is left for later stages (but many draws, where the list overflows)
+        const bool alone = !a.top_k_v && may_k && a.top_k <= kGroupsMaxK && a.draws <= 64;
         if (may_k) sample_groups_kernel<T><<<parts, 1024, 0, s>>>(a, work, alone);
         if (alone) return;
         if (may_k || may_p) {
@@ -1387,7 +1387,7 @@ void launch_sample(const SampleArgs &a, bool may_k, bool may_p, RowWork *work, h
 }  // namespace
 
 extern "C" int64_t nrf_sample_logits_workspace_bytes(int64_t n_rows, int32_t size, int32_t n_draws) {
-    return form_of(n_rows, size, n_draws, true) == kPartsForm ? n_rows * (int64_t)sizeof(RowWork) : 0;
+    return n_rows > 0 && form_of(n_rows, size, n_draws, true) == kPartsForm ? n_rows * (int64_t)sizeof(RowWork) : 0;
 }
 
 extern "C" int nrf_sample_logits(const void *logits, int64_t row_stride, int32_t dtype, int64_t n_rows, int32_t size, int32_t n_draws,

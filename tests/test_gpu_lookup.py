@@ -186,6 +186,31 @@ def test_gradient_of_a_large_table(kind):
     assert torch.equal(ops.lookup_bwd(g, ids, V, 0.5)[rows], ops.lookup_bwd(g, ids, V, 0.5)[rows])
 
 
+def test_offsets_beyond_32_bits():
+    from nerf_amd import ops
+    V, D = 540000, 4096                                                  # 2.2e9 elements
+    table = torch.zeros(V, D, dtype=torch.bfloat16, device="cuda")
+    ids = torch.tensor([V - 1, 0, 530000, V - 1, 524288], device="cuda")
+    rows = torch.randn(5, D, device="cuda").bfloat16()
+    rows[3] = rows[0]
+    table[ids] = rows
+    assert torch.equal(ops.lookup_fwd(table, ids), rows)
+    del table
+    for n in (5, 5000):                                                  # with and without the sort
+        many = ids.repeat(n // 5)
+        g = rows.repeat(n // 5, 1)
+        grad = ops.lookup_bwd(g, many, V)
+        want = torch.zeros(V, dtype=torch.float64)
+        want.index_add_(0, many.cpu(), g[:, -1].double().cpu())
+        tol = 2.0 ** -8 * want.abs() + n * 2.0 ** -24 * want.abs()
+        assert ((grad[:, -1].double().cpu() - want).abs() <= tol * 1.001).all()
+        assert int((grad != 0).any(1).sum()) == 4
+        del grad
+    # gradients whose rows lie far apart
+    wide = torch.randn(2 ** 30 * 2 + 64, device="cuda", dtype=torch.bfloat16).as_strided((3, 40), (2 ** 30, 1))
+    check_bwd(wide, ids[:3] % 7, 7, 1.0, None, ops.lookup_bwd(wide, ids[:3] % 7, 7))
+
+
 def test_autograd_and_differences():
     from nerf_amd.codes import CodeTable
     torch.manual_seed(0)

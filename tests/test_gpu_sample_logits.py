@@ -211,3 +211,46 @@ def test_another_stream_and_captured_graphs():
             want = run()
             for _, res in graphs:
                 assert torch.equal(res[0], want[0]) and torch.equal(res[1], want[1])
+
+
+def test_rows_far_apart_and_odd_addresses():
+    """Row offsets beyond 2^31 elements; 16-bit rows that begin at odd elements."""
+    from nerf_amd import ops
+    rng = np.random.RandomState(11)
+    base = torch.zeros(2 ** 31 + 80000, dtype=torch.bfloat16, device="cuda")
+    for V in (900, 5000, 70001):
+        x = base.as_strided((3, V), (2 ** 30, 1), 3)
+        x.copy_(make("normal", 3, V, rng).bfloat16())
+        u = torch.from_numpy(rng.rand(3, 4).astype(np.float32)).cuda()
+        for f in (dict(), dict(k=20, p=0.9), dict(p=0.8)):
+            check(x, u, **f)
+    del base
+    x = make("normal", 3, 3001, rng).half().cuda()[:, 1:]
+    check(x, torch.rand(3, 5, device="cuda"), k=9)
+    check(x[:, :1001], torch.rand(3, 5, device="cuda"))
+
+
+def test_values_near_the_ends_of_the_range():
+    from nerf_amd import ops
+    rng = np.random.RandomState(13)
+    tiny = torch.from_numpy((rng.randint(-400, 400, (4, 3000)) * 1.4e-45).astype(np.float32)).cuda()     # denormal logits
+    u = torch.from_numpy(rng.rand(4, 6).astype(np.float32)).cuda()
+    for f in (dict(), dict(k=7), dict(p=0.5), dict(t=1e-38, k=2000), dict(t=1e-38, p=0.9)):
+        check(tiny, u, **f)
+        check(tiny[:, :900], u, **f)
+    zeros = torch.zeros(2, 2500, device="cuda")
+    zeros[:, ::2] = -0.0                                                 # equal values, whatever their sign
+    check(zeros, u[:2], k=100)
+    check(zeros, u[:2], t=0.0)
+    assert ops.sample_logits(zeros, 1, temperature=0.0)[0].tolist() == [[0], [0]]
+
+
+def test_top_k_among_equal_values_and_many_draws():
+    """The groups' bound lets every entry through: the histogram and the first k by index."""
+    rng = np.random.RandomState(14)
+    x = torch.full((1, 70001), 0.5, device="cuda")
+    x[0, 60000:] = 0.25
+    for n in (3, 700):
+        u = torch.from_numpy(rng.rand(1, n).astype(np.float32)).cuda()
+        for f in (dict(k=50), dict(k=1400, p=0.7), dict(k=60500), dict(k=60500, p=0.999)):
+            check(x, u, **f)

@@ -44,5 +44,5 @@ def test_python_refuses_cpu_tensors():
 
 def test_workspace_sizes():
     f = _lib.lib().nrf_sample_logits_workspace_bytes
-    assert f(1, 2048, 1) == 0 and f(4096, 131072, 1) == 0 and f(0, 70000, 1) == 0
+    assert f(1, 2048, 1) == 0 and f(4096, 131072, 1) == 0 and f(0, 70000, 1) == 0 and f(-1, 70000, 1) == 0
     assert f(2, 70000, 1) == 2 * f(1, 640000, 1) == 2 * f(1, 3000, 500) > 0 and f(1, 70000, 1) % 16 == 0
