@@ -10,6 +10,7 @@
 //      tokens' rows and adds runs of equal ids in f32 registers.  A run inside the tile goes straight to its row of grad; one
 //      that reaches beyond an end of it leaves a partial sum (at most two per tile).
 //   3. the team whose tile a crossing run starts in adds up the run's partial sums.
+// Few tokens go without the sort, narrow rows of g travel with their ids instead of being gathered: below.
 // Any distribution of ids costs the same in 2, and a run of n tokens costs n / T partial sums in 3.
 #include "nrf_types.h"
 
@@ -642,6 +643,249 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const SumArgs a, const I 
     }
 }
 
+// ---------------------------------------------------------------------------------------------------- narrow rows
+// Rows of g of up to 8 elements, more than a tile of tokens.  Gathering such rows by position fetches a cache line for each (44 us of
+// 111 for 2^21 rows of two f32), and a second digit moves all pairs once more: here the rows travel with their ids through ONE
+// pass, by the ids' high bits, into at most 1024 buckets of 2^low neighbouring table rows.  A block then takes up to `chunk` tokens
+// of a bucket, ranks them by their low bits (stable), lays their rows out in that order in LDS, and a thread adds each element of the
+// bucket's table rows, zeros included.  Buckets of more than a chunk leave their sums per chunk, added in order by a last launch.
+struct NarrowArgs {
+    const void *g;
+    int64_t g_stride, n;
+    void *grad;
+    uint32_t *keys;            // [n] by bucket
+    void *rows;                // [n][dim] in g's type, by bucket
+    uint32_t *counts;          // [tiles][bins]
+    uint32_t *totals;          // [bins]
+    float *partial;            // [blocks][dim << low]: chunks of buckets that have more than one
+    uint32_t n_rows;
+    int dim, low, bins, chunk, tiles, blocks;
+    float scale;
+};
+
+template <typename I, int ITEMS>
+__global__ void __launch_bounds__(1024) narrow_count_kernel(const I *__restrict__ ids, int64_t padding, const NarrowArgs a) {
+    __shared__ uint32_t cnt[1 << kMaxDigit];
+    if ((int)threadIdx.x < a.bins) cnt[threadIdx.x] = 0;
+    const int64_t i0 = (int64_t)blockIdx.x * (1024 * ITEMS) + threadIdx.x;
+    uint32_t key[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) key[k] = key_of(ids[i0 + k * 1024 < a.n ? i0 + k * 1024 : a.n - 1], a.n_rows, padding);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+        if (i0 + k * 1024 < a.n && key[k] < a.n_rows) atomicAdd(&cnt[key[k] >> a.low], 1u);
+    __syncthreads();
+    if ((int)threadIdx.x < a.bins) a.counts[(int64_t)blockIdx.x * a.bins + threadIdx.x] = cnt[threadIdx.x];
+}
+
+// U: unit that rows are moved in (their size and all addresses are multiples of it), `units` of them a row
+template <typename I, int ITEMS, typename U>
+__global__ void __launch_bounds__(1024) narrow_scatter_kernel(const I *__restrict__ ids, int64_t padding, const NarrowArgs a, int units,
+                                                              int64_t unit_stride) {
+    __shared__ uint32_t base[1 << kMaxDigit];
+    __shared__ uint16_t cnt[16][1 << kMaxDigit], start[1 << kMaxDigit];
+    __shared__ uint32_t key_of_place[1024 * ITEMS];
+    __shared__ uint16_t item_of_place[1024 * ITEMS];
+    __shared__ uint32_t sums[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bins = a.bins;
+    const int64_t tile0 = (int64_t)blockIdx.x * (1024 * ITEMS);
+    const int first_item = wave * (64 * ITEMS) + lane;
+    uint32_t key[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const int64_t i = tile0 + first_item + k * 64;
+        key[k] = i < a.n ? key_of(ids[i], a.n_rows, padding) : a.n_rows;
+    }
+    uint32_t total = 0, before = 0;
+    if (tid < bins) {
+        if (a.tiles <= kFewTiles) {                        // no scan launch: the blocks before, and all of them
+#pragma unroll 8
+            for (int t = 0; t < a.tiles; ++t) {
+                const uint32_t c = a.counts[t * bins + tid];
+                total += c;
+                before += t < (int)blockIdx.x ? c : 0;
+            }
+            if (blockIdx.x == 0) a.totals[tid] = total;
+        } else {
+            total = a.totals[tid], before = a.counts[(int64_t)blockIdx.x * bins + tid];
+        }
+    }
+    int bits = 1;
+    while ((bins - 1) >> bits) ++bits;
+    for (int b = tid; b < 16 << bits; b += 1024) cnt[b >> bits][b & ((1 << bits) - 1)] = 0;
+    const uint32_t first = block_scan<16>(total, sums);
+    uint32_t rank[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const bool on = key[k] < a.n_rows;
+        rank[k] = wave_rank(cnt[wave], on ? key[k] >> a.low : 0, bits, on);
+    }
+    __syncthreads();
+    uint32_t mine = 0;
+    if (tid < bins) {
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            const uint32_t c = cnt[w][tid];
+            cnt[w][tid] = (uint16_t)mine;
+            mine += c;
+        }
+    }
+    const uint32_t local = block_scan<16>(mine, sums);
+    if (tid < bins) {
+        start[tid] = (uint16_t)local;
+        base[tid] = first + before - local;
+    }
+    if (tid == bins - 1) sums[0] = local + mine;           // items of this block that take part
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+        if (key[k] < a.n_rows) {
+            const uint32_t d = key[k] >> a.low, place = start[d] + cnt[wave][d] + rank[k];
+            key_of_place[place] = key[k];
+            item_of_place[place] = (uint16_t)(first_item + k * 64);
+        }
+    __syncthreads();
+    const int count = (int)sums[0];
+    for (int q = tid; q < count; q += 1024) {
+        const uint32_t k = key_of_place[q];
+        const int64_t to = (int64_t)(base[k >> a.low] + q);
+        a.keys[to] = k;
+        const U *from = (const U *)a.g + (tile0 + item_of_place[q]) * unit_stride;
+        U *row = (U *)a.rows + to * units;
+        for (int w = 0; w < units; ++w) row[w] = from[w];
+    }
+}
+
+// Which chunk of which bucket a block works on
+struct Piece {
+    int bucket, chunk, chunks, block0;         // block0: the bucket's first block
+    int64_t begin;
+    int count;
+};
+
+__device__ __forceinline__ Piece piece_of(const NarrowArgs &a, int block, uint32_t *sums, int *found) {
+    const int tid = threadIdx.x;
+    const uint32_t total = tid < a.bins ? a.totals[tid] : 0;
+    const uint32_t chunks = tid < a.bins ? (total <= (uint32_t)a.chunk ? 1 : (total + a.chunk - 1) / a.chunk) : 0;
+    if (tid == 0) found[0] = -1;
+    const uint32_t token0 = block_scan<16>(total, sums), block0 = block_scan<16>(chunks, sums);
+    if (tid < a.bins && (uint32_t)block - block0 < chunks) {
+        found[0] = tid, found[1] = (int)block0, found[2] = (int)chunks, found[3] = (int)token0, found[4] = (int)total;
+    }
+    __syncthreads();
+    Piece p;
+    p.bucket = found[0];
+    if (p.bucket < 0) return p;
+    p.block0 = found[1], p.chunks = found[2], p.chunk = block - p.block0;
+    p.begin = (int64_t)(uint32_t)found[3] + (int64_t)p.chunk * a.chunk;
+    const int left = found[4] - p.chunk * a.chunk;
+    p.count = left < a.chunk ? left : a.chunk;
+    return p;
+}
+
+// C: columns rounded up to a power of two; LDS holds chunk * dim <= 8192 values
+template <typename G, typename T, int C>
+__global__ void __launch_bounds__(1024) narrow_sum_kernel(const NarrowArgs a) {
+    __shared__ float row_lds[8192];
+    __shared__ uint16_t cnt[16][1 << kMaxDigit];
+    __shared__ uint32_t start[(1 << kMaxDigit) + 1];
+    __shared__ uint32_t sums[16];
+    __shared__ int found[5];
+    constexpr int kPer = 4;                                // chunk <= 4096
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const Piece p = piece_of(a, blockIdx.x, sums, found);
+    if (p.bucket < 0) return;
+    const int per_bucket = 1 << a.low, dim = a.dim;
+    uint32_t low[kPer];
+    float v[kPer][C];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int i = wave * (64 * kPer) + k * 64 + lane;
+        const int64_t at = p.begin + (i < p.count ? i : 0);
+        if (p.count > 0) {
+            low[k] = a.keys[at] & (per_bucket - 1);
+#pragma unroll
+            for (int c = 0; c < C; ++c) v[k][c] = c < dim ? to_f32(((const G *)a.rows)[at * dim + c]) : 0.0f;
+        }
+    }
+    for (int b = tid; b < 16 << a.low; b += 1024) cnt[b >> a.low][b & (per_bucket - 1)] = 0;
+    __syncthreads();
+    uint32_t rank[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const bool on = wave * (64 * kPer) + k * 64 + lane < p.count;
+        rank[k] = wave_rank(cnt[wave], on ? low[k] : 0, a.low, on);
+    }
+    __syncthreads();
+    uint32_t mine = 0;
+    if (tid < per_bucket) {
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            const uint32_t c = cnt[w][tid];
+            cnt[w][tid] = (uint16_t)mine;
+            mine += c;
+        }
+    }
+    const uint32_t first = block_scan<16>(mine, sums);
+    if (tid < per_bucket) start[tid] = first;
+    if (tid == 0) start[per_bucket] = p.count;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+        if (wave * (64 * kPer) + k * 64 + lane < p.count) {
+            const uint32_t place = start[low[k]] + cnt[wave][low[k]] + rank[k];
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (c < dim) row_lds[place * dim + c] = v[k][c];
+        }
+    __syncthreads();
+    for (int e = tid; e < per_bucket * C; e += 1024) {
+        const int r = e / C, c = e % C;
+        const int64_t row = ((int64_t)p.bucket << a.low) + r;
+        if (c >= dim || row >= (int64_t)a.n_rows) continue;
+        float sum = 0.0f;
+        const uint32_t hi = start[r + 1];
+#pragma unroll 8
+        for (uint32_t q = start[r]; q < hi; ++q) sum += row_lds[q * dim + c];
+        if (p.chunks == 1) ((T *)a.grad)[row * dim + c] = from_f32<T>(sum * a.scale);
+        else a.partial[(int64_t)blockIdx.x * (dim << a.low) + r * dim + c] = sum;
+    }
+}
+
+// Buckets of several chunks, a block each: four threads an element, each a quarter of the chunks.
+template <typename T>
+__global__ void __launch_bounds__(1024) narrow_join_kernel(const NarrowArgs a) {
+    __shared__ uint32_t sums[16];
+    __shared__ int found;
+    __shared__ float part[4][256];
+    const int tid = threadIdx.x, bucket = blockIdx.x;
+    const uint32_t own = a.totals[bucket];
+    if (own <= (uint32_t)a.chunk) return;
+    const uint32_t total = tid < a.bins ? a.totals[tid] : 0;
+    const uint32_t chunks = tid < a.bins ? (total <= (uint32_t)a.chunk ? 1 : (total + a.chunk - 1) / a.chunk) : 0;
+    const uint32_t block0 = block_scan<16>(chunks, sums);
+    if (tid == bucket) found = (int)block0;
+    __syncthreads();
+    const int n = (int)((own + a.chunk - 1) / a.chunk), size = a.dim << a.low, quarter = tid >> 8;
+    const int each = (n + 3) / 4, c0 = quarter * each, c1 = c0 + each < n ? c0 + each : n;
+    for (int e0 = 0; e0 < size; e0 += 256) {
+        const int e = e0 + (tid & 255);
+        float sum = 0.0f;
+        if (e < size) {
+            const float *p = a.partial + (int64_t)found * size + e;
+#pragma unroll 8
+            for (int c = c0; c < c1; ++c) sum += p[(int64_t)c * size];
+        }
+        part[quarter][tid & 255] = sum;
+        __syncthreads();
+        const int64_t at = (((int64_t)bucket << a.low) * a.dim) + e;
+        if (quarter == 0 && e < size && at < (int64_t)a.n_rows * a.dim)
+            ((T *)a.grad)[at] = from_f32<T>((((part[0][tid] + part[1][tid]) + part[2][tid]) + part[3][tid]) * a.scale);
+        __syncthreads();
+    }
+}
+
 // ---------------------------------------------------------------------------------------------------- host
 struct BwdPlan {
     int passes, digit;         // of the sort
@@ -649,6 +893,7 @@ struct BwdPlan {
     int sort_items;            // items of a thread in it
     int tile;                  // tokens of a sum tile
     int64_t sum_tiles;
+    int low, bins, chunk, blocks;      // narrow rows: bits of a bucket, buckets, tokens of a block, blocks; bins 0: the other way
     int64_t off_a, off_b, off_counts, off_totals, off_head, off_tail, bytes;       // all zero: few tokens, no workspace
 };
 
@@ -668,6 +913,25 @@ Few few_tokens(int64_t n, int64_t n_rows, int dim) {
 BwdPlan plan_bwd(int64_t n, int64_t n_rows, int dim) {
     BwdPlan p{};
     if (few_tokens(n, n_rows, dim) != kNotFew) return p;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
+    if (dim <= 8 && n_rows > 0 && n_rows <= 1 << 20 && n > kTile) {
+        // buckets no more than the digit has, and wide enough to keep half a block's threads in the sums
+        while ((n_rows - 1) >> p.low >= 1 << kMaxDigit || (dim << p.low < 512 && 1 << p.low < n_rows)) ++p.low;
+        p.bins = (int)(((n_rows - 1) >> p.low) + 1);
+        p.chunk = 4096;
+        while (p.chunk * dim > 8192) p.chunk >>= 1;
+        p.blocks = p.bins + (int)(n / p.chunk);            // a bucket's last chunk may be short, and empty buckets have one
+        p.sort_items = n <= (int64_t)kFewTiles * 1024 * kFewItems ? kFewItems : kTileItems;
+        p.sort_tiles = (n + 1024 * p.sort_items - 1) / (1024 * p.sort_items);
+        p.off_a = take(n * 4);
+        p.off_b = take(n * dim * 4);
+        p.off_counts = take(p.sort_tiles * p.bins * 4);
+        p.off_totals = take(p.bins * 4);
+        p.off_head = take((int64_t)p.blocks * (dim << p.low) * 4);
+        p.bytes = at;
+        return p;
+    }
     int bits = 1;
     while (bits < 32 && (n_rows >> bits) != 0) ++bits;     // keys go up to n_rows itself
     p.passes = (bits + kMaxDigit - 1) / kMaxDigit;
@@ -681,8 +945,6 @@ BwdPlan plan_bwd(int64_t n, int64_t n_rows, int dim) {
     const int64_t vectors = (dim + 3) / 4;
     while (p.tile > kBatch && n * vectors / p.tile < 256 * 8 * 64) p.tile >>= 1;
     p.sum_tiles = (n + p.tile - 1) / p.tile;
-    int64_t at = 0;
-    auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
     p.off_a = take(n * 8);
     p.off_b = p.passes > 1 && p.sort_tiles ? take(n * 8) : 0;
     p.off_counts = take(p.sort_tiles * (4 << p.digit));
@@ -737,6 +999,41 @@ const uint2 *sort_pairs(const BwdPlan &p, const I *ids, int64_t n, int64_t n_row
                                      : sort_many<I, kTileItems>(p, ids, n, n_rows, padding, ws, grad, grad_bytes, s);
 }
 
+template <typename I, int ITEMS>
+void narrow_scatter(const NarrowArgs &a, const I *ids, int64_t padding, int elem, hipStream_t s) {
+    narrow_count_kernel<I, ITEMS><<<a.tiles, 1024, 0, s>>>(ids, padding, a);
+    if (a.tiles > kFewTiles) sort_scan_kernel<<<(a.bins + 63) / 64, 1024, 0, s>>>(a.counts, a.totals, a.bins, a.tiles);
+    // the largest unit that rows and their addresses are made of
+    const int bytes = a.dim * elem;
+    const uint64_t all = (uint64_t)(uintptr_t)a.g | (uint64_t)a.g_stride * elem | (uint64_t)bytes;
+    const int unit = all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
+    const int units = bytes / unit;
+    const int64_t stride = a.g_stride * elem / unit;
+    if (unit == 16) narrow_scatter_kernel<I, ITEMS, uint4><<<a.tiles, 1024, 0, s>>>(ids, padding, a, units, stride);
+    else if (unit == 8) narrow_scatter_kernel<I, ITEMS, uint2><<<a.tiles, 1024, 0, s>>>(ids, padding, a, units, stride);
+    else if (unit == 4) narrow_scatter_kernel<I, ITEMS, uint32_t><<<a.tiles, 1024, 0, s>>>(ids, padding, a, units, stride);
+    else narrow_scatter_kernel<I, ITEMS, uint16_t><<<a.tiles, 1024, 0, s>>>(ids, padding, a, units, stride);
+}
+
+template <typename G, typename T>
+void launch_narrow(const SumArgs &sa, const BwdPlan &p, const void *ids, bool i64, int64_t padding, char *ws, hipStream_t s) {
+    NarrowArgs a;
+    a.g = sa.g, a.g_stride = sa.g_stride, a.n = sa.n, a.grad = sa.grad, a.n_rows = sa.n_rows, a.dim = sa.dim, a.scale = sa.scale;
+    a.keys = (uint32_t *)(ws + p.off_a), a.rows = ws + p.off_b, a.counts = (uint32_t *)(ws + p.off_counts);
+    a.totals = (uint32_t *)(ws + p.off_totals), a.partial = (float *)(ws + p.off_head);
+    a.low = p.low, a.bins = p.bins, a.chunk = p.chunk, a.tiles = (int)p.sort_tiles, a.blocks = p.blocks;
+    const int e = (int)sizeof(G);
+    if (i64) p.sort_items == kFewItems ? narrow_scatter<int64_t, kFewItems>(a, (const int64_t *)ids, padding, e, s)
+                                       : narrow_scatter<int64_t, kTileItems>(a, (const int64_t *)ids, padding, e, s);
+    else p.sort_items == kFewItems ? narrow_scatter<int32_t, kFewItems>(a, (const int32_t *)ids, padding, e, s)
+                                   : narrow_scatter<int32_t, kTileItems>(a, (const int32_t *)ids, padding, e, s);
+    if (a.dim == 1) narrow_sum_kernel<G, T, 1><<<a.blocks, 1024, 0, s>>>(a);
+    else if (a.dim == 2) narrow_sum_kernel<G, T, 2><<<a.blocks, 1024, 0, s>>>(a);
+    else if (a.dim <= 4) narrow_sum_kernel<G, T, 4><<<a.blocks, 1024, 0, s>>>(a);
+    else narrow_sum_kernel<G, T, 8><<<a.blocks, 1024, 0, s>>>(a);
+    narrow_join_kernel<T><<<a.bins, 1024, 0, s>>>(a);
+}
+
 template <typename G, typename T, int VW>
 void launch_sums(SumArgs a, const BwdPlan &p, const void *ids, bool i64, int64_t padding, hipStream_t s) {
     const int vectors = a.dim / VW;
@@ -763,7 +1060,8 @@ void launch_sums(SumArgs a, const BwdPlan &p, const void *ids, bool i64, int64_t
 }
 
 template <typename G, typename T>
-void pick_sums(int vw, const SumArgs &a, const BwdPlan &p, const void *ids, bool i64, int64_t padding, hipStream_t s) {
+void pick_sums(int vw, const SumArgs &a, const BwdPlan &p, const void *ids, bool i64, int64_t padding, char *ws, hipStream_t s) {
+    if (p.bins) return launch_narrow<G, T>(a, p, ids, i64, padding, ws, s);
     if constexpr (sizeof(G) == 2 && sizeof(T) == 2)
         if (vw == 8) return launch_sums<G, T, 8>(a, p, ids, i64, padding, s);
     if (vw >= 4) return launch_sums<G, T, 4>(a, p, ids, i64, padding, s);
@@ -833,18 +1131,18 @@ extern "C" int nrf_lookup_bwd(const void *g_out, int64_t g_stride, int32_t g_dty
     const bool i64 = ids_are_64 != 0;
     char *ws = (char *)workspace;
     SumArgs a{};
-    if (p.bytes)
+    if (p.bytes && !p.bins)
         a.pairs = i64 ? sort_pairs(p, (const int64_t *)ids, n, n_rows, padding_idx, ws, grad, grad_bytes, s)
                       : sort_pairs(p, (const int32_t *)ids, n, n_rows, padding_idx, ws, grad, grad_bytes, s);
     if (p.bytes == 0 || n > 0) {
         a.g = g_out, a.g_stride = g_stride, a.grad = grad, a.head = (float *)(ws + p.off_head), a.tail = (float *)(ws + p.off_tail);
         a.n = n, a.n_rows = (uint32_t)n_rows, a.dim = dim, a.tile = p.tile, a.scale = scale;
         const int vw = common_width(dim, eg, (uint64_t)(uintptr_t)g_out | (uint64_t)g_stride * eg, es, (uint64_t)(uintptr_t)grad);
-        if (g_dtype == NRF_F32 && dtype == NRF_F32) pick_sums<float, float>(vw, a, p, ids, i64, padding_idx, s);
-        else if (g_dtype == NRF_F32 && dtype == NRF_BF16) pick_sums<float, bf16_t>(vw, a, p, ids, i64, padding_idx, s);
-        else if (g_dtype == NRF_F32) pick_sums<float, f16_t>(vw, a, p, ids, i64, padding_idx, s);
-        else if (g_dtype == NRF_BF16) pick_sums<bf16_t, bf16_t>(vw, a, p, ids, i64, padding_idx, s);
-        else pick_sums<f16_t, f16_t>(vw, a, p, ids, i64, padding_idx, s);
+        if (g_dtype == NRF_F32 && dtype == NRF_F32) pick_sums<float, float>(vw, a, p, ids, i64, padding_idx, ws, s);
+        else if (g_dtype == NRF_F32 && dtype == NRF_BF16) pick_sums<float, bf16_t>(vw, a, p, ids, i64, padding_idx, ws, s);
+        else if (g_dtype == NRF_F32) pick_sums<float, f16_t>(vw, a, p, ids, i64, padding_idx, ws, s);
+        else if (g_dtype == NRF_BF16) pick_sums<bf16_t, bf16_t>(vw, a, p, ids, i64, padding_idx, ws, s);
+        else pick_sums<f16_t, f16_t>(vw, a, p, ids, i64, padding_idx, ws, s);
     }
     return check_launch("nrf_lookup_bwd");
 }

@@ -61,7 +61,8 @@ def check_bwd(g, ids, V, scale, pad, grad):
 
 # n, V, D: one token, one column, odd sizes, rows that are not 16-byte multiples, wide rows, sizes around the sorts' borders
 SHAPES = [(1, 1, 1), (1, 7, 48), (3, 2, 5), (64, 100, 32), (65, 100, 33), (1000, 3, 27), (4097, 300, 8), (300, 70000, 4),
-          (900, 100000, 4), (1024, 4097, 9), (2440, 9464, 8), (4096, 50000, 3), (8056, 195952, 5), (6000, 700, 65), (300001, 600000, 2), (4100, 5000, 33), (16384, 1025, 12), (16385, 1500, 16), (20000, 5, 2), (50001, 4096, 3), (33, 1000, 4096), (40, 9, 1111), (2, 3, 32768)]
+          (900, 100000, 4), (1024, 4097, 9), (2440, 9464, 8), (4096, 50000, 3), (8056, 195952, 5), (6000, 700, 65), (5000, 1, 8), (70000, 3, 1), (30000, 1000, 7),
+          (200000, 1 << 20, 1), (9000, (1 << 20) + 1, 2), (150000, 1025, 4), (300001, 600000, 2), (4100, 5000, 33), (16384, 1025, 12), (16385, 1500, 16), (20000, 5, 2), (50001, 4096, 3), (33, 1000, 4096), (40, 9, 1111), (2, 3, 32768)]
 
 
 @pytest.mark.parametrize("n,V,D", SHAPES)
@@ -79,7 +80,7 @@ def test_forward_and_gradient(n, V, D, kind):
 
 
 @pytest.mark.parametrize("t,o", [("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f16", "f32")])
-@pytest.mark.parametrize("n,V,D", [(1, 4, 64), (777, 50, 33), (5000, 900, 24), (20000, 1 << 19, 2), (130, 60, 2056)])
+@pytest.mark.parametrize("n,V,D", [(1, 4, 64), (777, 50, 33), (5000, 900, 24), (20000, 1 << 19, 2), (130, 60, 2056), (9001, 3000, 5), (8000, 70, 8)])
 def test_sixteen_bit_tables(t, o, n, V, D):
     from nerf_amd import ops
     rng = np.random.RandomState(D)
