@@ -656,12 +656,13 @@ struct NarrowArgs {
     uint32_t *keys;            // [n] by bucket
     void *rows;                // [n][dim] in g's type, by bucket
     uint32_t *counts;          // [tiles][bins]
-    uint32_t *totals;          // [bins]
+    uint32_t *totals;          // [bins]; behind them, where the bucket's tokens begin [bins], and the number of further chunks
     float *partial;            // [blocks][dim << low]: chunks of buckets that have more than one
     uint32_t n_rows;
     int dim, low, bins, chunk, tiles, blocks;
     float scale;
 };
+constexpr int kHeavy = 64;     // tokens of a table row beyond which a wave adds them
 
 template <typename I, int ITEMS>
 __global__ void __launch_bounds__(1024) narrow_count_kernel(const I *__restrict__ ids, int64_t padding, const NarrowArgs a) {
@@ -706,7 +707,6 @@ __global__ void __launch_bounds__(1024) narrow_scatter_kernel(const I *__restric
                 total += c;
                 before += t < (int)blockIdx.x ? c : 0;
             }
-            if (blockIdx.x == 0) a.totals[tid] = total;
         } else {
             total = a.totals[tid], before = a.counts[(int64_t)blockIdx.x * bins + tid];
         }
@@ -715,6 +715,12 @@ __global__ void __launch_bounds__(1024) narrow_scatter_kernel(const I *__restric
     while ((bins - 1) >> bits) ++bits;
     for (int b = tid; b < 16 << bits; b += 1024) cnt[b >> bits][b & ((1 << bits) - 1)] = 0;
     const uint32_t first = block_scan<16>(total, sums);
+    if (blockIdx.x == 0) {                                 // for the launches behind this one
+        const uint32_t further = total > (uint32_t)a.chunk ? (total - 1) / a.chunk : 0;
+        const uint32_t f = block_scan<16>(further, sums);
+        if (tid < bins) a.totals[tid] = total, a.totals[bins + tid] = first;
+        if (tid == bins - 1) a.totals[2 * bins] = f + further;
+    }
     uint32_t rank[ITEMS];
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
@@ -757,30 +763,39 @@ __global__ void __launch_bounds__(1024) narrow_scatter_kernel(const I *__restric
     }
 }
 
-// Which chunk of which bucket a block works on
+// Which chunk of which bucket a block works on: block b < bins the first chunk of bucket b, the blocks behind them the further ones.
 struct Piece {
-    int bucket, chunk, chunks, block0;         // block0: the bucket's first block
+    int bucket, chunks;
     int64_t begin;
     int count;
 };
 
+// Further chunks of the buckets before bucket `tid` (all threads call)
+__device__ __forceinline__ uint32_t further_before(const NarrowArgs &a, uint32_t *own, uint32_t *sums) {
+    const uint32_t total = (int)threadIdx.x < a.bins ? a.totals[threadIdx.x] : 0;
+    *own = total > (uint32_t)a.chunk ? (total - 1) / a.chunk : 0;
+    return block_scan<16>(*own, sums);
+}
+
 __device__ __forceinline__ Piece piece_of(const NarrowArgs &a, int block, uint32_t *sums, int *found) {
-    const int tid = threadIdx.x;
-    const uint32_t total = tid < a.bins ? a.totals[tid] : 0;
-    const uint32_t chunks = tid < a.bins ? (total <= (uint32_t)a.chunk ? 1 : (total + a.chunk - 1) / a.chunk) : 0;
-    if (tid == 0) found[0] = -1;
-    const uint32_t token0 = block_scan<16>(total, sums), block0 = block_scan<16>(chunks, sums);
-    if (tid < a.bins && (uint32_t)block - block0 < chunks) {
-        found[0] = tid, found[1] = (int)block0, found[2] = (int)chunks, found[3] = (int)token0, found[4] = (int)total;
-    }
-    __syncthreads();
     Piece p;
-    p.bucket = found[0];
-    if (p.bucket < 0) return p;
-    p.block0 = found[1], p.chunks = found[2], p.chunk = block - p.block0;
-    p.begin = (int64_t)(uint32_t)found[3] + (int64_t)p.chunk * a.chunk;
-    const int left = found[4] - p.chunk * a.chunk;
-    p.count = left < a.chunk ? left : a.chunk;
+    int chunk = 0;
+    p.bucket = block;
+    if (block >= a.bins) {
+        const uint32_t x = block - a.bins;
+        p.bucket = -1;
+        if (x >= a.totals[2 * a.bins]) return p;
+        uint32_t own;
+        const uint32_t before = further_before(a, &own, sums);
+        if (x - before < own) found[0] = threadIdx.x, found[1] = (int)(x - before) + 1;
+        __syncthreads();
+        p.bucket = found[0], chunk = found[1];
+    }
+    const uint32_t total = a.totals[p.bucket];
+    p.begin = (int64_t)a.totals[a.bins + p.bucket] + (int64_t)chunk * a.chunk;
+    p.chunks = total > (uint32_t)a.chunk ? (int)((total - 1) / a.chunk) + 1 : 1;
+    const int64_t left = (int64_t)total - (int64_t)chunk * a.chunk;
+    p.count = (int)(left < a.chunk ? left : a.chunk);
     return p;
 }
 
@@ -790,25 +805,31 @@ __global__ void __launch_bounds__(1024) narrow_sum_kernel(const NarrowArgs a) {
     __shared__ float row_lds[8192];
     __shared__ uint16_t cnt[16][1 << kMaxDigit];
     __shared__ uint32_t start[(1 << kMaxDigit) + 1];
-    __shared__ uint32_t sums[16];
-    __shared__ int found[5];
+    __shared__ uint32_t sums[16], heavy_count;
+    __shared__ uint16_t heavy[8192 / kHeavy];
+    __shared__ int found[2];
     constexpr int kPer = 4;                                // chunk <= 4096
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Piece p = piece_of(a, blockIdx.x, sums, found);
     if (p.bucket < 0) return;
     const int per_bucket = 1 << a.low, dim = a.dim;
+    const int64_t row0 = (int64_t)p.bucket << a.low;
+    if (p.count == 0) {                                    // no token: the zeros
+        const int64_t size = ((int64_t)a.n_rows - row0 < per_bucket ? (int64_t)a.n_rows - row0 : per_bucket) * dim;
+        for (int64_t e = tid; e < size; e += 1024) ((T *)a.grad)[row0 * dim + e] = from_f32<T>(0.0f);
+        return;
+    }
     uint32_t low[kPer];
     float v[kPer][C];
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
         const int i = wave * (64 * kPer) + k * 64 + lane;
         const int64_t at = p.begin + (i < p.count ? i : 0);
-        if (p.count > 0) {
-            low[k] = a.keys[at] & (per_bucket - 1);
+        low[k] = a.keys[at] & (per_bucket - 1);
 #pragma unroll
-            for (int c = 0; c < C; ++c) v[k][c] = c < dim ? to_f32(((const G *)a.rows)[at * dim + c]) : 0.0f;
-        }
+        for (int c = 0; c < C; ++c) v[k][c] = c < dim ? to_f32(((const G *)a.rows)[at * dim + c]) : 0.0f;
     }
+    if (tid == 0) heavy_count = 0;
     for (int b = tid; b < 16 << a.low; b += 1024) cnt[b >> a.low][b & (per_bucket - 1)] = 0;
     __syncthreads();
     uint32_t rank[kPer];
@@ -840,16 +861,38 @@ __global__ void __launch_bounds__(1024) narrow_sum_kernel(const NarrowArgs a) {
                 if (c < dim) row_lds[place * dim + c] = v[k][c];
         }
     __syncthreads();
+    const auto store = [&](int r, int c, float sum) {
+        if (p.chunks == 1) ((T *)a.grad)[(row0 + r) * dim + c] = from_f32<T>(sum * a.scale);
+        else a.partial[(int64_t)blockIdx.x * (dim << a.low) + r * dim + c] = sum;
+    };
     for (int e = tid; e < per_bucket * C; e += 1024) {
         const int r = e / C, c = e % C;
-        const int64_t row = ((int64_t)p.bucket << a.low) + r;
-        if (c >= dim || row >= (int64_t)a.n_rows) continue;
+        if (c >= dim || row0 + r >= (int64_t)a.n_rows) continue;
+        const uint32_t lo = start[r], hi = start[r + 1];
+        if (hi - lo > kHeavy) {
+            if (c == 0) heavy[atomicAdd(&heavy_count, 1u)] = (uint16_t)r;
+            continue;
+        }
         float sum = 0.0f;
-        const uint32_t hi = start[r + 1];
 #pragma unroll 8
-        for (uint32_t q = start[r]; q < hi; ++q) sum += row_lds[q * dim + c];
-        if (p.chunks == 1) ((T *)a.grad)[row * dim + c] = from_f32<T>(sum * a.scale);
-        else a.partial[(int64_t)blockIdx.x * (dim << a.low) + r * dim + c] = sum;
+        for (uint32_t q = lo; q < hi; ++q) sum += row_lds[q * dim + c];
+        store(r, c, sum);
+    }
+    __syncthreads();
+    // rows of many tokens: a wave each, its lanes a slice of the tokens and a column, the slices added by halves
+    constexpr int kSlices = 64 / C;
+    for (uint32_t h = wave; h < heavy_count; h += 16) {
+        const int r = heavy[h], c = lane % C;
+        const uint32_t lo = start[r], hi = start[r + 1], each = (hi - lo + kSlices - 1) / kSlices, q0 = lo + lane / C * each;
+        const uint32_t q1 = q0 + each < hi ? q0 + each : hi;
+        float sum = 0.0f;
+        if (c < dim) {
+#pragma unroll 8
+            for (uint32_t q = q0; q < q1; ++q) sum += row_lds[q * dim + c];
+        }
+#pragma unroll
+        for (int d = 32; d >= C; d >>= 1) sum += __shfl_xor(sum, d);
+        if (lane < dim) store(r, lane, sum);
     }
 }
 
@@ -862,10 +905,9 @@ __global__ void __launch_bounds__(1024) narrow_join_kernel(const NarrowArgs a) {
     const int tid = threadIdx.x, bucket = blockIdx.x;
     const uint32_t own = a.totals[bucket];
     if (own <= (uint32_t)a.chunk) return;
-    const uint32_t total = tid < a.bins ? a.totals[tid] : 0;
-    const uint32_t chunks = tid < a.bins ? (total <= (uint32_t)a.chunk ? 1 : (total + a.chunk - 1) / a.chunk) : 0;
-    const uint32_t block0 = block_scan<16>(chunks, sums);
-    if (tid == bucket) found = (int)block0;
+    uint32_t further;
+    const uint32_t before = further_before(a, &further, sums);
+    if (tid == bucket) found = (int)before;
     __syncthreads();
     const int n = (int)((own + a.chunk - 1) / a.chunk), size = a.dim << a.low, quarter = tid >> 8;
     const int each = (n + 3) / 4, c0 = quarter * each, c1 = c0 + each < n ? c0 + each : n;
@@ -873,9 +915,10 @@ __global__ void __launch_bounds__(1024) narrow_join_kernel(const NarrowArgs a) {
         const int e = e0 + (tid & 255);
         float sum = 0.0f;
         if (e < size) {
-            const float *p = a.partial + (int64_t)found * size + e;
+            // chunk 0 lies at the bucket's own block, the further ones behind all buckets
+            const float *p = a.partial + ((int64_t)a.bins + found - 1) * size + e;
 #pragma unroll 8
-            for (int c = c0; c < c1; ++c) sum += p[(int64_t)c * size];
+            for (int c = c0; c < c1; ++c) sum += c == 0 ? a.partial[(int64_t)bucket * size + e] : p[(int64_t)c * size];
         }
         part[quarter][tid & 255] = sum;
         __syncthreads();
@@ -921,13 +964,13 @@ BwdPlan plan_bwd(int64_t n, int64_t n_rows, int dim) {
         p.bins = (int)(((n_rows - 1) >> p.low) + 1);
         p.chunk = 4096;
         while (p.chunk * dim > 8192) p.chunk >>= 1;
-        p.blocks = p.bins + (int)(n / p.chunk);            // a bucket's last chunk may be short, and empty buckets have one
+        p.blocks = p.bins + (int)(n / p.chunk);            // a first chunk each, and at most so many further ones
         p.sort_items = n <= (int64_t)kFewTiles * 1024 * kFewItems ? kFewItems : kTileItems;
         p.sort_tiles = (n + 1024 * p.sort_items - 1) / (1024 * p.sort_items);
         p.off_a = take(n * 4);
         p.off_b = take(n * dim * 4);
         p.off_counts = take(p.sort_tiles * p.bins * 4);
-        p.off_totals = take(p.bins * 4);
+        p.off_totals = take((2 * p.bins + 1) * 4);
         p.off_head = take((int64_t)p.blocks * (dim << p.low) * 4);
         p.bytes = at;
         return p;
