@@ -95,16 +95,21 @@ __device__ __forceinline__ int bin_of(const Row &w, float scale, float x) {
     return (int)fminf((w.topf - x) * scale, (float)(kBins - 1));
 }
 
+// 16-byte pieces of a row, at any alignment of its elements
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Vec {
+    static constexpr int E = 16 / sizeof(T);
+    T e[E];
+};
+
 // f(x, i, u) for the entries begin .. end of a row, 16 bytes a load (at any alignment of the elements), four loads in flight;
 // u: which of the four the entry came in (0 for the odd ones at the end).
 template <int BLOCK, int U = 4, typename T, typename F>
 __device__ __forceinline__ void for_each(const T *row, int begin, int end, F f) {
-    constexpr int E = 16 / sizeof(T);
-    struct __attribute__((packed, aligned(sizeof(T)))) Vec { T e[E]; };
-    const Vec *v = reinterpret_cast<const Vec *>(row + begin);
+    constexpr int E = Vec<T>::E;
+    const Vec<T> *v = reinterpret_cast<const Vec<T> *>(row + begin);
     const int n = (end - begin) / E;
     for (int j = threadIdx.x; j < n; j += BLOCK * U) {
-        Vec p[U];
+        Vec<T> p[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) p[u] = v[min(j + u * BLOCK, n - 1)];
 #pragma unroll
@@ -549,48 +554,59 @@ struct Reach {
     }
 };
 
-// The entries of a part of a row into list[0 ..), in any order, as by_value; those beyond kList are counted only.  First a mask per
-// thread and 64 bytes, with one reservation for what is set in it, and the indices; then the values by their indices.
-template <int BLOCK, typename T>
-__device__ __forceinline__ uint32_t gather(Shared<BLOCK> &s, const RowState &o, const T *row, int begin, int end, const Reach &want) {
-    constexpr int E = 16 / sizeof(T), U = 4;
-    struct __attribute__((packed, aligned(sizeof(T)))) Vec { T e[E]; };
-    const Vec *v = reinterpret_cast<const Vec *>(row + begin);
-    const int nv = (end - begin) / E;
+__device__ __forceinline__ bool reached(const Reach &want, const RowState &o, float x) {
+    if (want.from < 0) return x >= want.least;
     // before the rounding down to whole bins; the last bin has no end
-    const float low = (float)want.from, high = want.to == kBins - 1 ? __builtin_inff() : (float)(want.to + 1);
-    const auto in = [&](float x) {
-        if (want.from < 0) return x >= want.least;
-        const float b = fminf((o.w.topf - x) * o.scale, (float)(kBins - 1));
-        return b >= low && b < high && x > -__builtin_inff();
-    };
-    uint32_t *index = reinterpret_cast<uint32_t *>(s.mass);
-    if (threadIdx.x == 0) s.count = 0;
-    __syncthreads();
-    for (int j = threadIdx.x; j < nv; j += BLOCK * U) {
-        Vec p[U];
+    const float b = fminf((o.w.topf - x) * o.scale, (float)(kBins - 1));
+    return b >= (float)want.from && b < (want.to == kBins - 1 ? __builtin_inff() : (float)(want.to + 1)) && x > -__builtin_inff();
+}
+
+// What is reached in four pieces (place j of the row and every BLOCK-th behind it), a bit an entry
+template <int BLOCK, typename T>
+__device__ __forceinline__ uint32_t reach_mask(const RowState &o, const Vec<T> *p, int j, int pieces, const Reach &want) {
+    constexpr int E = Vec<T>::E;
+    uint32_t mask = 0;
 #pragma unroll
-        for (int u = 0; u < U; ++u) p[u] = v[min(j + u * BLOCK, nv - 1)];
-        uint32_t mask = 0;
+    for (int u = 0; u < 4; ++u) {
+        uint32_t m = 0;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            uint32_t m = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e) m |= in(to_f32(p[u].e[e])) ? 1u << e : 0u;
-            mask |= j + u * BLOCK < nv ? m << (u * E) : 0u;
-        }
-        if (mask) {
-            uint32_t at = atomicAdd(&s.count, (uint32_t)__popc(mask));
-            do {
-                const int bit = __builtin_ctz(mask);
-                if (at < (uint32_t)kList) index[at] = begin + (j + bit / E * BLOCK) * E + bit % E;
-                ++at;
-                mask &= mask - 1;
-            } while (mask);
-        }
+        for (int e = 0; e < E; ++e) m |= reached(want, o, to_f32(p[u].e[e])) ? 1u << e : 0u;
+        mask |= j + u * BLOCK < pieces ? m << (u * E) : 0u;
     }
-    const int i = begin + nv * E + threadIdx.x;
-    if (i < end && in(to_f32(row[i]))) {
+    return mask;
+}
+
+// Places in the list for `n` entries of each lane: one addition a wave (all lanes call; an atomicAdd of different amounts would
+// be serialised lane by lane)
+__device__ __forceinline__ uint32_t reserve(uint32_t *count, uint32_t n) {
+    const uint32_t to = wave_scan(n), all = __builtin_amdgcn_readlane(to, 63);
+    uint32_t base = 0;
+    if (all) {
+        if ((threadIdx.x & 63) == 0) base = atomicAdd(count, all);
+        base = uniform(base);
+    }
+    return base + to - n;
+}
+
+// The indices of a mask's entries into the list from place `at` on
+template <int BLOCK, typename T>
+__device__ __forceinline__ uint32_t put_mask(uint32_t *index, uint32_t mask, uint32_t at, int j, int begin) {
+    constexpr int E = Vec<T>::E;
+    while (mask) {
+        const int bit = __builtin_ctz(mask);
+        if (at < (uint32_t)kList) index[at] = begin + (j + bit / E * BLOCK) * E + bit % E;
+        ++at;
+        mask &= mask - 1;
+    }
+    return at;
+}
+
+// The odd entries at the end, then the values by their indices: list[0 ..), in any order, as by_value.  Returns how many are reached
+// (those beyond kList are counted only).
+template <int BLOCK, typename T>
+__device__ __forceinline__ uint32_t finish_list(Shared<BLOCK> &s, const RowState &o, const T *row, int i, int end, const Reach &want) {
+    uint32_t *index = reinterpret_cast<uint32_t *>(s.mass);
+    if (i < end && reached(want, o, to_f32(row[i]))) {
         const uint32_t at = atomicAdd(&s.count, 1u);
         if (at < (uint32_t)kList) index[at] = i;
     }
@@ -599,6 +615,24 @@ __device__ __forceinline__ uint32_t gather(Shared<BLOCK> &s, const RowState &o, 
     for (uint32_t q = threadIdx.x; q < n && q < (uint32_t)kList; q += BLOCK) s.list[q] = by_value(key_of(to_f32(row[index[q]])), index[q]);
     __syncthreads();
     return n;
+}
+
+template <int BLOCK, typename T>
+__device__ __forceinline__ uint32_t gather(Shared<BLOCK> &s, const RowState &o, const T *row, int begin, int end, const Reach &want) {
+    constexpr int E = Vec<T>::E;
+    const Vec<T> *v = reinterpret_cast<const Vec<T> *>(row + begin);
+    const int pieces = (end - begin) / E;
+    if (threadIdx.x == 0) s.count = 0;
+    __syncthreads();
+    for (int j0 = 0; j0 < pieces; j0 += BLOCK * 4) {
+        const int j = j0 + threadIdx.x;
+        Vec<T> p[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) p[u] = v[min(j + u * BLOCK, pieces - 1)];
+        const uint32_t mask = reach_mask<BLOCK, T>(o, p, j, pieces, want), at = reserve(&s.count, __popc(mask));
+        put_mask<BLOCK, T>(reinterpret_cast<uint32_t *>(s.mass), mask, at, j, begin);
+    }
+    return finish_list<BLOCK, T>(s, o, row, begin + pieces * E + threadIdx.x, end, want);
 }
 
 template <int BLOCK>
@@ -777,14 +811,13 @@ __device__ __forceinline__ int tile_of(int size) {
 // This lane's 16 kept masses of the 1024 entries from `base`; their sum
 template <typename T>
 __device__ __forceinline__ double lane_masses(const RowState &o, const T *row, int size, int base, double *e) {
-    constexpr int E = 16 / sizeof(T);
-    struct __attribute__((packed, aligned(sizeof(T)))) Vec { T e[E]; };
+    constexpr int E = Vec<T>::E;
     const int i0 = base + (threadIdx.x & 63) * 16;
     T x[16];
     if (i0 + 16 <= size) {
 #pragma unroll
         for (int v = 0; v < 16 / E; ++v) {
-            const Vec p = *reinterpret_cast<const Vec *>(row + i0 + v * E);
+            const Vec<T> p = *reinterpret_cast<const Vec<T> *>(row + i0 + v * E);
 #pragma unroll
             for (int j = 0; j < E; ++j) x[v * E + j] = p.e[j];
         }
@@ -977,16 +1010,40 @@ __global__ void __launch_bounds__(256) sample_short_kernel(const SampleArgs a) {
     draw_top_k<BLOCK>(s, o, uniform(s.count), fmaxf(low, -3e38f), size, io.u, a.draws, io.ids, io.prob);
 }
 
-template <typename T>
+// HELD: 16-byte pieces a thread keeps in registers from the pass for the maximum to that for the list, 0 where the row is read again
+template <typename T, int HELD>
 __global__ void __launch_bounds__(1024) sample_row_kernel(const SampleArgs a) {
-    constexpr int BLOCK = 1024;
+    constexpr int BLOCK = 1024, E = Vec<T>::E;
     __shared__ Shared<BLOCK> s;
     __shared__ Histogram h;
     __shared__ double tiles[kMaxTiles];
-    const int tid = threadIdx.x, size = a.size;
+    const int tid = threadIdx.x, size = a.size, pieces = size / E;
     const RowIO<T> io(a, blockIdx.x);
     float group[4] = {-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()}, low = __builtin_inff();
-    for_each<BLOCK>(io.row, 0, size, [&](float x, int, int u) { group[u] = fmaxf(group[u], x), low = fminf(low, x); });
+    typedef uint32_t Raw __attribute__((ext_vector_type(4)));
+    Raw held[HELD > 0 ? HELD : 1];
+    if constexpr (HELD > 0) {
+        const Vec<T> *v = reinterpret_cast<const Vec<T> *>(io.row);
+#pragma unroll
+        for (int u = 0; u < HELD; ++u)
+            if (u * BLOCK < pieces) held[u] = __builtin_bit_cast(Raw, v[min(u * BLOCK + tid, pieces - 1)]);
+#pragma unroll
+        for (int u = 0; u < HELD; ++u)
+            if (u * BLOCK + tid < pieces) {
+                const Vec<T> p = __builtin_bit_cast(Vec<T>, held[u]);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float x = to_f32(p.e[e]);
+                    group[u & 3] = fmaxf(group[u & 3], x), low = fminf(low, x);
+                }
+            }
+        if (pieces * E + tid < size) {
+            const float x = to_f32(io.row[pieces * E + tid]);
+            group[0] = fmaxf(group[0], x), low = fminf(low, x);
+        }
+    } else {
+        for_each<BLOCK>(io.row, 0, size, [&](float x, int, int u) { group[u] = fmaxf(group[u], x), low = fminf(low, x); });
+    }
     if (tid < 16) s.tab[tid] = kRoots[tid];
     float top = fmaxf(fmaxf(group[0], group[1]), fmaxf(group[2], group[3]));
     block_max_min<BLOCK>(top, low, s);
@@ -996,6 +1053,7 @@ __global__ void __launch_bounds__(1024) sample_row_kernel(const SampleArgs a) {
         return draw_plain(o, at, io.u, a.draws, io.ids, io.prob, tid, BLOCK);
     }
     if (o.f.cut && o.f.k <= kGroupsMaxK) {
+        if (tid == 0) s.count = 0;
         clear_histogram<BLOCK>(h);
 #pragma unroll
         for (int u = 0; u < 4; ++u)
@@ -1004,7 +1062,33 @@ __global__ void __launch_bounds__(1024) sample_row_kernel(const SampleArgs a) {
         Above above{0, 0};
         const int bin = find_bin<BLOCK>(s, h, true, false, o.f.k, 0.0, above);
         if (bin < kBins) {
-            const uint32_t n = gather<BLOCK, T>(s, o, io.row, 0, size, Reach(o, bin));
+            const Reach want(o, bin);
+            uint32_t n;
+            if constexpr (HELD > 0) {
+                uint32_t mask[HELD / 4], hits = 0;
+#pragma unroll
+                for (int u = 0; u < HELD; u += 4) {
+                    mask[u / 4] = 0;
+                    if (u * BLOCK < pieces) {
+                        Vec<T> p[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            // opaque: else the widened values of the first pass would be kept, in twice the registers
+                            asm volatile("" : "+v"(held[u + k]));
+                            p[k] = __builtin_bit_cast(Vec<T>, held[u + k]);
+                        }
+                        mask[u / 4] = reach_mask<BLOCK, T>(o, p, u * BLOCK + tid, pieces, want);
+                        hits += __popc(mask[u / 4]);
+                    }
+                }
+                uint32_t at = reserve(&s.count, hits);
+#pragma unroll
+                for (int u = 0; u < HELD; u += 4)
+                    at = put_mask<BLOCK, T>(reinterpret_cast<uint32_t *>(s.mass), mask[u / 4], at, u * BLOCK + tid, 0);
+                n = finish_list<BLOCK, T>(s, o, io.row, pieces * E + tid, size, want);
+            } else {
+                n = gather<BLOCK, T>(s, o, io.row, 0, size, want);
+            }
             if (n <= (uint32_t)kList) return draw_top_k<BLOCK>(s, o, n, o.w.topf - (float)(bin + 1) / o.scale, size, io.u, a.draws, io.ids, io.prob);
         }
     }
@@ -1023,17 +1107,16 @@ __device__ __forceinline__ bool more_after(const double *all, int c) {
 // ---- short rows without a cut: a wave a row of up to 64 P entries, in chunks of 16 bytes a lane (entry: chunk, lane, place)
 template <typename T, int P>
 __global__ void __launch_bounds__(256) sample_wave_kernel(const SampleArgs a) {
-    constexpr int E = 16 / sizeof(T), C = P / E;
+    constexpr int E = Vec<T>::E, C = P / E;
     __shared__ double tab[16];
     const int lane = threadIdx.x & 63, r = min((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6), a.rows - 1), size = a.size;
     const RowIO<T> io(a, r);
-    struct __attribute__((packed, aligned(sizeof(T)))) Vec { T e[E]; };
     float x[C][E], top = -__builtin_inff(), u = io.u[0];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int i = (c * 64 + lane) * E;
         if (i + E <= size) {
-            const Vec p = *reinterpret_cast<const Vec *>(io.row + i);
+            const Vec<T> p = *reinterpret_cast<const Vec<T> *>(io.row + i);
 #pragma unroll
             for (int j = 0; j < E; ++j) x[c][j] = to_f32(p.e[j]);
         } else {
@@ -1365,7 +1448,10 @@ void launch_sample(const SampleArgs &a, bool may_k, bool may_p, RowWork *work, h
     } else if (form == kShortForm) {
         sample_short_kernel<T><<<a.rows, 256, 0, s>>>(a);
     } else if (form == kRowForm) {
-        sample_row_kernel<T><<<a.rows, 1024, 0, s>>>(a);
+        // 16 pieces of 1024 threads hold 131072 16-bit or 65536 f32 logits; they pay where top-k reads the row twice (256 rows of
+        // 131072: 40.0 us against 41.6)
+        if (may_k && a.size <= 16 * 1024 * Vec<T>::E) sample_row_kernel<T, 16><<<a.rows, 1024, 0, s>>>(a);
+        else sample_row_kernel<T, 0><<<a.rows, 1024, 0, s>>>(a);
     } else {
         const dim3 parts(kParts, a.rows);
         sample_max_kernel<T><<<parts, 1024, 0, s>>>(a, work);
