@@ -646,6 +646,198 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const SumArgs a, const I 
     }
 }
 
+// ---------------------------------------------------------------------------------------------------- up to 16384 tokens: ranges
+// One launch, no workspace: a block for each CU takes 2^low table rows and up to 64 vectors of their columns.  It reads all ids and
+// lists its own tokens in order (ballots), ranks them by row in LDS, and writes the sums of its rows, zeros included.  Rows of up to
+// kLight tokens are a team's (several to a wave), up to kWaveTokens times a wave's teams a wave's, others the block's; the teams' sums
+// are added by halves, the waves' in order.  Its rows lie in groups of 64 bytes or more, 2^bits groups apart: neighbouring rows are
+// often met alike (frequent ids first), and 16384 such tokens x 4 bf16 over 74009 rows take 45 us in one range, 24 in groups of 256
+// bytes and 17.5 in groups of 64.  4096 x 10 bf16 over 12011 rows: 9.9 us a call (sorted 17); 16384 x 64 over 8000: 11.8 (24).
+constexpr int kLight = 16;
+constexpr int kWaveTokens = 64;
+constexpr int kMaxLow = 10;
+struct Ranges {                // a row is high bits, block (`bits`), place in a group (`group`); its number in the block: first and last
+    int bits, group, low;
+    __device__ __forceinline__ uint32_t block_of(uint32_t row) const { return (row >> group) & ((1u << bits) - 1); }
+    __device__ __forceinline__ uint32_t own_of(uint32_t row) const { return row >> (bits + group) << group | (row & ((1u << group) - 1)); }
+    __device__ __forceinline__ uint32_t row_of(uint32_t block, uint32_t own) const {
+        return (own >> group << bits | block) << group | (own & ((1u << group) - 1));
+    }
+};
+
+template <typename G, typename T, int VW, int ITEMS>
+__global__ void __launch_bounds__(1024, 8) sum_ranges_kernel(const SumArgs a, const void *__restrict__ ids, int wide, int64_t padding, const Ranges w) {
+    __shared__ uint32_t list[1024 * ITEMS];                // row in the range << 14 | position; then positions by row
+    __shared__ union {
+        uint16_t cnt[16][1 << kMaxLow];
+        float part[16][64 * VW];
+    } u;
+    __shared__ uint16_t start[(1 << kMaxLow) + 1], heavy[1 << kMaxLow];
+    __shared__ uint32_t sums[16], heavy_count;
+    uint16_t *sorted = reinterpret_cast<uint16_t *>(list);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = (int)a.n;
+    const uint32_t range = blockIdx.x / a.chunks, rows = 1u << w.low;
+    const int teams = 64 / a.lanes, of_wave = lane / a.lanes, team = wave * teams + of_wave;           // teams of a wave
+    const int in_team = lane - of_wave * a.lanes, col = ((int)(blockIdx.x - range * a.chunks) * a.lanes + in_team) * VW;
+    const bool works = of_wave < teams && col < a.dim;
+    const G *g = (const G *)a.g + (works ? col : 0);
+    // the tokens of the range, in order (items in order: wave, item, lane)
+    const int items = (n + 1023) / 1024, per = items * 64;
+    uint32_t key[ITEMS], m = 0;
+    uint64_t hits[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+        if (k < items) {
+            const int i = wave * per + k * 64 + lane, at = i < n ? i : n - 1;
+            const uint32_t v = key_of(wide ? ((const int64_t *)ids)[at] : (int64_t)((const int32_t *)ids)[at], a.n_rows, padding);
+            key[k] = i < n ? v : a.n_rows;
+        }
+    if (tid == 0) heavy_count = 0;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+        if (k < items) {
+            hits[k] = __ballot(key[k] < a.n_rows && w.block_of(key[k]) == range);
+            m += __popcll(hits[k]);
+        }
+    if (lane == 0) sums[wave] = m;
+    __syncthreads();
+    uint32_t at = 0;
+    m = 0;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+        if (v == wave) at = m;
+        m += sums[v];
+    }
+    if (m == 0) {                                          // no token: the zeros
+        Pack<T, VW> zero;
+#pragma unroll
+        for (int j = 0; j < VW; ++j) zero.e[j] = from_f32<T>(0.0f);
+        if (works)
+            for (uint32_t r = team; r < rows; r += 16 * teams) {
+                const uint32_t row = w.row_of(range, r);
+                if (row < a.n_rows) *reinterpret_cast<Pack<T, VW> *>((T *)a.grad + (int64_t)row * a.dim + col) = zero;
+            }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+        if (k < items) {
+            if ((hits[k] >> lane) & 1) list[at + lanes_below(hits[k])] = w.own_of(key[k]) << 14 | (wave * per + k * 64 + lane);
+            at += __popcll(hits[k]);
+        }
+    for (uint32_t b = lane; b < (rows + 1) / 2; b += 64) reinterpret_cast<uint32_t *>(u.cnt[wave])[b] = 0;
+    __syncthreads();
+    // stable, by row
+    const int mine = (m + 1023) / 1024;
+    uint32_t entry[ITEMS], rank[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+        if (k < mine) {
+            const uint32_t e = wave * (mine * 64) + k * 64 + lane;
+            const bool on = e < m;
+            entry[k] = list[on ? e : 0];
+            rank[k] = wave_rank(u.cnt[wave], on ? entry[k] >> 14 : 0, w.low, on);
+        }
+    __syncthreads();
+    uint32_t total = 0;
+    if (tid < (int)rows)
+        for (int v = 0; v < 16; ++v) {
+            const uint32_t c = u.cnt[v][tid];
+            u.cnt[v][tid] = (uint16_t)total;
+            total += c;
+        }
+    const uint32_t first = block_scan<16>(total, sums);
+    if (tid < (int)rows) start[tid] = (uint16_t)first;
+    if (tid == 0) start[rows] = (uint16_t)m;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+        if (k < mine && wave * (mine * 64) + k * 64 + lane < m)
+            sorted[start[entry[k] >> 14] + u.cnt[wave][entry[k] >> 14] + rank[k]] = (uint16_t)(entry[k] & 0x3fff);
+    __syncthreads();
+    const auto load = [&](uint32_t q) { return *reinterpret_cast<const Pack<G, VW> *>(g + (int64_t)sorted[q] * a.g_stride); };
+    // acc += the tokens q, q + step ... below hi
+    const auto add = [&](float *acc, uint32_t q0, uint32_t hi, uint32_t step) {
+        for (uint32_t q = q0; q < hi; q += kBatch * step) {
+            Pack<G, VW> v[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) v[k] = load(q + k * step < hi ? q + k * step : q);
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+                for (int j = 0; j < VW; ++j) acc[j] += q + k * step < hi ? to_f32(v[k].e[j]) : 0.0f;
+        }
+    };
+    if (works)
+        for (uint32_t r0 = team; r0 < rows; r0 += 4 * 16 * teams) {         // four rows' first tokens in flight
+            Pack<G, VW> v[4];
+            uint32_t lo[4], c[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t r = r0 + k * 16 * teams < rows ? r0 + k * 16 * teams : r0;
+                lo[k] = start[r], c[k] = start[r + 1] - lo[k];
+            }
+            if (c[0] | c[1] | c[2] | c[3]) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = load(c[k] ? lo[k] : 0);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t r = r0 + k * 16 * teams, row = w.row_of(range, r);
+                if (r >= rows || row >= a.n_rows) break;
+                if (c[k] > kLight) {
+                    if (in_team == 0) heavy[atomicAdd(&heavy_count, 1u)] = (uint16_t)r;
+                    continue;
+                }
+                float acc[VW];
+#pragma unroll
+                for (int j = 0; j < VW; ++j) acc[j] = c[k] ? to_f32(v[k].e[j]) : 0.0f;
+                if (c[k] > 1) add(acc, lo[k] + 1, lo[k] + c[k], 1);
+                store_row<G, T, VW>(a, row, col, acc);
+            }
+        }
+    __syncthreads();
+    const auto add_teams = [&](float *acc) {               // the wave's sums, in its first team
+        for (int t = teams; t > 1;) {
+            const int half = (t + 1) / 2;
+#pragma unroll
+            for (int j = 0; j < VW; ++j) {
+                const float other = __shfl(acc[j], (lane + half * a.lanes) & 63);
+                acc[j] += of_wave + half < t ? other : 0.0f;
+            }
+            t = half;
+        }
+    };
+    const uint32_t heavies = heavy_count;
+    for (uint32_t h = wave; h < heavies; h += 16) {
+        const int r = heavy[h];
+        const uint32_t lo = start[r], hi = start[r + 1];
+        if ((int)(hi - lo) > kWaveTokens * teams) continue;
+        float acc[VW] = {};
+        if (works) add(acc, lo + of_wave, hi, teams);
+        add_teams(acc);
+        if (works && of_wave == 0) store_row<G, T, VW>(a, w.row_of(range, r), col, acc);
+    }
+    for (uint32_t h = 0; h < heavies; ++h) {
+        const int r = heavy[h];
+        const uint32_t lo = start[r], hi = start[r + 1];
+        if ((int)(hi - lo) <= kWaveTokens * teams) continue;
+        float acc[VW] = {};
+        if (works) add(acc, lo + team, hi, 16 * teams);
+        add_teams(acc);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < VW; ++j) u.part[wave][lane * VW + j] = acc[j];
+        __syncthreads();
+        if (works && team == 0) {
+            for (int v = 1; v < 16; ++v)
+#pragma unroll
+                for (int j = 0; j < VW; ++j) acc[j] += u.part[v][lane * VW + j];
+            store_row<G, T, VW>(a, w.row_of(range, r), col, acc);
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------------------- narrow rows
 // Rows of g of up to 8 elements, more than a tile of tokens.  Gathering such rows by position fetches a cache line for each (44 us of
 // 111 for 2^21 rows of two f32), and a second digit moves all pairs once more: here the rows travel with their ids through ONE
@@ -944,7 +1136,7 @@ struct BwdPlan {
     int64_t off_a, off_b, off_counts, off_totals, off_head, off_tail, bytes;       // all zero: few tokens, no workspace
 };
 
-// Few tokens: without a sort (one or two launches against three or more).  The ids are read once a row or token, and a block may
+// Few rows, few tokens: without a sort (one or two launches against three or more).  The ids are read once a row or token, and a block may
 // meet all of g: each of its teams then 256 tokens at most, about 20 us.
 // Measured, us a call, against the sorted way: 4096 tokens x 32 over 100 rows 9.0 / 16.5, all on one row 10.2 / 17.7; 16384 x 8 over
 // 256 rows 11.7 / 31; 64 x 1024 over 1024 rows 9.2 / 16.2.
@@ -957,9 +1149,16 @@ Few few_tokens(int64_t n, int64_t n_rows, int dim) {
     return n <= 4096 ? kFewTokens : kNotFew;
 }
 
+// Ranges (what few rows leave): not for large gradients, whose zeros a launch of their own writes faster than blocks that wait for ids
+// (27442 rows x 263 f32: one token 22 us against 12, 4096 tokens 27 against 26; 9298 x 544: 10.5 against 12, 17 against 24), nor where
+// many blocks would read many ids (16384 tokens over 2^19 rows x 10: 25 against 29).
+bool in_ranges(int64_t n, int64_t n_rows, int dim) {
+    return n <= kSmall && n_rows * dim <= 6 << 20 && n_rows * n <= (int64_t)1 << 33;
+}
+
 BwdPlan plan_bwd(int64_t n, int64_t n_rows, int dim) {
     BwdPlan p{};
-    if (few_tokens(n, n_rows, dim) != kNotFew) return p;
+    if (few_tokens(n, n_rows, dim) != kNotFew || in_ranges(n, n_rows, dim)) return p;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
     if (dim <= 8 && n_rows > 0 && n_rows <= 1 << 20 && n > kTile) {
@@ -1081,6 +1280,28 @@ void launch_narrow(const SumArgs &sa, const BwdPlan &p, const void *ids, bool i6
     narrow_join_kernel<T><<<a.bins, 1024, 0, s>>>(a);
 }
 
+// A block for each of 256 CUs: as many ranges of rows as give that, then columns in pieces, which share a row of many tokens
+template <typename G, typename T, int VW>
+void launch_ranges(SumArgs a, const void *ids, bool i64, int64_t padding, hipStream_t s) {
+    const int vectors = a.dim / VW;
+    int most = 64, total = 0;                              // vectors: 4 MB of f32 in a block, should all tokens be its own
+    while (most > 1 && (int64_t)most * VW * a.n > 1 << 20) most /= 2;
+    while ((int64_t)1 << total < a.n_rows) ++total;
+    a.chunks = (vectors + most - 1) / most;
+    Ranges w{};
+    while (w.bits < total && (2 << w.bits) * a.chunks <= 256) ++w.bits;
+    const int pieces = a.dim * (int)sizeof(G) / 32;        // of 32 bytes or more
+    const int split = pieces < 256 >> w.bits ? pieces : 256 >> w.bits;
+    if (w.bits == total && split > a.chunks) a.chunks = split;
+    while (total - w.bits > kMaxLow) ++w.bits;
+    w.low = total - w.bits;
+    while (w.group < w.low && a.dim * (int)sizeof(T) << w.group < 64) ++w.group;
+    a.lanes = (vectors + a.chunks - 1) / a.chunks;
+    const unsigned blocks = (1u << w.bits) * a.chunks;
+    if (a.n <= kTile) sum_ranges_kernel<G, T, VW, kTileItems><<<blocks, 1024, 0, s>>>(a, ids, i64, padding, w);
+    else sum_ranges_kernel<G, T, VW, kItems><<<blocks, 1024, 0, s>>>(a, ids, i64, padding, w);
+}
+
 template <typename G, typename T, int VW>
 void launch_sums(SumArgs a, const BwdPlan &p, const void *ids, bool i64, int64_t padding, hipStream_t s) {
     const int vectors = a.dim / VW;
@@ -1092,6 +1313,7 @@ void launch_sums(SumArgs a, const BwdPlan &p, const void *ids, bool i64, int64_t
             else sum_rows_kernel<G, T, VW, int32_t, false><<<blocks, 256, 0, s>>>(a, (const int32_t *)ids, padding);
             return;
         }
+        if (in_ranges(a.n, a.n_rows, a.dim)) return launch_ranges<G, T, VW>(a, ids, i64, padding, s);
         const int64_t bytes = (int64_t)a.n_rows * a.dim * (int64_t)sizeof(T);
         zero_kernel<<<(unsigned)((bytes + kFill - 1) / kFill), 1024, 0, s>>>((char *)a.grad, bytes);
         const unsigned blocks = (unsigned)a.n * a.chunks;

@@ -62,7 +62,9 @@ def check_bwd(g, ids, V, scale, pad, grad):
 # n, V, D: one token, one column, odd sizes, rows that are not 16-byte multiples, wide rows, sizes around the sorts' borders
 SHAPES = [(1, 1, 1), (1, 7, 48), (3, 2, 5), (64, 100, 32), (65, 100, 33), (1000, 3, 27), (4097, 300, 8), (300, 70000, 4),
           (900, 100000, 4), (1024, 4097, 9), (2440, 9464, 8), (4096, 50000, 3), (8056, 195952, 5), (6000, 700, 65), (5000, 1, 8), (70000, 3, 1), (30000, 1000, 7),
-          (200000, 1 << 20, 1), (9000, (1 << 20) + 1, 2), (150000, 1025, 4), (300001, 600000, 2), (4100, 5000, 33), (16384, 1025, 12), (16385, 1500, 16), (20000, 5, 2), (50001, 4096, 3), (33, 1000, 4096), (40, 9, 1111), (2, 3, 32768)]
+          (200000, 1 << 20, 1), (9000, (1 << 20) + 1, 2), (150000, 1025, 4), (300001, 600000, 2), (4100, 5000, 33), (16384, 1025, 12), (16385, 1500, 16), (20000, 5, 2), (50001, 4096, 3), (33, 1000, 4096), (40, 9, 1111), (2, 3, 32768),
+          (17, 50000, 40), (2000, 1, 512), (4095, 2049, 1), (4096, 3000, 258), (9000, 2, 4100), (12000, 5000, 515), (16383, 524288, 12),
+          (16384, 1000, 64), (16384, 20000, 1), (300, 1, 32767), (3000, 4000, 1700), (100, 1 << 21, 5), (70000, 900, 36)]
 
 
 @pytest.mark.parametrize("n,V,D", SHAPES)
@@ -80,7 +82,7 @@ def test_forward_and_gradient(n, V, D, kind):
 
 
 @pytest.mark.parametrize("t,o", [("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f16", "f32")])
-@pytest.mark.parametrize("n,V,D", [(1, 4, 64), (777, 50, 33), (5000, 900, 24), (20000, 1 << 19, 2), (130, 60, 2056), (9001, 3000, 5), (8000, 70, 8)])
+@pytest.mark.parametrize("n,V,D", [(1, 4, 64), (777, 50, 33), (5000, 900, 24), (20000, 1 << 19, 2), (130, 60, 2056), (9001, 3000, 5), (8000, 70, 8), (15000, 3001, 36)])
 def test_sixteen_bit_tables(t, o, n, V, D):
     from nerf_amd import ops
     rng = np.random.RandomState(D)
@@ -95,7 +97,7 @@ def test_sixteen_bit_tables(t, o, n, V, D):
     check_bwd(g, ids, V, 5.5, None, grad)
 
 
-@pytest.mark.parametrize("n", [500, 40000])
+@pytest.mark.parametrize("n", [500, 15000, 40000])
 def test_ids_outside_the_table_and_the_padding_row(n):
     from nerf_amd import ops
     rng = np.random.RandomState(3)
@@ -239,12 +241,13 @@ def test_autograd_and_differences():
         assert not codes(ids).requires_grad
 
 
-def test_another_stream_and_a_captured_training_step():
+@pytest.mark.parametrize("n", [700, 12000, 20000])
+def test_another_stream_and_a_captured_training_step(n):
     from nerf_amd.codes import lookup
     rng = np.random.RandomState(2)
     table = torch.from_numpy(rng.normal(size=(300, 24)).astype(np.float32)).cuda().requires_grad_()
-    ids = make_ids("zipf", 20000, 300, rng).cuda()
-    w = torch.from_numpy(rng.normal(size=(20000, 24)).astype(np.float32)).cuda()
+    ids = make_ids("zipf", n, 300, rng).cuda()
+    w = torch.from_numpy(rng.normal(size=(n, 24)).astype(np.float32)).cuda()
 
     def step():
         out = lookup(table, ids, 0.5)
