@@ -23,6 +23,7 @@
 // about 1000 and top-p: 45 us, instructions: two passes of some four a logit; top-p alone 117 us, an f64 exponential a logit); and,
 // for few long rows, 32 blocks a row over several launches (4096 draws from 640000 f32, top-p: 54 us in five; one of 131072 by top-k: 17 us
 // in two), where the block that arrives last at a stage's end does what needs the whole row.
+#include <algorithm>
 #include "nrf_types.h"
 
 using namespace nrf;
@@ -866,14 +867,14 @@ __device__ __forceinline__ bool pick_entry(const double *e, double sum, double c
     return over != 0;
 }
 
-// tiles[0 .. n) -> running sums
-template <int BLOCK>
-__device__ __forceinline__ void scan_tiles(Shared<BLOCK> &s, double *tiles, int n) {
+// tiles[0 .. n) -> running sums; load(q): tile q
+template <int BLOCK, typename S, typename L>
+__device__ __forceinline__ void scan_tiles(S &s, double *tiles, int n, L load) {
     constexpr int kPer = kMaxTiles / BLOCK;
     const int q0 = threadIdx.x * kPer;
     double v[kPer], run = 0.0, total;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] = q0 + j < n ? tiles[q0 + j] : 0.0, run += v[j];
+    for (int j = 0; j < kPer; ++j) v[j] = q0 + j < n ? load(q0 + j) : 0.0, run += v[j];
     double cum = block_scan<BLOCK, double>(run, s.wave_d, &total);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
@@ -939,7 +940,7 @@ __device__ __forceinline__ void draw_whole_row(Shared<BLOCK> &s, double *tiles, 
         if ((tid & 63) == 0) tiles[q] = m;
     }
     __syncthreads();
-    scan_tiles<BLOCK>(s, tiles, n_tiles);
+    scan_tiles<BLOCK>(s, tiles, n_tiles, [&](int q) { return tiles[q]; });
     for (int j = tid >> 6; j < draws; j += BLOCK / 64) draw_from_tiles<T>(o, row, size, tile, tiles, n_tiles, u[j], ids + j, prob + j);
 }
 
@@ -1206,18 +1207,25 @@ __device__ __forceinline__ RowState state_of(const SampleArgs &a, int r, const R
     return row_state(a, r, wave_max(w.top[part]), -wave_max(-w.low[part]), tab);
 }
 
-// Whether this block is the last of its row at this point: what the others wrote before is visible to it then.  Every wave's
-// stores have left the compute unit before the barrier; one release (a write-back of the XCD's L2) and one acquire a block.
-template <int BLOCK>
-__device__ __forceinline__ bool last_to_arrive(Shared<BLOCK> &s, uint32_t *counter) {
+// What blocks of one launch hand to the last of them goes through the memory that all XCDs see, word by word (their L2s do not see
+// each other's writes).  A fence at device scope instead writes back a whole L2 for each block: 33 us for 1024 blocks.
+template <typename V>
+__device__ __forceinline__ void publish(V *p, V v) {
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename V>
+__device__ __forceinline__ V fetch(const V *p) {
+    return __builtin_bit_cast(V, __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// Whether this block is the last of its row at this point: what the others published before is there then.  Every wave waits for
+// its stores to arrive before the barrier, and the count is raised behind it.
+template <typename S>
+__device__ __forceinline__ bool last_to_arrive(S &s, uint32_t *counter) {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        s.found[0] = atomicAdd(counter, 1u) + 1 == gridDim.x;
-        __threadfence();
-    }
+    if (threadIdx.x == 0) s.found[0] = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == gridDim.x;
     __syncthreads();
     const bool last = uniform((uint32_t)s.found[0]);
     __syncthreads();
@@ -1232,7 +1240,7 @@ __device__ __forceinline__ void gather_part(Shared<BLOCK> &s, const RowState &o,
     if (threadIdx.x == 0) s.found[0] = n ? atomicAdd(count, n) : 0;
     __syncthreads();
     const uint32_t at = uniform((uint32_t)s.found[0]);
-    for (uint32_t i = threadIdx.x; i < n && i < (uint32_t)kList && at + i < (uint32_t)kList; i += BLOCK) list[at + i] = s.list[i];
+    for (uint32_t i = threadIdx.x; i < n && i < (uint32_t)kList && at + i < (uint32_t)kList; i += BLOCK) publish(&list[at + i], s.list[i]);
 }
 
 // The row's whole list into LDS; its length
@@ -1240,8 +1248,8 @@ template <int BLOCK>
 __device__ __forceinline__ uint32_t load_list(Shared<BLOCK> &s, const uint64_t *list, const uint32_t *count) {
     uint64_t c[kList / BLOCK];                             // in flight together with the length
 #pragma unroll
-    for (int j = 0; j < kList / BLOCK; ++j) c[j] = list[j * BLOCK + threadIdx.x];
-    const uint32_t n = uniform(*count);
+    for (int j = 0; j < kList / BLOCK; ++j) c[j] = fetch(&list[j * BLOCK + threadIdx.x]);
+    const uint32_t n = uniform(__hip_atomic_load(count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 #pragma unroll
     for (int j = 0; j < kList / BLOCK; ++j) s.list[j * BLOCK + threadIdx.x] = c[j];
     if (threadIdx.x == 0) s.count = n;
@@ -1314,7 +1322,7 @@ __global__ void __launch_bounds__(1024) sample_groups_kernel(const SampleArgs a,
     const int bin = find_bin<BLOCK>(s, h, true, false, o.f.k, 0.0, above);
     const Part p = part_of(a.size, blockIdx.x);
     if (bin < kBins) gather_part<BLOCK, T>(s, o, io.row, p, Reach(o, bin), w.list, &w.count[0]);
-    if (!last_to_arrive<BLOCK>(s, &w.arrived[0])) return;
+    if (!last_to_arrive(s, &w.arrived[0])) return;
     const uint32_t n = load_list<BLOCK>(s, w.list, &w.count[0]);
     if (bin < kBins && n <= (uint32_t)kList) {
         draw_top_k<BLOCK>(s, o, n, o.w.topf - (float)(bin + 1) / o.scale, a.size, io.u, a.draws, io.ids, io.prob);
@@ -1365,7 +1373,7 @@ __global__ void __launch_bounds__(1024) sample_cut_kernel(const SampleArgs a, Ro
     const Part p = part_of(a.size, blockIdx.x);
     const Step st = first_step<BLOCK>(s, h, o);
     if (st.any && st.fits) gather_part<BLOCK, T>(s, o, io.row, p, Reach(st.from, st.bin), w.list, &w.count[1]);
-    if (!last_to_arrive<BLOCK>(s, &w.arrived[1])) return;
+    if (!last_to_arrive(s, &w.arrived[1])) return;
     if (st.any && st.fits) load_list<BLOCK>(s, w.list, &w.count[1]);       // as many as the histogram counted: they fit
     const int listed = select_cut<BLOCK, T>(s, h, o, io.row, a.size, st, st.any && st.fits);
     if (listed > 0) {
@@ -1382,11 +1390,15 @@ __device__ __forceinline__ RowState cut_state(const SampleArgs &a, int r, const 
     return o;
 }
 
-// Stage 5: masses of the tiles, a wave each; by the last block their running sums.
+// Stage 5: masses of the tiles, a wave each (64 rows of 524288: 41 us); by the last block their running sums.
+struct TileShared {
+    double tab[16], wave_d[4];
+    uint64_t found[1];
+};
 template <typename T>
 __global__ void __launch_bounds__(256) sample_tiles_kernel(const SampleArgs a, RowWork *work) {
     constexpr int BLOCK = 256;
-    __shared__ Shared<BLOCK> s;
+    __shared__ TileShared s;
     const int tid = threadIdx.x, r = blockIdx.y, tile = tile_of(a.size), n = (a.size + tile - 1) / tile;
     RowWork &w = work[r];
     if (w.done) return;
@@ -1394,13 +1406,12 @@ __global__ void __launch_bounds__(256) sample_tiles_kernel(const SampleArgs a, R
     __syncthreads();
     const RowState o = cut_state(a, r, w, s.tab);
     if (o.plain()) return;
-    const int q = blockIdx.x * 4 + (tid >> 6);
     const RowIO<T> io(a, r);
-    if (q < n) {
+    for (int q = blockIdx.x * 4 + (tid >> 6); q < n; q += gridDim.x * 4) {
         const double m = tile_mass<T>(o, io.row, a.size, tile, q);
-        if ((tid & 63) == 0) w.tiles[q] = m;
+        if ((tid & 63) == 0) publish(&w.tiles[q], m);
     }
-    if (last_to_arrive<BLOCK>(s, &w.arrived[2])) scan_tiles<BLOCK>(s, w.tiles, n);
+    if (last_to_arrive(s, &w.arrived[2])) scan_tiles<BLOCK>(s, w.tiles, n, [&](int q) { return fetch(&w.tiles[q]); });
 }
 
 // Stage 6: the draws, a wave each.
@@ -1427,21 +1438,32 @@ __global__ void __launch_bounds__(256) sample_draw_kernel(const SampleArgs a, co
 
 // ---- host
 enum Form { kWaveForm, kShortForm, kRowForm, kPartsForm };
+enum Cut { kNoCut, kListCut, kWideCut };       // kListCut: a top-k that the groups' maxima bound
 
-// Long rows: with many of them, a block each fills the chip and is done in one launch; few of them are split.  Measured, one draw,
-// bf16, one block a row against split rows: top-k 50 131072 x 1: 19 / 18 us, 640000 x 1: 46 / 20, 640000 x 32: 55 / 50; top-p 32768 x 1:
-// 40 / 36, 32768 x 16: 41 / 51, 131072 x 16: 116 / 67, 131072 x 64: 117 / 196; no cut 131072 x 1: 45 / 19, x 16: 45 / 30, x 32: 45 / 49.
-// One block draws 16 at a time where the list does not hold all that is kept: one row of 37446, top-p, 16 draws 50 / 38, 64: 71 / 38, 2181:
-// 972 / 40.
-Form form_of(int64_t rows, int size, int draws, bool may_cut) {
-    if (size <= kList) return !may_cut && draws <= 16 ? kWaveForm : kShortForm;
-    if (rows <= 16) return size >= 65536 || draws > 16 ? kPartsForm : kRowForm;
-    return rows <= 64 && draws > 256 ? kPartsForm : kRowForm;
+// Long rows: with many of them, a block each fills the chip and is done in one launch; few of them are split.  Measured, bf16, one block
+// a row against split rows, us a call (one draw; 64; 256):
+//   no cut  65536 x 64 rows: 28 / 26, 48 / 29, 116 / 46    131072 x 96: 47 / 40, 67 / 46, 134 / 71    524288 x 32: 157 / 39, 177 / 41, 245 / 49
+//   top-k 50  131072 x 4: 19 / 18  131072 x 16: 19 / 33  262144 x 4: 28 / 20  524288 x 16: 43 / 34  524288 x 32: 44 / 56
+//   top-p 0.9  32768 x 16: 42 / 64, 65 / 65, 147 / 67    131072 x 32: 117 / 110, 141 / 110, 223 / 119    524288 x 64: 440 / 308, 464 / 311, 546 / 329
+// Without a list that holds all that is kept, one block draws 16 at a time.
+Form form_of(int64_t rows, int size, int draws, Cut cut) {
+    if (size <= kList) return cut == kNoCut && draws <= 16 ? kWaveForm : kShortForm;
+    bool parts;
+    if (cut == kNoCut) parts = draws > 16 ? rows <= 96 : size >= 65536 && rows <= 128 - (1 << 22) / size;
+    else if (cut == kListCut) parts = size >= 131072 && rows <= std::min(size / 32768, 64);
+    else parts = rows <= std::min(size / 4096 + draws / 8, std::clamp(draws / 8, 64, 512));
+    return parts ? kPartsForm : kRowForm;
+}
+
+// (a k of each row is unknown here: taken for a small one, but where many draws would make a large one slow)
+Cut cut_of(const SampleArgs &a, bool may_k, bool may_p) {
+    if (may_k && (a.top_k_v ? a.draws <= 64 : a.top_k <= kGroupsMaxK)) return kListCut;
+    return may_k || may_p ? kWideCut : kNoCut;
 }
 
 template <typename T>
 void launch_sample(const SampleArgs &a, bool may_k, bool may_p, RowWork *work, hipStream_t s) {
-    const Form form = form_of(a.rows, a.size, a.draws, may_k || may_p);
+    const Form form = form_of(a.rows, a.size, a.draws, cut_of(a, may_k, may_p));
     if (form == kWaveForm) {
         if (a.size <= 1024) sample_wave_kernel<T, 16><<<(a.rows + 3) / 4, 256, 0, s>>>(a);
         else sample_wave_kernel<T, 32><<<(a.rows + 3) / 4, 256, 0, s>>>(a);
@@ -1466,7 +1488,8 @@ void launch_sample(const SampleArgs &a, bool may_k, bool may_p, RowWork *work, h
         int tile = 1024;
         while ((a.size + tile - 1) / tile > kMaxTiles) tile <<= 1;
         const int n_tiles = (a.size + tile - 1) / tile;
-        sample_tiles_kernel<T><<<dim3((n_tiles + 3) / 4, a.rows), 256, 0, s>>>(a, work);
+        const int tile_blocks = std::min((n_tiles + 3) / 4, std::max(1, 2048 / a.rows));
+        sample_tiles_kernel<T><<<dim3(tile_blocks, a.rows), 256, 0, s>>>(a, work);
         const int draw_blocks = (a.draws + 3) / 4 < 1024 ? (a.draws + 3) / 4 : 1024;
         sample_draw_kernel<T><<<dim3(draw_blocks, a.rows), 256, 0, s>>>(a, work);
     }
@@ -1475,7 +1498,9 @@ void launch_sample(const SampleArgs &a, bool may_k, bool may_p, RowWork *work, h
 }  // namespace
 
 extern "C" int64_t nrf_sample_logits_workspace_bytes(int64_t n_rows, int32_t size, int32_t n_draws) {
-    return n_rows > 0 && form_of(n_rows, size, n_draws, true) == kPartsForm ? n_rows * (int64_t)sizeof(RowWork) : 0;
+    bool parts = false;
+    for (const Cut cut : {kNoCut, kListCut, kWideCut}) parts |= n_rows > 0 && form_of(n_rows, size, n_draws, cut) == kPartsForm;
+    return parts ? n_rows * (int64_t)sizeof(RowWork) : 0;
 }
 
 extern "C" int nrf_sample_logits(const void *logits, int64_t row_stride, int32_t dtype, int64_t n_rows, int32_t size, int32_t n_draws,
