@@ -82,7 +82,7 @@ def test_forward_and_gradient(n, V, D, kind):
 
 
 @pytest.mark.parametrize("t,o", [("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f16", "f32")])
-@pytest.mark.parametrize("n,V,D", [(1, 4, 64), (777, 50, 33), (5000, 900, 24), (20000, 1 << 19, 2), (130, 60, 2056), (9001, 3000, 5), (8000, 70, 8), (15000, 3001, 36)])
+@pytest.mark.parametrize("n,V,D", [(1, 4, 64), (777, 50, 33), (5000, 900, 24), (20000, 1 << 19, 2), (130, 60, 2056), (9001, 3000, 5), (8000, 70, 8), (15000, 3001, 36), (9000, 40, 2056), (9000, 40, 2057)])
 def test_sixteen_bit_tables(t, o, n, V, D):
     from nerf_amd import ops
     rng = np.random.RandomState(D)
