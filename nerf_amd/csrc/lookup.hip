@@ -23,15 +23,21 @@ namespace {
 
 constexpr int kMaxDim = 32768;
 
+// Rows are taken in vectors of VW elements at any alignment (the hardware splits what crosses a line); where VW does not divide a row,
+// its last vector overlaps the one before and both give the shared elements the same bits.  786432 x 33 f32, the sums of tiles: 20.8 us against
+// 37 by single elements.
+template <int VW>
+__device__ __forceinline__ int column(int vector, int dim) { return min(vector * VW, dim - VW); }
+
 // ---------------------------------------------------------------------------------------------------- forward
 constexpr int kFwdUnroll = 4;
 
 // A store past the caches, in words of up to 16 bytes
 template <int BYTES> struct Word;
 template <> struct Word<2> { typedef uint16_t type; };
-template <> struct Word<4> { typedef uint32_t type; };
-template <> struct Word<8> { typedef uint32_t type __attribute__((ext_vector_type(2))); };
-template <> struct Word<16> { typedef uint32_t type __attribute__((ext_vector_type(4))); };
+template <> struct Word<4> { typedef uint32_t type __attribute__((aligned(2))); };
+template <> struct Word<8> { typedef uint32_t type __attribute__((ext_vector_type(2), aligned(2))); };
+template <> struct Word<16> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2))); };
 template <typename V>
 __device__ __forceinline__ void store_once(V *p, V v) {
     constexpr int W = sizeof(V) < 16 ? sizeof(V) : 16, N = sizeof(V) / W;
@@ -42,11 +48,11 @@ __device__ __forceinline__ void store_once(V *p, V v) {
     for (int k = 0; k < N; ++k) __builtin_nontemporal_store(all.w[k], reinterpret_cast<U *>(p) + k);
 }
 
-// blockDim 256; chunk = VW elements of one row; `per_row` = dim / VW; magic = ceil(2^32 / per_row).  An output that the L2s could not
+// blockDim 256; chunk = VW elements of one row; `per_row` = dim / VW, up; magic = ceil(2^32 / per_row).  An output that the L2s could not
 // hold (32 MB) goes past them, which leaves them to rows that are met again: 16384 ids x 4096 bf16 34.5 us against 36.8.
 template <typename T, typename O, int VW, typename I>
 __global__ void __launch_bounds__(256) lookup_fwd_kernel(const T *__restrict__ table, int64_t stride, int64_t n_rows,
-                                                         const I *__restrict__ ids, int64_t chunks, uint32_t per_row,
+                                                         const I *__restrict__ ids, int64_t chunks, int dim, uint32_t per_row,
                                                          uint32_t magic, float scale, O *__restrict__ out) {
     const int64_t c0 = (int64_t)blockIdx.x * (256 * kFwdUnroll);
     const int64_t r0 = c0 / per_row;                       // block-uniform: one 64-bit division a block
@@ -54,7 +60,8 @@ __global__ void __launch_bounds__(256) lookup_fwd_kernel(const T *__restrict__ t
     const bool once = chunks * (int64_t)sizeof(Pack<O, VW>) > 32 << 20;
     Pack<T, VW> v[kFwdUnroll];
     int64_t id[kFwdUnroll];
-    uint32_t col[kFwdUnroll];
+    int col[kFwdUnroll];
+    int64_t row[kFwdUnroll];
     // loads without branches between them: chunks behind the last one read the last one's row, ids outside the table row 0
 #pragma unroll
     for (int u = 0; u < kFwdUnroll; ++u) {
@@ -63,8 +70,9 @@ __global__ void __launch_bounds__(256) lookup_fwd_kernel(const T *__restrict__ t
         const uint32_t off = rem + local;
         // off < per_row + 1024 and per_row <= 32768: off * per_row < 2^32, where the product with the magic is exact
         const uint32_t q = per_row == 1 ? off : __umulhi(off, magic);
-        id[u] = (int64_t)ids[r0 + q];
-        col[u] = (off - q * per_row) * VW;
+        row[u] = r0 + q;
+        id[u] = (int64_t)ids[row[u]];
+        col[u] = column<VW>((int)(off - q * per_row), dim);
     }
     if (n_rows > 0) {
 #pragma unroll
@@ -81,7 +89,7 @@ __global__ void __launch_bounds__(256) lookup_fwd_kernel(const T *__restrict__ t
 #pragma unroll
             for (int j = 0; j < VW; ++j)
                 o.e[j] = from_f32<O>((uint64_t)id[u] < (uint64_t)n_rows ? to_f32(v[u].e[j]) * scale : __uint_as_float(0x7fc00000u));
-            Pack<O, VW> *to = reinterpret_cast<Pack<O, VW> *>(out + c * VW);
+            Pack<O, VW> *to = reinterpret_cast<Pack<O, VW> *>(out + row[u] * dim + col[u]);
             if (once) store_once(to, o);
             else *to = o;
         }
@@ -91,16 +99,16 @@ __global__ void __launch_bounds__(256) lookup_fwd_kernel(const T *__restrict__ t
 template <typename T, typename O, int VW>
 void launch_fwd(const void *table, int64_t stride, int64_t n_rows, const void *ids, bool i64, int64_t n, int dim, float scale,
                 void *out, hipStream_t s) {
-    const uint32_t per_row = (uint32_t)(dim / VW);
+    const uint32_t per_row = (uint32_t)((dim + VW - 1) / VW);
     const uint32_t magic = (uint32_t)(((1ull << 32) + per_row - 1) / per_row);
     const int64_t chunks = n * per_row;
     const int blocks = (int)((chunks + 256 * kFwdUnroll - 1) / (256 * kFwdUnroll));
     if (i64)
         lookup_fwd_kernel<T, O, VW, int64_t><<<blocks, 256, 0, s>>>((const T *)table, stride, n_rows, (const int64_t *)ids, chunks,
-                                                                    per_row, magic, scale, (O *)out);
+                                                                    dim, per_row, magic, scale, (O *)out);
     else
         lookup_fwd_kernel<T, O, VW, int32_t><<<blocks, 256, 0, s>>>((const T *)table, stride, n_rows, (const int32_t *)ids, chunks,
-                                                                    per_row, magic, scale, (O *)out);
+                                                                    dim, per_row, magic, scale, (O *)out);
 }
 
 template <typename T, typename O>
@@ -432,8 +440,9 @@ __device__ __forceinline__ Place place_of(const SumArgs &a) {
     const int64_t at = (int64_t)blockIdx.x * teams + team;
     Place p;
     p.tile = a.chunks == 1 ? at : at / a.chunks;
-    p.col = (int)(((at - p.tile * a.chunks) * a.lanes + (threadIdx.x - team * a.lanes)) * VW);
-    p.on = team < teams && p.tile < a.tiles && p.col < a.dim;
+    const int vector = (int)((at - p.tile * a.chunks) * a.lanes + (threadIdx.x - team * a.lanes));
+    p.col = column<VW>(vector, a.dim);
+    p.on = team < teams && p.tile < a.tiles && vector * VW < a.dim;
     return p;
 }
 
@@ -553,7 +562,7 @@ __global__ void __launch_bounds__(256) sum_join_kernel(const SumArgs a) {
     for (int q = 0; q < count; ++q) {
         const int who = long_team[q];
         const int64_t wat = (int64_t)blockIdx.x * teams + who, wt = a.chunks == 1 ? wat : wat / a.chunks;
-        const int col = (int)(((wat - wt * a.chunks) * a.lanes + lane) * VW);
+        const int vector = (int)((wat - wt * a.chunks) * a.lanes + lane), col = column<VW>(vector, a.dim);
         const uint32_t key = a.pairs[wt * a.tile + a.tile - 1].x;
         // tiles of the run behind the first: the last one whose first token carries the id, 256 probes a round
         int64_t lo = wt + 1, hi = a.tiles;                     // lo is one of them; hi is not
@@ -569,11 +578,11 @@ __global__ void __launch_bounds__(256) sum_join_kernel(const SumArgs a) {
         for (int j = 0; j < VW; ++j) acc[j] = 0.0f;
         const int64_t heads = lo - wt, slice = (heads + teams - 1) / teams, s0 = wt + 1 + team * slice;
         const int64_t s1 = s0 + slice < lo + 1 ? s0 + slice : lo + 1;
-        if (team < teams && col < a.dim && s0 < s1) add_heads<VW>(a, s0, s1, col, acc);
+        if (team < teams && vector * VW < a.dim && s0 < s1) add_heads<VW>(a, s0, s1, col, acc);
 #pragma unroll
         for (int j = 0; j < VW; ++j) part[threadIdx.x * VW + j] = acc[j];
         __syncthreads();
-        if (team == 0 && col < a.dim) {
+        if (team == 0 && vector * VW < a.dim) {
             float sum[VW];
 #pragma unroll
             for (int j = 0; j < VW; ++j) sum[j] = a.tail[wt * a.dim + col + j];
@@ -603,11 +612,11 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const SumArgs a, const I 
     __shared__ uint32_t waves[4];
     __shared__ float part[256 * VW];
     const int teams = 256 / a.lanes, team = threadIdx.x / a.lanes, lane = threadIdx.x - team * a.lanes;
-    const int which = blockIdx.x / a.chunks, col = ((int)(blockIdx.x - which * a.chunks) * a.lanes + lane) * VW;
+    const int which = blockIdx.x / a.chunks, vector = (int)(blockIdx.x - which * a.chunks) * a.lanes + lane, col = column<VW>(vector, a.dim);
     const int wave = threadIdx.x >> 6, wl = threadIdx.x & 63, n = (int)a.n;
     const int64_t row = BY_TOKEN ? (int64_t)ids[which] : which;
     if (BY_TOKEN && ((uint64_t)row >= (uint64_t)a.n_rows || row == padding)) return;
-    const bool works = team < teams && col < a.dim;
+    const bool works = team < teams && vector * VW < a.dim;
     const G *g = (const G *)a.g + (works ? col : 0);
     float acc[VW];
 #pragma unroll
@@ -686,7 +695,7 @@ struct Ranges {                // a row is high bits, block (`bits`), place in a
 };
 
 template <typename G, typename T, int VW, int ITEMS>
-__global__ void __launch_bounds__(1024, 8) sum_ranges_kernel(const SumArgs a, const void *__restrict__ ids, int wide, int64_t padding, const Ranges w) {
+__global__ void __launch_bounds__(1024, ITEMS > kTileItems ? 4 : 8) sum_ranges_kernel(const SumArgs a, const void *__restrict__ ids, int wide, int64_t padding, const Ranges w) {
     __shared__ uint32_t list[1024 * ITEMS];                // row in the range << 14 | position; then positions by row
     __shared__ union {
         uint16_t cnt[16][1 << kMaxLow];
@@ -698,8 +707,9 @@ __global__ void __launch_bounds__(1024, 8) sum_ranges_kernel(const SumArgs a, co
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = (int)a.n;
     const uint32_t range = blockIdx.x / a.chunks, rows = 1u << w.low;
     const int teams = 64 / a.lanes, of_wave = lane / a.lanes, team = wave * teams + of_wave;           // teams of a wave
-    const int in_team = lane - of_wave * a.lanes, col = ((int)(blockIdx.x - range * a.chunks) * a.lanes + in_team) * VW;
-    const bool works = of_wave < teams && col < a.dim;
+    const int in_team = lane - of_wave * a.lanes, vector = (int)(blockIdx.x - range * a.chunks) * a.lanes + in_team;
+    const int col = column<VW>(vector, a.dim);
+    const bool works = of_wave < teams && vector * VW < a.dim;
     const G *g = (const G *)a.g + (works ? col : 0);
     // the tokens of the range, in order (items in order: wave, item, lane)
     const int items = (n + 1023) / 1024, per = items * 64;
@@ -1162,8 +1172,8 @@ struct BwdPlan {
 // 256 rows 11.7 / 31; 64 x 1024 over 1024 rows 9.2 / 16.2.
 enum Few { kNotFew, kFewRows, kFewTokens };
 Few few_tokens(int64_t n, int64_t n_rows, int dim) {
-    const int vw = dim % 4 == 0 ? 4 : dim % 2 == 0 ? 2 : 1, lanes = dim / vw < 256 ? dim / vw : 256;
-    const int chunks = (dim / vw + 255) / 256;
+    const int vw = dim >= 4 ? 4 : dim >= 2 ? 2 : 1, vectors = (dim + vw - 1) / vw, lanes = vectors < 256 ? vectors : 256;
+    const int chunks = (vectors + 255) / 256;
     if (n > 256 * (256 / lanes)) return kNotFew;
     if (n_rows * chunks <= 4096 && n_rows * n <= 1 << 22) return kFewRows;
     return n <= 4096 ? kFewTokens : kNotFew;
@@ -1303,7 +1313,7 @@ void launch_narrow(const SumArgs &sa, const BwdPlan &p, const void *ids, bool i6
 // A block for each of 256 CUs: as many ranges of rows as give that, then columns in pieces, which share a row of many tokens
 template <typename G, typename T, int VW>
 void launch_ranges(SumArgs a, const void *ids, bool i64, int64_t padding, hipStream_t s) {
-    const int vectors = a.dim / VW;
+    const int vectors = (a.dim + VW - 1) / VW;
     int most = 64, total = 0;                              // vectors: 4 MB of f32 in a block, should all tokens be its own
     while (most > 1 && (int64_t)most * VW * a.n > 1 << 20) most /= 2;
     while ((int64_t)1 << total < a.n_rows) ++total;
@@ -1324,7 +1334,7 @@ void launch_ranges(SumArgs a, const void *ids, bool i64, int64_t padding, hipStr
 
 template <typename G, typename T, int VW>
 void launch_sums(SumArgs a, const BwdPlan &p, const void *ids, bool i64, int64_t padding, hipStream_t s) {
-    const int vectors = a.dim / VW;
+    const int vectors = (a.dim + VW - 1) / VW;
     a.chunks = (vectors + 255) / 256, a.lanes = (vectors + a.chunks - 1) / a.chunks, a.tiles = p.sum_tiles;
     if (p.bytes == 0) {
         if (few_tokens(a.n, a.n_rows, a.dim) == kFewRows) {
@@ -1358,10 +1368,10 @@ void pick_sums(int vw, const SumArgs &a, const BwdPlan &p, const void *ids, bool
     launch_sums<G, T, 1>(a, p, ids, i64, padding, s);
 }
 
-// the wider side's 16 bytes set the vector; both sides' addresses must be aligned to their share of it
-int common_width(int dim, int esz_a, uint64_t addr_a, int esz_b, uint64_t addr_b) {
-    const int a = vector_width(dim, esz_a, addr_a), b = vector_width(dim, esz_b, addr_b);
-    return a < b ? a : b;
+// Elements of a vector: 16 bytes of f32, or of 16-bit types where that divides a row (4096 x 420 bf16: 11 us a call by 4, 15 by 8)
+int width_of(int dim, int es_a, int es_b) {
+    if (es_a == 2 && es_b == 2 && dim % 8 == 0) return 8;
+    return dim >= 4 ? 4 : dim >= 2 ? 2 : 1;
 }
 
 bool pair_ok(int32_t narrow, int32_t wide) { return narrow == wide || (wide == NRF_F32 && dtype_size(narrow) == 2); }
@@ -1380,8 +1390,7 @@ extern "C" int nrf_lookup_fwd(const void *table, int64_t table_stride, int32_t d
     if (n == 0) return NRF_OK;
     NRF_REQUIRE(ids && out && (table || n_rows == 0), "nrf_lookup_fwd: null pointer");
     NRF_REQUIRE(table_stride >= dim, "nrf_lookup_fwd: table_stride %lld below dim %d", (long long)table_stride, dim);
-    const int es = dtype_size(dtype), eo = dtype_size(out_dtype);
-    const int vw = common_width(dim, es, (uint64_t)(uintptr_t)table | (uint64_t)table_stride * es, eo, (uint64_t)(uintptr_t)out);
+    const int vw = width_of(dim, dtype_size(dtype), dtype_size(out_dtype));
     hipStream_t s = as_stream(stream);
     const bool i64 = ids_are_64 != 0;
     if (dtype == NRF_F32) pick_fwd<float, float>(vw, table, table_stride, n_rows, ids, i64, n, dim, scale, out, s);
@@ -1414,8 +1423,7 @@ extern "C" int nrf_lookup_bwd(const void *g_out, int64_t g_stride, int32_t g_dty
     NRF_REQUIRE(grad && (n == 0 || (g_out && ids)) && (p.bytes == 0 || workspace), "nrf_lookup_bwd: null pointer");
     NRF_REQUIRE(n == 0 || g_stride >= dim, "nrf_lookup_bwd: g_stride %lld below dim %d", (long long)g_stride, dim);
     NRF_REQUIRE(((uintptr_t)workspace & 15) == 0, "nrf_lookup_bwd: workspace must be 16-byte aligned");
-    const int eg = dtype_size(g_dtype), es = dtype_size(dtype);
-    const int64_t grad_bytes = n_rows * dim * es;
+    const int64_t grad_bytes = n_rows * dim * dtype_size(dtype);
     hipStream_t s = as_stream(stream);
     const bool i64 = ids_are_64 != 0;
     char *ws = (char *)workspace;
@@ -1426,7 +1434,7 @@ extern "C" int nrf_lookup_bwd(const void *g_out, int64_t g_stride, int32_t g_dty
     if (p.bytes == 0 || n > 0) {
         a.g = g_out, a.g_stride = g_stride, a.grad = grad, a.head = (float *)(ws + p.off_head), a.tail = (float *)(ws + p.off_tail);
         a.n = n, a.n_rows = (uint32_t)n_rows, a.dim = dim, a.tile = p.tile, a.scale = scale;
-        const int vw = common_width(dim, eg, (uint64_t)(uintptr_t)g_out | (uint64_t)g_stride * eg, es, (uint64_t)(uintptr_t)grad);
+        const int vw = width_of(dim, dtype_size(g_dtype), dtype_size(dtype));
         if (g_dtype == NRF_F32 && dtype == NRF_F32) pick_sums<float, float>(vw, a, p, ids, i64, padding_idx, ws, s);
         else if (g_dtype == NRF_F32 && dtype == NRF_BF16) pick_sums<float, bf16_t>(vw, a, p, ids, i64, padding_idx, ws, s);
         else if (g_dtype == NRF_F32) pick_sums<float, f16_t>(vw, a, p, ids, i64, padding_idx, ws, s);

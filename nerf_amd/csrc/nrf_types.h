@@ -1,5 +1,5 @@
 // Element types of the operators that take more than f32 (nrf_dtype): loads of VW neighbouring elements as f32, stores with one
-// rounding (to nearest, ties to even).  A vector access needs its address aligned to the whole vector; callers pick VW so.
+// rounding (to nearest, ties to even).  A vector access needs its address aligned to an element only.
 #pragma once
 #include "nrf_common.h"
 
@@ -17,16 +17,8 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float v) { return bf16_t{__builtin_bit_cast(uint16_t, (__bf16)v)}; }
 template <> __device__ __forceinline__ f16_t from_f32<f16_t>(float v) { return f16_t{__builtin_bit_cast(uint16_t, (_Float16)v)}; }
 
-template <typename T, int VW> struct alignas(sizeof(T) * VW) Pack { T e[VW]; };
+template <typename T, int VW> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T e[VW]; };
 
 inline int dtype_size(int32_t t) { return t == NRF_F32 ? 4 : (t == NRF_BF16 || t == NRF_F16) ? 2 : 0; }
-
-// Largest of 16 bytes' worth of elements, halved until it divides `dim` and every address (base and row stride, in bytes)
-// is aligned to it: one element always is.
-inline int vector_width(int64_t dim, int elem, uint64_t addresses) {
-    int vw = 16 / elem;
-    while (vw > 1 && (dim % vw != 0 || addresses % (uint64_t)(vw * elem) != 0)) vw >>= 1;
-    return vw;
-}
 
 }  // namespace nrf
