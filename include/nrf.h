@@ -387,8 +387,9 @@ int nrf_lookup_fwd(const void *table, int64_t table_stride, int32_t dtype, int64
 
 /* grad [n_rows, dim] (dtype: the table's type) = scale * sum over the i with ids[i] == row of g_out[i]; every row is written,
  * rows that no id names with zeros.  g_out: row i at g_out + i * g_stride elements, of the table's type or f32.  Ids outside
- * the table and `padding_idx` (-1: none) take no part.  n_rows * dim < 2^33.  Sums in f32, in an order that depends on the ids and sizes alone:
- * repeated calls agree bit for bit.  workspace: nrf_lookup_bwd_workspace_bytes (-1: unsupported), 16-byte aligned. */
+ * the table and `padding_idx` (-1: none) take no part.  n_rows * dim < 2^33.  Sums in f32, in an order that depends on
+ * the ids, sizes and types alone: repeated calls agree bit for bit.  workspace: nrf_lookup_bwd_workspace_bytes (0: may be NULL;
+ * -1: unsupported), 16-byte aligned. */
 int64_t nrf_lookup_bwd_workspace_bytes(int64_t n, int64_t n_rows, int32_t dim);
 int nrf_lookup_bwd(const void *g_out, int64_t g_stride, int32_t g_dtype, const void *ids, int32_t ids_are_64, int64_t n,
                    int64_t n_rows, int32_t dim, float scale, int64_t padding_idx, void *grad, int32_t dtype, void *workspace,

@@ -1197,9 +1197,9 @@ struct RowWork {
 struct Part {
     int begin, end;
 };
-__device__ __forceinline__ Part part_of(int size, int part) {
-    const int each = ((size + kParts - 1) / kParts + 15) / 16 * 16;
-    return Part{min(size, part * each), min(size, (part + 1) * each)};
+__device__ __forceinline__ Part part_of(int size, int part, int parts) {
+    const int each = ((size + parts - 1) / parts + 15) / 16 * 16;
+    return Part{(int)min((int64_t)size, (int64_t)part * each), (int)min((int64_t)size, (int64_t)(part + 1) * each)};
 }
 
 __device__ __forceinline__ RowState state_of(const SampleArgs &a, int r, const RowWork &w, const double *tab) {
@@ -1265,7 +1265,7 @@ __global__ void __launch_bounds__(1024) sample_max_kernel(const SampleArgs a, Ro
     const int tid = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
     RowWork &w = work[r];
     const RowIO<T> io(a, r);
-    const Part p = part_of(a.size, part);
+    const Part p = part_of(a.size, part, kParts);
     float top = -__builtin_inff(), low = __builtin_inff();
     for_each<BLOCK>(io.row, p.begin, p.end, [&](float x, int, int) { top = fmaxf(top, x), low = fminf(low, x); });
     constexpr int kEach = kGroups / kParts, kOf = BLOCK / kEach;       // groups of a part, threads of a group
@@ -1320,7 +1320,7 @@ __global__ void __launch_bounds__(1024) sample_groups_kernel(const SampleArgs a,
     __syncthreads();
     Above above{0, 0};
     const int bin = find_bin<BLOCK>(s, h, true, false, o.f.k, 0.0, above);
-    const Part p = part_of(a.size, blockIdx.x);
+    const Part p = part_of(a.size, blockIdx.x, gridDim.x);
     if (bin < kBins) gather_part<BLOCK, T>(s, o, io.row, p, Reach(o, bin), w.list, &w.count[0]);
     if (!last_to_arrive(s, &w.arrived[0])) return;
     const uint32_t n = load_list<BLOCK>(s, w.list, &w.count[0]);
@@ -1346,7 +1346,7 @@ __global__ void __launch_bounds__(1024) sample_bins_kernel(const SampleArgs a, R
     if (o.plain() || !o.f.cut) return;
     clear_histogram<BLOCK>(h);
     const RowIO<T> io(a, r);
-    const Part p = part_of(a.size, blockIdx.x);
+    const Part p = part_of(a.size, blockIdx.x, gridDim.x);
     add_to_histogram<BLOCK, T>(h, o, io.row, p.begin, p.end, o.use_p);
     __syncthreads();
     for (int b = tid; b < kBins; b += BLOCK) {
@@ -1370,7 +1370,7 @@ __global__ void __launch_bounds__(1024) sample_cut_kernel(const SampleArgs a, Ro
     for (int b = tid; b < kBins; b += BLOCK) h.cnt[b] = w.h.cnt[b], h.mass[b] = w.h.mass[b];
     __syncthreads();
     const RowIO<T> io(a, r);
-    const Part p = part_of(a.size, blockIdx.x);
+    const Part p = part_of(a.size, blockIdx.x, gridDim.x);
     const Step st = first_step<BLOCK>(s, h, o);
     if (st.any && st.fits) gather_part<BLOCK, T>(s, o, io.row, p, Reach(st.from, st.bin), w.list, &w.count[1]);
     if (!last_to_arrive(s, &w.arrived[1])) return;
@@ -1482,8 +1482,10 @@ void launch_sample(const SampleArgs &a, bool may_k, bool may_p, RowWork *work, h
         if (may_k) sample_groups_kernel<T><<<parts, 1024, 0, s>>>(a, work, alone);
         if (alone) return;
         if (may_k || may_p) {
-            sample_bins_kernel<T><<<parts, 1024, 0, s>>>(a, work);
-            sample_cut_kernel<T><<<parts, 1024, 0, s>>>(a, work);
+            // 4096 draws from one row of 640000 by top-p: 51.1 us with 32 blocks a row, 47.4 with 64, 48.8 with 128
+            const dim3 more(std::clamp(128 / a.rows, kParts, 64), a.rows);
+            sample_bins_kernel<T><<<more, 1024, 0, s>>>(a, work);
+            sample_cut_kernel<T><<<more, 1024, 0, s>>>(a, work);
         }
         int tile = 1024;
         while ((a.size + tile - 1) / tile > kMaxTiles) tile <<= 1;

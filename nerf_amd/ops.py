@@ -206,7 +206,7 @@ def sample_logits(logits, n_samples, temperature=1.0, top_k=0, top_p=1.0, min_p=
     dev, lead, V, n = logits.device, logits.shape[:-1], logits.shape[-1], int(n_samples)
     if n < 0:
         raise ValueError(f"n_samples: {n}")
-    x = logits.reshape(-1, V)
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
     if V > 1 and x.stride(1) != 1:
         x = x.contiguous()
     R = x.shape[0]
@@ -217,7 +217,7 @@ def sample_logits(logits, n_samples, temperature=1.0, top_k=0, top_p=1.0, min_p=
             raise RuntimeError(f"u: expected a tensor on {dev}, got {u.device}")
         if u.shape != (*lead, n):
             raise ValueError(f"u: expected {(*lead, n)}, got {tuple(u.shape)}")
-        u = u.float().contiguous()
+        u = (u if u.dtype == torch.float32 else u.float()).contiguous()
     t, tv = _per_row(temperature, "temperature", torch.float32, lead, dev)
     k, kv = _per_row(top_k, "top_k", torch.int32, lead, dev)
     p, pv = _per_row(top_p, "top_p", torch.float32, lead, dev)
@@ -299,7 +299,7 @@ def lookup_bwd(g_out, ids, n_rows, scale=1.0, padding_idx=None, dtype=None):
     pad = -1 if padding_idx is None else int(padding_idx)
     if padding_idx is not None and not 0 <= pad < V:
         raise ValueError(f"padding_idx {pad} is outside the table's {V} rows")
-    g, stride = _rows(g_out.reshape(n, D))
+    g, stride = _rows(g_out if g_out.dim() == 2 else g_out.reshape(n, D))
     nbytes = _lib.lib().nrf_lookup_bwd_workspace_bytes(n, V, D)
     if nbytes < 0:
         raise RuntimeError("nrf_lookup_bwd_workspace_bytes: " + _lib.lib().nrf_last_error_string().decode())

@@ -91,7 +91,7 @@ def test_filters(kind, R, V):
 
 @pytest.mark.parametrize("kind", ["normal", "errors", "flat", "two", "masked", "outlier", "narrow"])
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("R,V,n", [(1, 131072, 1), (2, 100003, 40), (18, 65537, 3), (200, 4099, 2), (3, 2500, 300)])
+@pytest.mark.parametrize("R,V,n", [(1, 131072, 1), (2, 100003, 40), (18, 65537, 3), (200, 4099, 2), (3, 2500, 300), (70, 30000, 20)])
 def test_long_rows(kind, dtype, R, V, n):
     rng = np.random.RandomState(V + n)
     x = make(kind, R, V, rng)
@@ -103,11 +103,12 @@ def test_long_rows(kind, dtype, R, V, n):
         check(x, u, **f)
 
 
-def test_an_error_map_and_many_draws():
+@pytest.mark.parametrize("R,V,n", [(1, 640000, 4096), (20, 40000, 300)])
+def test_an_error_map_and_many_draws(R, V, n):
     rng = np.random.RandomState(1)
-    x = make("errors", 1, 640000, rng).cuda()
-    u = torch.from_numpy(rng.rand(1, 4096).astype(np.float32)).cuda()
-    for f in (dict(t=0.5, p=0.95), dict(), dict(m=0.01)):
+    x = make("errors", R, V, rng).cuda()
+    u = torch.from_numpy(rng.rand(R, n).astype(np.float32)).cuda()
+    for f in (dict(t=0.5, p=0.95), dict(), dict(m=0.01), dict(k=V // 3)):
         check(x, u, **f)
 
 
