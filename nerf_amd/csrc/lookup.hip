@@ -2,7 +2,7 @@
 //
 // Forward: every output element is one load, one product, one store; HBM-bound.  The output is cut into chunks of up to 16
 // bytes, consecutive lanes on consecutive chunks, so narrow rows (two features) and wide ones take the same path.  16384 rows of
-// 4096 bf16: 37 us (134 MB written, repeated rows read once); 2^21 rows of two f32 from 524288: 17.8 us, a cache line a row.
+// 4096 bf16: 34 us (134 MB written, repeated rows read once); 2^21 rows of two f32 from 524288: 17.5 us, a cache line a row.
 //
 // Gradient: the sum over equal ids is taken in a fixed order (no float atomics: results repeat bit for bit).
 //   1. a stable sort of the pairs (id, position): least significant digit first, digits of up to 10 bits.  The blocks of the
@@ -11,10 +11,10 @@
 //      tokens' rows and adds runs of equal ids in f32 registers.  A run inside the tile goes straight to its row of grad; one
 //      that reaches beyond an end of it leaves a partial sum (at most two per tile).
 //   3. the team whose tile a crossing run starts in adds up the run's partial sums.
-// Few tokens go without the sort, narrow rows of g travel with their ids instead of being gathered: below.
+// Few rows and up to 16384 tokens go without the sort, narrow rows of g travel with their ids instead of being gathered: below.
 // Any distribution of ids costs the same in 2, and a run of n tokens costs n / T partial sums in 3.  16384 rows of 4096 bf16 into
-// 131072: 231 us, 154 of them the zeros (7.0 TB/s), 70 the sums; 786432 rows of 33 f32 into 200: 69 us, of which 37 are 2 (2.8 TB/s:
-// 4-byte loads, a batch of pairs and rows at a time) and 22 the sort.
+// 131072: 231 us, 154 of them the zeros (7.0 TB/s), 70 the sums; 786432 rows of 33 f32 into 200: 55 us, of which 21 to 26 are 2 (4 to
+// 5 TB/s) and 22 the sort.
 #include "nrf_types.h"
 
 using namespace nrf;

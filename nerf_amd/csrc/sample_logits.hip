@@ -20,9 +20,9 @@
 // masses of the row's tiles of 1024 entries.
 //
 // Three forms: short rows without a cut, a wave each (4096 rows of 1001 f32: 11 us); one block a row (256 rows of 131072 bf16, top-k
-// about 1000 and top-p: 45 us, instructions: two passes of some four a logit; top-p alone 117 us, an f64 exponential a logit); and,
-// for few long rows, 32 blocks a row over several launches (4096 draws from 640000 f32, top-p: 54 us in five; one of 131072 by top-k: 17 us
-// in two), where the block that arrives last at a stage's end does what needs the whole row.
+// about 1000 and top-p: 40 us, instructions: two passes of some four a logit; top-p alone 117 us, an f64 exponential a logit); and,
+// for few long rows, 32 or 64 blocks a row over several launches (4096 draws from 640000 f32, top-p: 47 us in five; one of 131072 by
+// top-k: 17.6 us in two), where the block that arrives last at a stage's end does what needs the whole row.
 #include <algorithm>
 #include "nrf_types.h"
 
