@@ -54,10 +54,10 @@ def test_nothing_to_do_launches_nothing():
 
 def test_workspace_sizes():
     f = _lib.lib().nrf_lookup_bwd_workspace_bytes
-    assert f(0, 10, 4) >= 0 and f(4096, 5000, 32) == 0         # few tokens: no sort, no workspace
+    assert f(0, 10, 4) >= 0 and f(4096, 5000, 32) == f(16384, 5000, 32) == 0         # up to 16384 tokens: no sort, no workspace
     assert f(-1, 10, 4) == -1 and f(10, 10, 0) == -1 and f(10, 10, 32769) == -1 and f(2 ** 31, 10, 1) == -1
     # pairs of (id, position), twice for more than one pass, and two partial sums a tile: within a small multiple of the input
-    for n, rows, dim in ((9000, 5000, 32), (786432, 200, 33), (2097152, 524288, 2), (16384, 131072, 4096)):
+    for n, rows, dim in ((17000, 5000, 32), (9000, 50000, 300), (786432, 200, 33), (2097152, 524288, 2), (16384, 131072, 4096)):
         assert n * 8 <= f(n, rows, dim) <= n * 24 + n * dim * 4 + (1 << 24)
 
 
