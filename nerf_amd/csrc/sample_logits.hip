@@ -22,7 +22,7 @@
 // Three forms: short rows without a cut, a wave each (4096 rows of 1001 f32: 11 us); one block a row (256 rows of 131072 bf16, top-k
 // about 1000 and top-p: 40 us, instructions: two passes of some four a logit; top-p alone 117 us, an f64 exponential a logit); and,
 // for few long rows, 32 or 64 blocks a row over several launches (4096 draws from 640000 f32, top-p: 47 us in five; one of 131072 by
-// top-k: 17.6 us in two), where the block that arrives last at a stage's end does what needs the whole row.
+// top-k: 16 us in two), where the block that arrives last at a stage's end does what needs the whole row.
 #include <algorithm>
 #include "nrf_types.h"
 
@@ -766,7 +766,28 @@ __device__ __forceinline__ double mass_or_zero(const RowState &o, uint32_t key) 
     return e >= o.f.m ? e : 0.0;
 }
 
-// From the list: kept entries 0 .. n by index as (index, key); a thread a draw.
+// From the list, kept entries 0 .. n by index as (index, key), and their running masses: draws first, first + step ...
+template <int BLOCK>
+__device__ __forceinline__ void draw_by_search(Shared<BLOCK> &s, const RowState &o, int n, double total, const float *u, int draws, int64_t *ids,
+                                               float *prob, int first, int step) {
+    for (int j = first; j < draws; j += step) {
+        const float uj = u[j];
+        const double want = (double)fminf(fmaxf(uj, 0.0f), 1.0f) * total;
+        int a = 0, b = n - 1;                          // first entry whose running mass exceeds `want`
+        while (a < b) {
+            const int mid = (a + b) >> 1;
+            if (s.mass[mid] > want) b = mid;
+            else a = mid + 1;
+        }
+        // u = 1, or a product that rounds up to the total: back to the last entry that has mass
+        while (a > 0 && mass_or_zero(o, (uint32_t)s.list[a]) == 0.0) --a;
+        const double m = mass_or_zero(o, (uint32_t)s.list[a]);
+        ids[j] = uj == uj ? (int64_t)(s.list[a] >> 32) : -1;
+        prob[j] = uj == uj ? (float)(m / total) : 0.0f;
+    }
+}
+
+// The kept entries' running masses, then a thread a draw.
 template <int BLOCK>
 __device__ __forceinline__ void draw_from_list(Shared<BLOCK> &s, const RowState &o, int n, const float *u, int draws, int64_t *ids, float *prob) {
     constexpr int kPer = kList / BLOCK;
@@ -785,21 +806,7 @@ __device__ __forceinline__ void draw_from_list(Shared<BLOCK> &s, const RowState 
     }
     __syncthreads();
     total = s.mass[n - 1];
-    for (int j = tid; j < draws; j += BLOCK) {
-        const float uj = u[j];
-        const double want = (double)fminf(fmaxf(uj, 0.0f), 1.0f) * total;
-        int a = 0, b = n - 1;                          // first entry whose running mass exceeds `want`
-        while (a < b) {
-            const int mid = (a + b) >> 1;
-            if (s.mass[mid] > want) b = mid;
-            else a = mid + 1;
-        }
-        // u = 1, or a product that rounds up to the total: back to the last entry that has mass
-        while (a > 0 && mass_or_zero(o, (uint32_t)s.list[a]) == 0.0) --a;
-        const double m = mass_or_zero(o, (uint32_t)s.list[a]);
-        ids[j] = uj == uj ? (int64_t)(s.list[a] >> 32) : -1;
-        prob[j] = uj == uj ? (float)(m / total) : 0.0f;
-    }
+    draw_by_search(s, o, n, total, u, draws, ids, prob, tid, BLOCK);
 }
 
 // Tiles of a row: 1024 entries, or a multiple of them where a row has more than kMaxTiles; 16 consecutive entries a lane.
@@ -921,9 +928,88 @@ __device__ __forceinline__ void draw_plain(const RowState &o, int at, const floa
     }
 }
 
+// LDS written by lanes of this wave before, read by others behind (a wave's LDS accesses are in order; this holds the compiler to it)
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// n <= 64 P entries of the list into rising order, by one wave: each counts the smaller ones; c: entries P * lane + j
+template <int P>
+__device__ __forceinline__ void wave_sort(uint64_t *list, int n, uint64_t *c) {
+    const int i0 = (threadIdx.x & 63) * P;
+    uint32_t rank[P] = {};
+#pragma unroll 16
+    for (int q = 0; q < n; ++q) {
+        const uint64_t v = list[q];
+#pragma unroll
+        for (int j = 0; j < P; ++j) rank[j] += v < c[j];
+    }
+    wave_sync();
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+        if (i0 + j < n) list[rank[j]] = c[j];
+    wave_sync();
+#pragma unroll
+    for (int j = 0; j < P; ++j) c[j] = list[min(i0 + j, n - 1)];
+}
+
+// draw_top_k by one wave, for a list of at most 64 P entries and few draws: no barriers.  One row of 131072, top-k 50: 15.8 us a
+// call against 18.0 by the block's steps, 256 rows of 32768 11.7 against 14.0; lists of 200 with four entries a lane 23.6 against 21.6.
+template <int P, int BLOCK>
+__device__ __forceinline__ void draw_few(Shared<BLOCK> &s, const RowState &o, int n, const float *u, int draws, int64_t *ids, float *prob) {
+    const int lane = threadIdx.x & 63, i0 = lane * P, last = min(o.f.k, n);
+    uint64_t c[P], e[P], run = 0, at_last = 0;
+#pragma unroll
+    for (int j = 0; j < P; ++j) c[j] = s.list[min(i0 + j, n - 1)];
+    wave_sort<P>(s.list, n, c);
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        e[j] = i0 + j < n ? fixed(mass_of(o.w, value_of(~(uint32_t)(c[j] >> 32))), o.shift) : 0;
+        run += e[j];
+        if (i0 + j == last - 1) at_last = run;
+    }
+    uint64_t before = wave_scan<unsigned long long>(run) - run;
+    const double want = o.f.p * (double)__shfl((unsigned long long)(before + at_last), (last - 1) / P);
+    uint32_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        if (i0 + j < last && (!o.use_p || (double)before < want || i0 + j == 0)) ++mine;
+        before += e[j];
+    }
+    const int kept = (int)__builtin_amdgcn_readlane(wave_scan(mine), 63);
+    wave_sync();
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        c[j] = (c[j] << 32) | (uint32_t)~(uint32_t)(c[j] >> 32);
+        if (i0 + j < kept) s.list[i0 + j] = c[j];
+    }
+    wave_sync();
+    wave_sort<P>(s.list, kept, c);
+    double m[P], sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        m[j] = i0 + j < kept ? mass_or_zero(o, (uint32_t)c[j]) : 0.0;
+        sum += m[j];
+    }
+    double cum = wave_scan(sum) - sum;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        cum += m[j];
+        if (i0 + j < kept) s.mass[i0 + j] = cum;
+    }
+    wave_sync();
+    draw_by_search(s, o, kept, s.mass[kept - 1], u, draws, ids, prob, lane, 64);
+}
+
 // The list holds all that top-k can keep (values down to `low`): both cuts and the draws from it.
 template <int BLOCK>
 __device__ __forceinline__ void draw_top_k(Shared<BLOCK> &s, RowState &o, int n, float low, int size, const float *u, int draws, int64_t *ids, float *prob) {
+    if (n <= 128 && draws <= 64) {
+        if (threadIdx.x < 64) draw_few<2>(s, o, n, u, draws, ids, prob);
+        return;
+    }
     uint64_t mass_at;
     sort_by_value<BLOCK>(s, n, o.w.topf, fminf((float)kBins / (o.w.topf - low), 1e30f));
     const int kept = cut_list<BLOCK>(s, o, o.f, n, Above{0, 0}, min(o.f.k, n), o.use_p, o.f.p, 0.0, &mass_at);
