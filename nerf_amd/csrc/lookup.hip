@@ -695,7 +695,8 @@ struct Ranges {                // a row is high bits, block (`bits`), place in a
 };
 
 template <typename G, typename T, int VW, int ITEMS>
-__global__ void __launch_bounds__(1024, ITEMS > kTileItems ? 4 : 8) sum_ranges_kernel(const SumArgs a, const void *__restrict__ ids, int wide, int64_t padding, const Ranges w) {
+__global__ void __launch_bounds__(1024, ITEMS > kTileItems ? 4 : 8) sum_ranges_kernel(const SumArgs a, const void *__restrict__ ids,
+                                                                                        int wide, int64_t padding, const Ranges w) {
     __shared__ uint32_t list[1024 * ITEMS];                // row in the range << 14 | position; then positions by row
     __shared__ union {
         uint16_t cnt[16][1 << kMaxLow];

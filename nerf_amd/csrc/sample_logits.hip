@@ -1147,37 +1147,36 @@ __global__ void __launch_bounds__(1024) sample_row_kernel(const SampleArgs a) {
             if (group[u] > -__builtin_inff()) atomicAdd(&h.cnt[bin_of(o.w, o.scale, group[u])], 1u);
         __syncthreads();
         Above above{0, 0};
-        const int bin = find_bin<BLOCK>(s, h, true, false, o.f.k, 0.0, above);
-        if (bin < kBins) {
-            const Reach want(o, bin);
-            uint32_t n;
-            if constexpr (HELD > 0) {
-                uint32_t mask[HELD / 4], hits = 0;
+        // where fewer than k groups hold anything: all entries, if they fit
+        const int bin = min(find_bin<BLOCK>(s, h, true, false, o.f.k, 0.0, above), kBins - 1);
+        const Reach want(o, bin);
+        uint32_t n;
+        if constexpr (HELD > 0) {
+            uint32_t mask[HELD / 4], hits = 0;
 #pragma unroll
-                for (int u = 0; u < HELD; u += 4) {
-                    mask[u / 4] = 0;
-                    if (u * BLOCK < pieces) {
-                        Vec<T> p[4];
+            for (int u = 0; u < HELD; u += 4) {
+                mask[u / 4] = 0;
+                if (u * BLOCK < pieces) {
+                    Vec<T> p[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            // opaque: else the widened values of the first pass would be kept, in twice the registers
-                            asm volatile("" : "+v"(held[u + k]));
-                            p[k] = __builtin_bit_cast(Vec<T>, held[u + k]);
-                        }
-                        mask[u / 4] = reach_mask<BLOCK, T>(o, p, u * BLOCK + tid, pieces, want);
-                        hits += __popc(mask[u / 4]);
+                    for (int k = 0; k < 4; ++k) {
+                        // opaque: else the widened values of the first pass would be kept, in twice the registers
+                        asm volatile("" : "+v"(held[u + k]));
+                        p[k] = __builtin_bit_cast(Vec<T>, held[u + k]);
                     }
+                    mask[u / 4] = reach_mask<BLOCK, T>(o, p, u * BLOCK + tid, pieces, want);
+                    hits += __popc(mask[u / 4]);
                 }
-                uint32_t at = reserve(&s.count, hits);
-#pragma unroll
-                for (int u = 0; u < HELD; u += 4)
-                    at = put_mask<BLOCK, T>(reinterpret_cast<uint32_t *>(s.mass), mask[u / 4], at, u * BLOCK + tid, 0);
-                n = finish_list<BLOCK, T>(s, o, io.row, pieces * E + tid, size, want);
-            } else {
-                n = gather<BLOCK, T>(s, o, io.row, 0, size, want);
             }
-            if (n <= (uint32_t)kList) return draw_top_k<BLOCK>(s, o, n, o.w.topf - (float)(bin + 1) / o.scale, size, io.u, a.draws, io.ids, io.prob);
+            uint32_t at = reserve(&s.count, hits);
+#pragma unroll
+            for (int u = 0; u < HELD; u += 4)
+                at = put_mask<BLOCK, T>(reinterpret_cast<uint32_t *>(s.mass), mask[u / 4], at, u * BLOCK + tid, 0);
+            n = finish_list<BLOCK, T>(s, o, io.row, pieces * E + tid, size, want);
+        } else {
+            n = gather<BLOCK, T>(s, o, io.row, 0, size, want);
         }
+        if (n <= (uint32_t)kList) return draw_top_k<BLOCK>(s, o, n, o.w.topf - (float)(bin + 1) / o.scale, size, io.u, a.draws, io.ids, io.prob);
     }
     draw_long_row<BLOCK, T>(s, h, tiles, o, io, a);
 }
@@ -1405,12 +1404,12 @@ __global__ void __launch_bounds__(1024) sample_groups_kernel(const SampleArgs a,
     }
     __syncthreads();
     Above above{0, 0};
-    const int bin = find_bin<BLOCK>(s, h, true, false, o.f.k, 0.0, above);
+    const int bin = min(find_bin<BLOCK>(s, h, true, false, o.f.k, 0.0, above), kBins - 1);
     const Part p = part_of(a.size, blockIdx.x, gridDim.x);
-    if (bin < kBins) gather_part<BLOCK, T>(s, o, io.row, p, Reach(o, bin), w.list, &w.count[0]);
+    gather_part<BLOCK, T>(s, o, io.row, p, Reach(o, bin), w.list, &w.count[0]);
     if (!last_to_arrive(s, &w.arrived[0])) return;
     const uint32_t n = load_list<BLOCK>(s, w.list, &w.count[0]);
-    if (bin < kBins && n <= (uint32_t)kList) {
+    if (n <= (uint32_t)kList) {
         draw_top_k<BLOCK>(s, o, n, o.w.topf - (float)(bin + 1) / o.scale, a.size, io.u, a.draws, io.ids, io.prob);
         if (tid == 0) w.done = 1;
     } else if (alone) {

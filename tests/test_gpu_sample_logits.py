@@ -91,7 +91,7 @@ def test_filters(kind, R, V):
 
 @pytest.mark.parametrize("kind", ["normal", "errors", "flat", "two", "masked", "outlier", "narrow"])
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("R,V,n", [(1, 131072, 1), (2, 100003, 40), (18, 65537, 3), (200, 4099, 2), (3, 2500, 300), (70, 30000, 20)])
+@pytest.mark.parametrize("R,V,n", [(1, 131072, 1), (2, 100003, 40), (18, 65537, 3), (200, 4099, 2), (3, 2500, 300), (70, 30000, 20), (3, 65536, 2), (6, 131072, 1)])
 def test_long_rows(kind, dtype, R, V, n):
     rng = np.random.RandomState(V + n)
     x = make(kind, R, V, rng)
@@ -110,6 +110,19 @@ def test_an_error_map_and_many_draws(R, V, n):
     u = torch.from_numpy(rng.rand(R, n).astype(np.float32)).cuda()
     for f in (dict(t=0.5, p=0.95), dict(), dict(m=0.01), dict(k=V // 3)):
         check(x, u, **f)
+
+
+def test_top_k_of_rows_that_hold_fewer():
+    """Masks that leave fewer entries than k: none, one, fewer and more than the list; both forms of long rows."""
+    rng = np.random.RandomState(6)
+    for V, rows in ((16550, 7), (140000, 3), (140000, 7)):
+        x = rng.normal(size=(rows, V)).astype(np.float32) * 2.5
+        for r, left in enumerate((1, 0, 300, 1200, 2048, 2049, 5000)[:rows]):
+            x[r, rng.permutation(V)[left:]] = -np.inf
+        for k, n in ((536, 70), (1500, 3), (1400, 1)):
+            u = torch.from_numpy(rng.rand(rows, n).astype(np.float32)).cuda()
+            check(torch.from_numpy(x).cuda(), u, k=k, t=0.7)
+            check(torch.from_numpy(x).cuda().half(), u, k=k, p=0.9)
 
 
 def test_filters_of_each_row():
