@@ -138,6 +138,7 @@ template <int BLOCK> struct Shared {
     double wave_d[kWaves];
     uint64_t wave_u[kWaves];
     uint32_t wave_a[kWaves];
+    int32_t wave_last[kWaves];
     uint32_t count;                    // entries in `list`
     uint64_t found[3];                 // what one thread found for all
     uint32_t crowded, bucket[kBins];   // sort_list
@@ -171,6 +172,16 @@ __device__ __forceinline__ V wave_scan(V v) {
     v += dpp<0x118, 0xf>(v);      // row_shr:8
     v += dpp<0x142, 0xa>(v);      // row_bcast:15 into rows 1 and 3
     v += dpp<0x143, 0xc>(v);      // row_bcast:31 into rows 2 and 3
+    return v;
+}
+// Largest of the lanes up to this one, of values that are not negative (the same moves)
+__device__ __forceinline__ double wave_running_max(double v) {
+    v = fmax(v, dpp<0x111, 0xf>(v));
+    v = fmax(v, dpp<0x112, 0xf>(v));
+    v = fmax(v, dpp<0x114, 0xf>(v));
+    v = fmax(v, dpp<0x118, 0xf>(v));
+    v = fmax(v, dpp<0x142, 0xa>(v));
+    v = fmax(v, dpp<0x143, 0xc>(v));
     return v;
 }
 __device__ __forceinline__ double last_lane(double v) {
@@ -766,20 +777,26 @@ __device__ __forceinline__ double mass_or_zero(const RowState &o, uint32_t key) 
     return e >= o.f.m ? e : 0.0;
 }
 
+// What a running mass has to exceed.  u = 1, and what is clamped to it, lies behind all of them, whatever their roundings, and so names
+// the last entry with mass; below, u <= 1 - 2^-24 keeps far from the total.
+__device__ __forceinline__ double target(float u, double total) {
+    return u >= 1.0f ? __builtin_inf() : (double)fmaxf(u, 0.0f) * total;
+}
+
 // From the list, kept entries 0 .. n by index as (index, key), and their running masses: draws first, first + step ...
 template <int BLOCK>
 __device__ __forceinline__ void draw_by_search(Shared<BLOCK> &s, const RowState &o, int n, double total, const float *u, int draws, int64_t *ids,
                                                float *prob, int first, int step) {
     for (int j = first; j < draws; j += step) {
         const float uj = u[j];
-        const double want = (double)fminf(fmaxf(uj, 0.0f), 1.0f) * total;
+        const double want = target(uj, total);
         int a = 0, b = n - 1;                          // first entry whose running mass exceeds `want`
         while (a < b) {
             const int mid = (a + b) >> 1;
             if (s.mass[mid] > want) b = mid;
             else a = mid + 1;
         }
-        // u = 1, or a product that rounds up to the total: back to the last entry that has mass
+        // back from the end of the list (u = 1), or from a running sum that an entry without mass rounds up
         while (a > 0 && mass_or_zero(o, (uint32_t)s.list[a]) == 0.0) --a;
         const double m = mass_or_zero(o, (uint32_t)s.list[a]);
         ids[j] = uj == uj ? (int64_t)(s.list[a] >> 32) : -1;
@@ -874,36 +891,55 @@ __device__ __forceinline__ bool pick_entry(const double *e, double sum, double c
     return over != 0;
 }
 
-// tiles[0 .. n) -> running sums; load(q): tile q
+// tiles[0 .. n) -> running sums; load(q): tile q.  Returns the last tile with mass.
+// The sums are added in another order from thread to thread, so those of neighbours may differ by a rounding either way where the tile
+// between them is empty.  A tile with mass gets the largest sum up to its own, an empty one exactly that of the last with mass before
+// it: the first tile whose running sum exceeds a number always has mass.
 template <int BLOCK, typename S, typename L>
-__device__ __forceinline__ void scan_tiles(S &s, double *tiles, int n, L load) {
+__device__ __forceinline__ int scan_tiles(S &s, double *tiles, int n, L load) {
     constexpr int kPer = kMaxTiles / BLOCK;
-    const int q0 = threadIdx.x * kPer;
+    const int q0 = threadIdx.x * kPer, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double v[kPer], run = 0.0, total;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) v[j] = q0 + j < n ? load(q0 + j) : 0.0, run += v[j];
-    double cum = block_scan<BLOCK, double>(run, s.wave_d, &total);
+    double cum = block_scan<BLOCK, double>(run, s.wave_d, &total), most = 0.0;
+    int last = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
         cum += v[j];
-        if (q0 + j < n) tiles[q0 + j] = cum;
+        if (v[j] > 0.0) most = fmax(most, cum), last = q0 + j;
+        v[j] = most;
     }
+    const uint64_t some = __ballot(most > 0.0);
+    last = some ? __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(some)) : 0;
+    most = wave_running_max(most);
+    if (lane == 63) s.wave_d[wave] = most, s.wave_last[wave] = last;
+    most = lane_before(most);
     __syncthreads();
+#pragma unroll
+    for (int w = 0; w < BLOCK / 64; ++w) {
+        if (w < wave) most = fmax(most, s.wave_d[w]);
+        last = max(last, s.wave_last[w]);
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+        if (q0 + j < n) tiles[q0 + j] = fmax(most, v[j]);
+    __syncthreads();
+    return last;
 }
 
 // One draw by a wave: the tile by its running sum, then the entry.
 template <typename T>
-__device__ __forceinline__ void draw_from_tiles(const RowState &o, const T *row, int size, int tile, const double *tiles, int n_tiles, float uj,
-                                int64_t *id, float *prob) {
+__device__ __forceinline__ void draw_from_tiles(const RowState &o, const T *row, int size, int tile, const double *tiles, int n_tiles, int last,
+                                float uj, int64_t *id, float *prob) {
     const int lane = threadIdx.x & 63;
-    const double total = tiles[n_tiles - 1], want = (double)fminf(fmaxf(uj, 0.0f), 1.0f) * total;
-    // the first tile whose running sum exceeds `want` (else the last one): 64 probes, 16 tiles apart, then 16
+    const double total = tiles[n_tiles - 1], want = target(uj, total);
+    // the first tile whose running sum exceeds `want` (u = 1: the last with mass): 64 probes, 16 tiles apart, then 16
     static_assert(kMaxTiles == 64 * 16, "two steps");
     const uint64_t far = __ballot(tiles[min(lane * 16 + 15, n_tiles - 1)] > want);
     const int from = (far ? __builtin_ctzll(far) : 63) * 16;
     const uint64_t near = __ballot(tiles[min(from + (lane & 15), n_tiles - 1)] > want);
-    int a = min(from + (near ? __builtin_ctzll(near) : 15), n_tiles - 1);
-    while (a > 0 && tiles[a] <= tiles[a - 1]) --a;       // u = 1: back to the last tile that has mass
+    const int a = near ? min(from + __builtin_ctzll(near), n_tiles - 1) : last;
     double before = a > 0 ? tiles[a - 1] : 0.0, mass = 0.0, e[16];
     int at = 0;
     const int end = min(size, (a + 1) * tile);
@@ -1026,8 +1062,8 @@ __device__ __forceinline__ void draw_whole_row(Shared<BLOCK> &s, double *tiles, 
         if ((tid & 63) == 0) tiles[q] = m;
     }
     __syncthreads();
-    scan_tiles<BLOCK>(s, tiles, n_tiles, [&](int q) { return tiles[q]; });
-    for (int j = tid >> 6; j < draws; j += BLOCK / 64) draw_from_tiles<T>(o, row, size, tile, tiles, n_tiles, u[j], ids + j, prob + j);
+    const int last = scan_tiles<BLOCK>(s, tiles, n_tiles, [&](int q) { return tiles[q]; });
+    for (int j = tid >> 6; j < draws; j += BLOCK / 64) draw_from_tiles<T>(o, row, size, tile, tiles, n_tiles, last, u[j], ids + j, prob + j);
 }
 
 // ---- one block a row
@@ -1246,7 +1282,7 @@ __global__ void __launch_bounds__(256) sample_wave_kernel(const SampleArgs a) {
     }
     for (int d = 0; d < a.draws; ++d) {
         if (d > 0) u = io.u[d];
-        const double want = (double)fminf(fmaxf(u, 0.0f), 1.0f) * total;
+        const double want = target(u, total);
         int at = 0;
         double mass = 0.0, before = 0.0;
         bool found = false;
@@ -1272,7 +1308,7 @@ struct RowWork {
     uint32_t arrived[3];
     uint32_t done;                         // the draws are out
     uint32_t cut, cut_key;
-    int32_t cut_idx, k;
+    int32_t cut_idx, last_tile;
     alignas(256) float group[kGroups];
     Histogram h;
     uint64_t list[kList];
@@ -1478,6 +1514,7 @@ __device__ __forceinline__ RowState cut_state(const SampleArgs &a, int r, const 
 // Stage 5: masses of the tiles, a wave each (64 rows of 524288: 41 us); by the last block their running sums.
 struct TileShared {
     double tab[16], wave_d[4];
+    int32_t wave_last[4];
     uint64_t found[1];
 };
 template <typename T>
@@ -1496,7 +1533,9 @@ __global__ void __launch_bounds__(256) sample_tiles_kernel(const SampleArgs a, R
         const double m = tile_mass<T>(o, io.row, a.size, tile, q);
         if ((tid & 63) == 0) publish(&w.tiles[q], m);
     }
-    if (last_to_arrive(s, &w.arrived[2])) scan_tiles<BLOCK>(s, w.tiles, n, [&](int q) { return fetch(&w.tiles[q]); });
+    if (!last_to_arrive(s, &w.arrived[2])) return;
+    const int last = scan_tiles<BLOCK>(s, w.tiles, n, [&](int q) { return fetch(&w.tiles[q]); });
+    if (tid == 0) w.last_tile = last;
 }
 
 // Stage 6: the draws, a wave each.
@@ -1518,7 +1557,7 @@ __global__ void __launch_bounds__(256) sample_draw_kernel(const SampleArgs a, co
     for (int q = tid; q < n; q += 256) tiles[q] = w.tiles[q];
     __syncthreads();
     for (int j = blockIdx.x * 4 + (tid >> 6); j < a.draws; j += gridDim.x * 4)
-        draw_from_tiles<T>(o, io.row, a.size, tile, tiles, n, io.u[j], io.ids + j, io.prob + j);
+        draw_from_tiles<T>(o, io.row, a.size, tile, tiles, n, w.last_tile, io.u[j], io.ids + j, io.prob + j);
 }
 
 // ---- host
