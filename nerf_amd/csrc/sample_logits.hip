@@ -174,16 +174,6 @@ __device__ __forceinline__ V wave_scan(V v) {
     v += dpp<0x143, 0xc>(v);      // row_bcast:31 into rows 2 and 3
     return v;
 }
-// Largest of the lanes up to this one, of values that are not negative (the same moves)
-__device__ __forceinline__ double wave_running_max(double v) {
-    v = fmax(v, dpp<0x111, 0xf>(v));
-    v = fmax(v, dpp<0x112, 0xf>(v));
-    v = fmax(v, dpp<0x114, 0xf>(v));
-    v = fmax(v, dpp<0x118, 0xf>(v));
-    v = fmax(v, dpp<0x142, 0xa>(v));
-    v = fmax(v, dpp<0x143, 0xc>(v));
-    return v;
-}
 __device__ __forceinline__ double last_lane(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)b, 63), hi = __builtin_amdgcn_readlane((uint32_t)(b >> 32), 63);
@@ -892,38 +882,28 @@ __device__ __forceinline__ bool pick_entry(const double *e, double sum, double c
 }
 
 // tiles[0 .. n) -> running sums; load(q): tile q.  Returns the last tile with mass.
-// The sums are added in another order from thread to thread, so those of neighbours may differ by a rounding either way where the tile
-// between them is empty.  A tile with mass gets the largest sum up to its own, an empty one exactly that of the last with mass before
-// it: the first tile whose running sum exceeds a number always has mass.
 template <int BLOCK, typename S, typename L>
 __device__ __forceinline__ int scan_tiles(S &s, double *tiles, int n, L load) {
     constexpr int kPer = kMaxTiles / BLOCK;
-    const int q0 = threadIdx.x * kPer, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int q0 = threadIdx.x * kPer;
     double v[kPer], run = 0.0, total;
+    int last = -1;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] = q0 + j < n ? load(q0 + j) : 0.0, run += v[j];
-    double cum = block_scan<BLOCK, double>(run, s.wave_d, &total), most = 0.0;
-    int last = 0;
+    for (int j = 0; j < kPer; ++j) {
+        v[j] = q0 + j < n ? load(q0 + j) : 0.0, run += v[j];
+        last = v[j] > 0.0 ? q0 + j : last;
+    }
+    const uint64_t some = __ballot(last >= 0);
+    last = some ? __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(some)) : 0;
+    if ((threadIdx.x & 63) == 0) s.wave_last[threadIdx.x >> 6] = last;
+    double cum = block_scan<BLOCK, double>(run, s.wave_d, &total);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
         cum += v[j];
-        if (v[j] > 0.0) most = fmax(most, cum), last = q0 + j;
-        v[j] = most;
-    }
-    const uint64_t some = __ballot(most > 0.0);
-    last = some ? __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(some)) : 0;
-    most = wave_running_max(most);
-    if (lane == 63) s.wave_d[wave] = most, s.wave_last[wave] = last;
-    most = lane_before(most);
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < BLOCK / 64; ++w) {
-        if (w < wave) most = fmax(most, s.wave_d[w]);
-        last = max(last, s.wave_last[w]);
+        if (q0 + j < n) tiles[q0 + j] = cum;
     }
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-        if (q0 + j < n) tiles[q0 + j] = fmax(most, v[j]);
+    for (int w = 0; w < BLOCK / 64; ++w) last = max(last, s.wave_last[w]);
     __syncthreads();
     return last;
 }
@@ -933,20 +913,27 @@ template <typename T>
 __device__ __forceinline__ void draw_from_tiles(const RowState &o, const T *row, int size, int tile, const double *tiles, int n_tiles, int last,
                                 float uj, int64_t *id, float *prob) {
     const int lane = threadIdx.x & 63;
-    const double total = tiles[n_tiles - 1], want = target(uj, total);
+    const double total = tiles[n_tiles - 1];
+    double want = target(uj, total);
     // the first tile whose running sum exceeds `want` (u = 1: the last with mass): 64 probes, 16 tiles apart, then 16
     static_assert(kMaxTiles == 64 * 16, "two steps");
     const uint64_t far = __ballot(tiles[min(lane * 16 + 15, n_tiles - 1)] > want);
     const int from = (far ? __builtin_ctzll(far) : 63) * 16;
     const uint64_t near = __ballot(tiles[min(from + (lane & 15), n_tiles - 1)] > want);
-    const int a = near ? min(from + __builtin_ctzll(near), n_tiles - 1) : last;
-    double before = a > 0 ? tiles[a - 1] : 0.0, mass = 0.0, e[16];
-    int at = 0;
-    const int end = min(size, (a + 1) * tile);
-    for (int base = a * tile; base < end; base += 1024) {
-        const double sum = lane_masses<T>(o, row, size, base, e), cum = wave_scan(sum);
-        if (pick_entry<16>(e, sum, cum, before, want, base, at, mass)) break;
-        before += __shfl(cum, 63);
+    int a = near ? min(from + __builtin_ctzll(near), n_tiles - 1) : last, at = 0;
+    double mass = 0.0, e[16];
+    // The sums are added in another order from thread to thread, so an empty tile's may lie a rounding above that of the tile before:
+    // where that much led to it, the draw is the last entry with mass before it.  (There is one: the sums of empty tiles are exactly 0 up to
+    // the first tile with mass.)
+    for (;; --a, want = __builtin_inf()) {
+        double before = a > 0 ? tiles[a - 1] : 0.0;
+        const int end = min(size, (a + 1) * tile);
+        for (int base = a * tile; base < end; base += 1024) {
+            const double sum = lane_masses<T>(o, row, size, base, e), cum = wave_scan(sum);
+            if (pick_entry<16>(e, sum, cum, before, want, base, at, mass)) break;
+            before += __shfl(cum, 63);
+        }
+        if (mass > 0.0 || a == 0) break;
     }
     if (lane == 0) {
         *id = uj == uj ? at : -1;
