@@ -12,10 +12,11 @@
 // The cut (the last kept entry, by value and index) is found among few entries:
 //   - top-k with k up to some 1500: the row is split into 4096 groups, and the k-th largest of the groups' maxima bounds the k-th
 //     largest entry from below.  The entries above that bound (a few more than k) go into a list in LDS.
-//   - else a histogram of the row, 2048 bins of equal width below the maximum, counts and masses.  Masses there are 64-bit
-//     fixed point (2^62 / V for e = 1), because integer atomics give the same sums in any order.  The bin of the cut, or all
-//     entries down to it, go into the list.  A bin that holds more than the list (many equal values, far outliers) is split again
-//     by the bits of its values until it does not, or holds one value only.
+//   - else a histogram of the row, 2048 bins of equal width below the maximum, counts and masses.  Masses are added there as 64-bit
+//     integers, because these give the same sums in any order, in units that go down with the bin's masses, and are f64 from then on:
+//     what a bin holds is right to 2^-41 of itself, however small it is.  The bin of the cut, or all entries down to it, go into the
+//     list.  A bin that holds more than the list (many equal values, far outliers) is split again by the bits of its values until it
+//     does not, or holds one value only.
 // The list (up to 2048 entries) is sorted.  Where it holds everything that is kept, the draws come from it; else from the
 // masses of the row's tiles of 1024 entries.
 //
@@ -32,6 +33,7 @@ namespace {
 
 constexpr int kBins = 2048, kList = 2048, kGroups = 4096, kMaxTiles = 1024;
 constexpr int kMaxSize = 1 << 28, kMaxRows = 1 << 21;
+constexpr int kSegment = 1 << 20;           // entries whose masses a word of the histogram holds
 constexpr int kParts = 32;                  // blocks of a row, many-block form
 constexpr int kCrowd = 160;                 // entries of a bucket from which sort_list falls back
 constexpr int kGroupsMaxK = 1500;           // above it the groups' bound lets more entries through than the list holds
@@ -75,10 +77,11 @@ struct Row {
 };
 
 // exp(y), y = (x - M) / T <= 0: y = (16 q + j) ln2 / 16 + r, |r| <= ln2 / 32, exp = 2^q tab[j] exp(r); the Taylor polynomial of
-// degree 6 leaves r^7 / 5040 < 5e-16.  x = M gives 1 exactly; -inf and NaN end in the clamp's 2^-1154, which is 0.
-__device__ __forceinline__ double mass_of(const Row &w, float x) {
-    if (w.flat) return x == w.topf ? 1.0 : 0.0;
-    const double y = fmax(((double)x - w.top) * w.inv_t, -800.0);
+// degree 6 leaves r^7 / 5040 < 5e-16.  x = M gives 1 exactly; -inf and NaN end in the clamp's 2^-4328, which is 0.  2^up (up to 2^2200)
+// times that, with the one rounding.
+__device__ __forceinline__ double mass_of(const Row &w, float x, int up = 0) {
+    if (w.flat) return x == w.topf ? __builtin_ldexp(1.0, up) : 0.0;
+    const double y = fmax(((double)x - w.top) * w.inv_t, -3000.0);
     const double n = __builtin_rint(y * (16.0 * 1.44269504088896340736));
     const double r = fma(n, -0.69314718055994530942 / 16.0, y);
     double s = fma(r, 1.0 / 720.0, 1.0 / 120.0);
@@ -88,7 +91,7 @@ __device__ __forceinline__ double mass_of(const Row &w, float x) {
     s = fma(r, s, 1.0);
     s = fma(r, s, 1.0);
     const int q = (int)n;
-    return __builtin_ldexp(s * w.tab[q & 15], q >> 4);
+    return __builtin_ldexp(s * w.tab[q & 15], (q >> 4) + up);
 }
 
 // Bin of the first histogram: equal widths below the maximum, the last bin open.  Every step is monotone in x.
@@ -141,13 +144,17 @@ template <int BLOCK> struct Shared {
     int32_t wave_last[kWaves];
     uint32_t count;                    // entries in `list`
     uint64_t found[3];                 // what one thread found for all
+    int32_t first, back;               // find_bin
     uint32_t crowded, bucket[kBins];   // sort_list
     uint64_t list[kList];
     double mass[kList];
 };
 struct Histogram {
     uint32_t cnt[kBins];
-    uint64_t mass[kBins];
+    union {
+        uint64_t word[kBins];          // while entries are added: fixed point, see `raise`
+        double mass[kBins];            // afterwards
+    };
 };
 
 // The value of the lane that DPP control CTRL names, 0 where there is none (4- and 8-byte types)
@@ -358,11 +365,8 @@ __device__ __forceinline__ double kept_mass(const Row &w, const Filter &f, float
 // What stands before a place in the order: entries and their mass.
 struct Above {
     uint32_t cnt;
-    uint64_t mass;
+    double mass;
 };
-
-// Fixed-point masses: e * 2^shift, the sum of a whole row stays below 2^63.
-__device__ __forceinline__ uint64_t fixed(double e, int shift) { return (uint64_t)__builtin_ldexp(e, shift); }
 
 // ---- a row's parameters
 struct RowState {
@@ -370,7 +374,8 @@ struct RowState {
     Filter f;
     bool valid, use_p;      // use_p: top-p leaves something out, if anything does
     float t, scale;         // scale: bins of the first histogram
-    int shift;
+    float lift;             // log2 of how much smaller a bin's masses are than those of the bin before
+    int shift;              // bits behind the point of a histogram's word, bin 0
     __device__ __forceinline__ bool plain() const { return !valid || t == 0.0f; }
 };
 
@@ -392,10 +397,21 @@ __device__ __forceinline__ RowState row_state(const SampleArgs &a, int r, float 
     o.f.key = 0, o.f.idx = a.size;
     // 64 temperatures reach masses of 1e-28; top-k, which does not look at masses, gets some room where they are narrow
     o.scale = fminf((float)kBins / fminf(top - low, fmaxf(64.0f * o.t, 16.0f)), 1e30f);
+    // (scale 0, or so small that bins end beyond f32's range, leaves bins without an order of mass: no lift)
+    o.lift = o.w.flat || o.scale == 0.0f ? 0.0f : fminf(1.44269504f / (o.scale * o.t), 1.0f);
     o.shift = 62;
-    for (int v = a.size; v > 0; v >>= 1) --o.shift;
+    for (int v = min(a.size, kSegment); v > 0; v >>= 1) --o.shift;
+    o.shift = min(o.shift, 50);
     return o;
 }
+
+// Masses of a histogram are added as 64-bit integers, which give the same sums in any order.  A bin's unit goes down with its masses:
+// the entries of bin b weigh at most 2^(-b lift) (but for some 1e-3 that f32 rounds into the bin), so e * 2^raise <= 2^shift * 1.001 and
+// the words of kSegment entries stay below 2^63.  An entry is held to half a unit, 2^-42 of its bin's largest at kSegment entries.
+__device__ __forceinline__ int raise(const RowState &o, int bin) { return o.shift + (int)((float)bin * o.lift); }
+// Nearest integer of 0 <= v < 2^52: the bits of 2^52 + v behind those of 2^52 (shift is at most 50: rows in a histogram have more than
+// 2048 entries)
+__device__ __forceinline__ uint64_t fixed(double v) { return __builtin_bit_cast(uint64_t, v + 0x1p52) - __builtin_bit_cast(uint64_t, 0x1p52); }
 
 // Lowest index in begin .. end that holds x (size where none does)
 template <int BLOCK, typename T>
@@ -412,22 +428,58 @@ __device__ __forceinline__ int find_value(Shared<BLOCK> &s, const T *row, int be
     return at;
 }
 
+template <int BLOCK>
+__device__ __forceinline__ void clear_histogram(Histogram &h) {
+    for (int b = threadIdx.x; b < kBins; b += BLOCK) h.cnt[b] = 0, h.word[b] = 0;
+    __syncthreads();
+}
+
 template <int BLOCK, typename T>
-__device__ __forceinline__ void add_to_histogram(Histogram &h, const RowState &o, const T *row, int begin, int end, bool masses) {
-    if (!masses) {
-        for_each<BLOCK>(row, begin, end, [&](float x, int, int) {
-            if (key_of(x)) atomicAdd(&h.cnt[bin_of(o.w, o.scale, x)], 1u);
-        });
-        return;
-    }
+__device__ __forceinline__ void add_counts(Histogram &h, const RowState &o, const T *row, int begin, int end) {
+    for_each<BLOCK>(row, begin, end, [&](float x, int, int) {
+        if (key_of(x)) atomicAdd(&h.cnt[bin_of(o.w, o.scale, x)], 1u);
+    });
+    __syncthreads();
+}
+
+// Counts and words of begin .. end, at most kSegment entries.  bin(x, key): below 0 for entries of no bin; up(b): the unit of bin b
+template <int BLOCK, typename T, typename B, typename X>
+__device__ __forceinline__ void add_words(Histogram &h, const RowState &o, const T *row, int begin, int end, B bin, X up) {
     for_each<BLOCK, 1>(row, begin, end, [&](float x, int, int) {
         const uint32_t key = key_of(x);
-        if (key) {
-            const int b = bin_of(o.w, o.scale, x);
+        const int b = bin(x, key);
+        if (b >= 0) {
             atomicAdd(&h.cnt[b], 1u);
-            atomicAdd((unsigned long long *)&h.mass[b], (unsigned long long)fixed(mass_of(o.w, x), o.shift));
+            atomicAdd((unsigned long long *)&h.word[b], (unsigned long long)fixed(mass_of(o.w, x, up(b))));
         }
     });
+    __syncthreads();
+}
+
+// Counts and masses of a whole row; a thread adds up its bins' words behind each segment.
+template <int BLOCK, typename T, typename B, typename X>
+__device__ __forceinline__ void fill_histogram(Histogram &h, const RowState &o, const T *row, int size, B bin, X up) {
+    constexpr int kPer = kBins / BLOCK;
+    double sum[kPer] = {};
+    clear_histogram<BLOCK>(h);
+    for (int begin = 0; begin < size; begin += kSegment) {
+        add_words<BLOCK, T>(h, o, row, begin, min(size, begin + kSegment), bin, up);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int b = j * BLOCK + threadIdx.x;
+            sum[j] += __builtin_ldexp((double)h.word[b], -up(b));
+            h.word[b] = 0;
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) h.mass[j * BLOCK + threadIdx.x] = sum[j];
+    __syncthreads();
+}
+template <int BLOCK, typename T>
+__device__ __forceinline__ void fill_histogram(Histogram &h, const RowState &o, const T *row, int size) {
+    fill_histogram<BLOCK, T>(h, o, row, size, [&](float x, uint32_t key) { return key ? bin_of(o.w, o.scale, x) : -1; },
+                             [&](int b) { return raise(o, b); });
 }
 
 // ---- the cut
@@ -435,34 +487,33 @@ __device__ __forceinline__ void add_to_histogram(Histogram &h, const RowState &o
 // than `want` of mass before them (by_mass).  Returns how many entries of the list that keeps; mass_at: mass up to entry `last`.
 template <int BLOCK>
 __device__ __forceinline__ int cut_list(Shared<BLOCK> &s, const RowState &o, Filter &f, int n, Above above, int last, bool by_mass, double p,
-                        double want, uint64_t *mass_at) {
+                        double want, double *mass_at) {
     constexpr int kPer = kList / BLOCK;
-    uint64_t e[kPer], run = 0;
+    double e[kPer], run = 0.0, all;
     const int i0 = threadIdx.x * kPer;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-        e[j] = i0 + j < n ? fixed(mass_of(o.w, value_of(~(uint32_t)(s.list[i0 + j] >> 32))), o.shift) : 0;
+        e[j] = i0 + j < n ? mass_of(o.w, value_of(~(uint32_t)(s.list[i0 + j] >> 32))) : 0.0;
         run += e[j];
     }
-    unsigned long long all;
-    uint64_t before = above.mass + block_scan<BLOCK, unsigned long long>(run, (unsigned long long *)s.wave_u, &all);
+    double before = above.mass + block_scan<BLOCK, double>(run, s.wave_d, &all);
     if (last <= n) {
-        uint64_t b = before;
+        double b = before;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
             b += e[j];
-            if (i0 + j == last - 1) s.found[0] = b;
+            if (i0 + j == last - 1) s.found[0] = __builtin_bit_cast(uint64_t, b);
         }
         __syncthreads();
-        *mass_at = uniform(s.found[0]);
+        *mass_at = __builtin_bit_cast(double, uniform(s.found[0]));
         __syncthreads();
-        if (p >= 0.0) want = p * (double)*mass_at;                     // top-p of the mass found here
+        if (p >= 0.0) want = p * *mass_at;                             // top-p of the mass found here
     }
     uint32_t mine = 0, kept;                                           // a prefix: counting is enough
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
         const bool first = above.cnt == 0 && i0 + j == 0;
-        if (i0 + j < min(n, last) && (!by_mass || (double)before < want || first)) ++mine;
+        if (i0 + j < min(n, last) && (!by_mass || before < want || first)) ++mine;
         before += e[j];
     }
     block_scan<BLOCK, uint32_t>(mine, s.wave_a, &kept);
@@ -475,28 +526,51 @@ __device__ __forceinline__ int cut_list(Shared<BLOCK> &s, const RowState &o, Fil
 }
 
 // The bin that takes the running count to `want` (by_count), or the running mass to `wantm`; adds what stands before it to
-// `above` (masses only where the histogram has them).  kBins: none does.
+// `above` (masses only where the histogram has them).  kBins: none does by count, or all are empty.
 template <int BLOCK>
 __device__ __forceinline__ int find_bin(Shared<BLOCK> &s, const Histogram &h, bool by_count, bool masses, uint32_t want, double wantm, Above &above) {
     constexpr int kPer = kBins / BLOCK;
     const int b0 = threadIdx.x * kPer;
     uint32_t c[kPer], cs = 0, call;
-    uint64_t m[kPer], ms = 0, mb = 0;
-    unsigned long long mall;
+    double m[kPer], ms = 0.0, mb = 0.0, mall;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) c[j] = h.cnt[b0 + j], m[j] = masses ? h.mass[b0 + j] : 0, cs += c[j], ms += m[j];
-    if (threadIdx.x == 0) s.found[0] = kBins;
-    uint64_t cb = above.cnt + block_scan<BLOCK, uint32_t>(cs, s.wave_a, &call);
-    if (masses) mb = above.mass + block_scan<BLOCK, unsigned long long>(ms, (unsigned long long *)s.wave_u, &mall);
+    for (int j = 0; j < kPer; ++j) c[j] = h.cnt[b0 + j], m[j] = masses ? h.mass[b0 + j] : 0.0, cs += c[j], ms += m[j];
+    if (threadIdx.x == 0) s.found[0] = kBins, s.first = kBins, s.back = -1;
+    uint32_t cb = above.cnt + block_scan<BLOCK, uint32_t>(cs, s.wave_a, &call);
+    if (masses) mb = above.mass + block_scan<BLOCK, double>(ms, s.wave_d, &mall);
+    const uint32_t cb0 = cb;
+    const double mb0 = mb;
+    int hit = kBins;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-        const bool hit = by_count ? cb < want && cb + c[j] >= want : (double)mb < wantm && (double)(mb + m[j]) >= wantm;
-        if (hit) s.found[0] = b0 + j, s.found[1] = cb, s.found[2] = mb;
+        if (hit == kBins && c[j] && (by_count ? cb < want && cb + c[j] >= want : mb + m[j] >= wantm)) hit = b0 + j;
         cb += c[j], mb += m[j];
+    }
+    if (!by_count) {
+        // the first of all threads' (their running masses differ by roundings, so several may see the crossing); where no one sees it,
+        // the sums of a bin's parts having rounded below its own, the last bin that holds anything
+        int back = -1;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) back = c[j] ? b0 + j : back;
+        const uint64_t over = __ballot(hit < kBins), some = __ballot(back >= 0);
+        const int lane = threadIdx.x & 63;
+        if (over && lane == __builtin_ctzll(over)) atomicMin(&s.first, hit);
+        if (some && lane == 63 - __builtin_clzll(some)) atomicMax(&s.back, back);
+        __syncthreads();
+        const int bin = s.first < kBins ? s.first : s.back;
+        hit = bin >= b0 && bin < b0 + kPer ? bin : kBins;
+    }
+    if (hit < kBins) {
+        uint32_t cnt = cb0;
+        double mass = mb0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+            if (b0 + j < hit) cnt += c[j], mass += m[j];
+        s.found[0] = hit, s.found[1] = cnt, s.found[2] = __builtin_bit_cast(uint64_t, mass);
     }
     __syncthreads();
     const int bin = (int)uniform(s.found[0]);
-    if (bin < kBins) above.cnt = (uint32_t)uniform(s.found[1]), above.mass = uniform(s.found[2]);
+    if (bin < kBins) above.cnt = (uint32_t)uniform(s.found[1]), above.mass = __builtin_bit_cast(double, uniform(s.found[2]));
     __syncthreads();
     return bin;
 }
@@ -511,18 +585,18 @@ struct Step {
 };
 
 template <int BLOCK>
-__device__ __forceinline__ Step make_step(Shared<BLOCK> &s, const Histogram &h, const RowState &o, bool by_count, uint64_t mass_k) {
+__device__ __forceinline__ Step make_step(Shared<BLOCK> &s, const Histogram &h, const RowState &o, bool by_count, double mass_k) {
     Step st;
     st.by_count = by_count;
-    st.wantm = fmax(o.f.p * (double)mass_k, 0.5);          // top-p keeps at least the first
-    st.above = Above{0, 0};
+    st.wantm = o.f.p * mass_k;
+    st.above = Above{0, 0.0};
     st.bin = find_bin<BLOCK>(s, h, by_count, true, o.f.k, st.wantm, st.above);
     st.any = st.bin < kBins;
     st.n = st.any ? uniform(h.cnt[st.bin]) : 0;
     st.prefix = st.above.cnt + st.n <= (uint32_t)kList;
     st.fits = st.prefix || st.n <= (uint32_t)kList;
     st.from = st.prefix ? 0 : st.bin;
-    if (st.prefix) st.above = Above{0, 0};
+    if (st.prefix) st.above = Above{0, 0.0};
     return st;
 }
 
@@ -531,15 +605,15 @@ template <int BLOCK>
 __device__ __forceinline__ Step first_step(Shared<BLOCK> &s, const Histogram &h, RowState &o) {
     constexpr int kPer = kBins / BLOCK;
     uint32_t c = 0, total;
-    unsigned long long m = 0, mass;
+    double m = 0.0, mass;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) c += h.cnt[threadIdx.x * kPer + j], m += h.mass[threadIdx.x * kPer + j];
     block_scan<BLOCK, uint32_t>(c, s.wave_a, &total);
-    block_scan<BLOCK, unsigned long long>(m, (unsigned long long *)s.wave_u, &mass);
-    total = uniform(total), mass = uniform((uint64_t)mass);
-    if (o.f.k < (int)total) return make_step<BLOCK>(s, h, o, true, 0);
+    block_scan<BLOCK, double>(m, s.wave_d, &mass);
+    total = uniform(total), mass = __builtin_bit_cast(double, uniform(__builtin_bit_cast(uint64_t, mass)));
+    if (o.f.k < (int)total) return make_step<BLOCK>(s, h, o, true, 0.0);
     o.f.k = (int)total;
-    if (o.use_p && mass) return make_step<BLOCK>(s, h, o, false, mass);
+    if (o.use_p && mass > 0.0) return make_step<BLOCK>(s, h, o, false, mass);
     Step none{};
     return none;
 }
@@ -637,17 +711,11 @@ __device__ __forceinline__ uint32_t gather(Shared<BLOCK> &s, const RowState &o, 
     return finish_list<BLOCK, T>(s, o, row, begin + pieces * E + threadIdx.x, end, want);
 }
 
-template <int BLOCK>
-__device__ __forceinline__ void clear_histogram(Histogram &h) {
-    for (int b = threadIdx.x; b < kBins; b += BLOCK) h.cnt[b] = 0, h.mass[b] = 0;
-    __syncthreads();
-}
-
 // A cut inside a bin that holds more than the list: the bin's range of keys is split again (whole row per step) until the
 // entries fit, or share one value.  Uses up the histogram.
 template <int BLOCK, typename T>
 __device__ __forceinline__ void cut_range(Shared<BLOCK> &s, Histogram &h, const RowState &o, Filter &f, const T *row, int size, const Step &st,
-                          uint64_t *mass_at) {
+                          double *mass_at) {
     uint32_t hi = 0, lo = 0xffffffffu, n = st.n;
     {
         float top = -__builtin_inff(), low = __builtin_inff();
@@ -661,15 +729,9 @@ __device__ __forceinline__ void cut_range(Shared<BLOCK> &s, Histogram &h, const 
     while (n > (uint32_t)kList && lo < hi) {
         int bits = 0;
         while (((hi - lo) >> bits) >= (uint32_t)kBins) ++bits;
-        clear_histogram<BLOCK>(h);
-        for_each<BLOCK, 1>(row, 0, size, [&](float x, int, int) {
-            const uint32_t key = key_of(x);
-            if (key >= lo && key <= hi) {
-                atomicAdd(&h.cnt[(hi - key) >> bits], 1u);
-                atomicAdd((unsigned long long *)&h.mass[(hi - key) >> bits], (unsigned long long)fixed(mass_of(o.w, x), o.shift));
-            }
-        });
-        __syncthreads();
+        const int up = raise(o, st.bin);                 // all of these entries lie in that bin
+        fill_histogram<BLOCK, T>(h, o, row, size, [=](float, uint32_t key) { return key >= lo && key <= hi ? (int)((hi - key) >> bits) : -1; },
+                                 [=](int) { return up; });
         const int bin = min(find_bin<BLOCK>(s, h, st.by_count, true, f.k, st.wantm, above), kBins - 1);
         n = uniform(h.cnt[bin]);
         hi -= (uint32_t)bin << bits;
@@ -689,14 +751,14 @@ __device__ __forceinline__ void cut_range(Shared<BLOCK> &s, Histogram &h, const 
         return;
     }
     // one value, more than kList times: the first q of them by index
-    const uint64_t e = fixed(mass_of(o.w, value_of(hi)), o.shift);
+    const double e = mass_of(o.w, value_of(hi));
     uint32_t q = n;
     if (st.by_count) q = f.k - above.cnt;
-    else if (e > 0) {
-        // the smallest q whose mass reaches the target; the quotient's rounding is mended
-        q = (uint32_t)fmin((double)n, fmax(1.0, __builtin_ceil((st.wantm - (double)above.mass) / (double)e)));
-        while (q > 1 && (double)(above.mass + (q - 1) * e) >= st.wantm) --q;
-        while (q < n && (double)(above.mass + q * e) < st.wantm) ++q;
+    else if (e > 0.0) {
+        // as many as have less than the target before them; the quotient's rounding is mended
+        q = (uint32_t)fmin((double)n, fmax(1.0, __builtin_ceil((st.wantm - above.mass) / e)));
+        if (q > 1 && above.mass + (q - 1) * e >= st.wantm) --q;
+        else if (q < n && above.mass + q * e < st.wantm) ++q;
     }
     *mass_at = above.mass + q * e;
     f.key = hi;
@@ -714,16 +776,16 @@ __device__ __forceinline__ void cut_range(Shared<BLOCK> &s, Histogram &h, const 
     __syncthreads();
 }
 
-// Mass (fixed point) of the entries that top-k's cut keeps
+// Mass of the entries that top-k's cut keeps
 template <int BLOCK, typename T>
-__device__ __forceinline__ uint64_t mass_of_first(Shared<BLOCK> &s, const RowState &o, const T *row, int size) {
-    unsigned long long mine = 0, all;
+__device__ __forceinline__ double mass_of_first(Shared<BLOCK> &s, const RowState &o, const T *row, int size) {
+    double mine = 0.0, all;
     for_each<BLOCK, 1>(row, 0, size, [&](float x, int i, int) {
         const uint32_t key = key_of(x);
-        if (key && o.f.keeps(key, i)) mine += fixed(mass_of(o.w, x), o.shift);
+        if (key && o.f.keeps(key, i)) mine += mass_of(o.w, x);
     });
-    block_scan<BLOCK, unsigned long long>(mine, (unsigned long long *)s.wave_u, &all);
-    return uniform((uint64_t)all);
+    block_scan<BLOCK, double>(mine, s.wave_d, &all);
+    return __builtin_bit_cast(double, uniform(__builtin_bit_cast(uint64_t, all)));
 }
 
 // Both cuts of a long row, from its histogram (used up where a bin is too full).  gathered: the entries of the first step are in
@@ -731,7 +793,7 @@ __device__ __forceinline__ uint64_t mass_of_first(Shared<BLOCK> &s, const RowSta
 template <int BLOCK, typename T>
 __device__ __forceinline__ int select_cut(Shared<BLOCK> &s, Histogram &h, RowState &o, const T *row, int size, Step st, bool gathered) {
     while (st.any) {
-        uint64_t mass_at = 0;
+        double mass_at = 0.0;
         if (st.fits) {
             const int n = gathered ? uniform(s.count) : gather<BLOCK, T>(s, o, row, 0, size, Reach(st.from, st.bin));
             gathered = false;
@@ -751,9 +813,7 @@ __device__ __forceinline__ int select_cut(Shared<BLOCK> &s, Histogram &h, RowSta
         }
         if (!(st.by_count && o.use_p)) break;
         // top-k's list was not the whole prefix: top-p by masses, which a histogram for top-k's sake has not got
-        clear_histogram<BLOCK>(h);
-        add_to_histogram<BLOCK, T>(h, o, row, 0, size, true);
-        __syncthreads();
+        fill_histogram<BLOCK, T>(h, o, row, size);
         mass_at = mass_of_first<BLOCK, T>(s, o, row, size);
         st = make_step<BLOCK>(s, h, o, false, mass_at);
     }
@@ -983,22 +1043,23 @@ __device__ __forceinline__ void wave_sort(uint64_t *list, int n, uint64_t *c) {
 template <int P, int BLOCK>
 __device__ __forceinline__ void draw_few(Shared<BLOCK> &s, const RowState &o, int n, const float *u, int draws, int64_t *ids, float *prob) {
     const int lane = threadIdx.x & 63, i0 = lane * P, last = min(o.f.k, n);
-    uint64_t c[P], e[P], run = 0, at_last = 0;
+    uint64_t c[P];
+    double e[P], run = 0.0, at_last = 0.0;
 #pragma unroll
     for (int j = 0; j < P; ++j) c[j] = s.list[min(i0 + j, n - 1)];
     wave_sort<P>(s.list, n, c);
 #pragma unroll
     for (int j = 0; j < P; ++j) {
-        e[j] = i0 + j < n ? fixed(mass_of(o.w, value_of(~(uint32_t)(c[j] >> 32))), o.shift) : 0;
+        e[j] = i0 + j < n ? mass_of(o.w, value_of(~(uint32_t)(c[j] >> 32))) : 0.0;
         run += e[j];
         if (i0 + j == last - 1) at_last = run;
     }
-    uint64_t before = wave_scan<unsigned long long>(run) - run;
-    const double want = o.f.p * (double)__shfl((unsigned long long)(before + at_last), (last - 1) / P);
+    double before = lane_before(wave_scan(run));
+    const double want = o.f.p * __shfl(before + at_last, (last - 1) / P);
     uint32_t mine = 0;
 #pragma unroll
     for (int j = 0; j < P; ++j) {
-        if (i0 + j < last && (!o.use_p || (double)before < want || i0 + j == 0)) ++mine;
+        if (i0 + j < last && (!o.use_p || before < want || i0 + j == 0)) ++mine;
         before += e[j];
     }
     const int kept = (int)__builtin_amdgcn_readlane(wave_scan(mine), 63);
@@ -1033,9 +1094,9 @@ __device__ __forceinline__ void draw_top_k(Shared<BLOCK> &s, RowState &o, int n,
         if (threadIdx.x < 64) draw_few<2>(s, o, n, u, draws, ids, prob);
         return;
     }
-    uint64_t mass_at;
+    double mass_at;
     sort_by_value<BLOCK>(s, n, o.w.topf, fminf((float)kBins / (o.w.topf - low), 1e30f));
-    const int kept = cut_list<BLOCK>(s, o, o.f, n, Above{0, 0}, min(o.f.k, n), o.use_p, o.f.p, 0.0, &mass_at);
+    const int kept = cut_list<BLOCK>(s, o, o.f, n, Above{0, 0.0}, min(o.f.k, n), o.use_p, o.f.p, 0.0, &mass_at);
     list_by_index<BLOCK>(s, kept, size);
     draw_from_list<BLOCK>(s, o, kept, u, draws, ids, prob);
 }
@@ -1070,14 +1131,15 @@ template <int BLOCK, typename T>
 __device__ __forceinline__ void draw_long_row(Shared<BLOCK> &s, Histogram &h, double *tiles, RowState &o, const RowIO<T> &io, const SampleArgs &a) {
     if (o.f.cut) {
         const bool by_k = o.f.k < a.size;
-        clear_histogram<BLOCK>(h);
-        add_to_histogram<BLOCK, T>(h, o, io.row, 0, a.size, !by_k);
-        __syncthreads();
+        if (by_k) {
+            clear_histogram<BLOCK>(h);
+            add_counts<BLOCK, T>(h, o, io.row, 0, a.size);
+        } else {
+            fill_histogram<BLOCK, T>(h, o, io.row, a.size);
+        }
         Step st = first_step<BLOCK>(s, h, o);
         if (by_k && !st.any && o.use_p) {          // fewer than k can be drawn: top-p of them all
-            clear_histogram<BLOCK>(h);
-            add_to_histogram<BLOCK, T>(h, o, io.row, 0, a.size, true);
-            __syncthreads();
+            fill_histogram<BLOCK, T>(h, o, io.row, a.size);
             st = first_step<BLOCK>(s, h, o);
         }
         const int listed = select_cut<BLOCK, T>(s, h, o, io.row, a.size, st, false);
@@ -1169,7 +1231,7 @@ __global__ void __launch_bounds__(1024) sample_row_kernel(const SampleArgs a) {
         for (int u = 0; u < 4; ++u)
             if (group[u] > -__builtin_inff()) atomicAdd(&h.cnt[bin_of(o.w, o.scale, group[u])], 1u);
         __syncthreads();
-        Above above{0, 0};
+        Above above{0, 0.0};
         // where fewer than k groups hold anything: all entries, if they fit
         const int bin = min(find_bin<BLOCK>(s, h, true, false, o.f.k, 0.0, above), kBins - 1);
         const Reach want(o, bin);
@@ -1298,6 +1360,7 @@ struct RowWork {
     int32_t cut_idx, last_tile;
     alignas(256) float group[kGroups];
     Histogram h;
+    uint64_t high[kBins];                  // upper halves of the words, apart where more than kSegment entries could pass 64 bits
     uint64_t list[kList];
     double tiles[kMaxTiles];
 };
@@ -1381,7 +1444,10 @@ __global__ void __launch_bounds__(1024) sample_max_kernel(const SampleArgs a, Ro
 #pragma unroll
     for (int d = 1; d < kOf; d <<= 1) g = fmaxf(g, __shfl_xor(g, d));
     if (tid % kOf == 0) w.group[part * kEach + tid / kOf] = g;
-    for (int b = tid; b < kBins / kParts; b += BLOCK) w.h.cnt[part * (kBins / kParts) + b] = 0, w.h.mass[part * (kBins / kParts) + b] = 0;
+    for (int i = tid; i < kBins / kParts; i += BLOCK) {
+        const int b = part * (kBins / kParts) + i;
+        w.h.cnt[b] = 0, w.h.word[b] = 0, w.high[b] = 0;
+    }
     block_max_min<BLOCK>(top, low, s);
     const float t = a.temperature_v ? a.temperature_v[r] : a.temperature;
     const int first = t == 0.0f ? find_value<BLOCK, T>(s, io.row, p.begin, p.end, top, a.size) : 0;
@@ -1426,7 +1492,7 @@ __global__ void __launch_bounds__(1024) sample_groups_kernel(const SampleArgs a,
         if (group[u] > -__builtin_inff()) atomicAdd(&h.cnt[bin_of(o.w, o.scale, group[u])], 1u);
     }
     __syncthreads();
-    Above above{0, 0};
+    Above above{0, 0.0};
     const int bin = min(find_bin<BLOCK>(s, h, true, false, o.f.k, 0.0, above), kBins - 1);
     const Part p = part_of(a.size, blockIdx.x, gridDim.x);
     gather_part<BLOCK, T>(s, o, io.row, p, Reach(o, bin), w.list, &w.count[0]);
@@ -1452,14 +1518,24 @@ __global__ void __launch_bounds__(1024) sample_bins_kernel(const SampleArgs a, R
     if (tid < 16) tab[tid] = kRoots[tid];
     const RowState o = state_of(a, r, w, tab);
     if (o.plain() || !o.f.cut) return;
-    clear_histogram<BLOCK>(h);
     const RowIO<T> io(a, r);
     const Part p = part_of(a.size, blockIdx.x, gridDim.x);
-    add_to_histogram<BLOCK, T>(h, o, io.row, p.begin, p.end, o.use_p);
-    __syncthreads();
-    for (int b = tid; b < kBins; b += BLOCK) {
-        if (h.cnt[b]) atomicAdd(&w.h.cnt[b], h.cnt[b]);
-        if (h.mass[b]) atomicAdd((unsigned long long *)&w.h.mass[b], (unsigned long long)h.mass[b]);
+    for (int begin = p.begin; begin < p.end; begin += kSegment) {
+        const int end = min(p.end, begin + kSegment);
+        clear_histogram<BLOCK>(h);
+        if (o.use_p)
+            add_words<BLOCK, T>(h, o, io.row, begin, end, [&](float x, uint32_t key) { return key ? bin_of(o.w, o.scale, x) : -1; },
+                                [&](int b) { return raise(o, b); });
+        else add_counts<BLOCK, T>(h, o, io.row, begin, end);
+        for (int b = tid; b < kBins; b += BLOCK) {
+            const unsigned long long v = h.word[b];
+            if (h.cnt[b]) atomicAdd(&w.h.cnt[b], h.cnt[b]);
+            if (v == 0) continue;
+            const bool apart = a.size > kSegment;
+            atomicAdd((unsigned long long *)&w.h.word[b], apart ? v & 0xffffffffu : v);
+            if (apart) atomicAdd((unsigned long long *)&w.high[b], v >> 32);
+        }
+        __syncthreads();
     }
 }
 
@@ -1475,7 +1551,11 @@ __global__ void __launch_bounds__(1024) sample_cut_kernel(const SampleArgs a, Ro
     if (tid < 16) s.tab[tid] = kRoots[tid];
     RowState o = state_of(a, r, w, s.tab);
     if (o.plain() || !o.f.cut) return;
-    for (int b = tid; b < kBins; b += BLOCK) h.cnt[b] = w.h.cnt[b], h.mass[b] = w.h.mass[b];
+    for (int b = tid; b < kBins; b += BLOCK) {
+        h.cnt[b] = w.h.cnt[b];
+        const double high = a.size > kSegment ? (double)w.high[b] * 0x1p32 : 0.0;
+        h.mass[b] = __builtin_ldexp(high + (double)w.h.word[b], -raise(o, b));
+    }
     __syncthreads();
     const RowIO<T> io(a, r);
     const Part p = part_of(a.size, blockIdx.x, gridDim.x);
