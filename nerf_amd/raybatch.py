@@ -120,7 +120,10 @@ class ImageRaySampler:
         sampling.sample_logits -- an error map's logarithm draws the pixels the network still gets wrong (no counterpart in the
         reference).  logits: one per candidate pixel, in the order of crop_pixels() (all H*W where precrop_frac is None).
         -> (batch_rays [2, N_rand, 3], target_s [N_rand, 3], pix [N_rand], prob [N_rand]): pix = y*W + x, prob what each was
-        drawn with (weights 1 / (n prob) make a loss unbiased).  Where nothing can be drawn, pix is -1 and the ray NaN."""
+        drawn with.  Weights 1 / (n prob), n the number of candidate pixels, make a mean over the draws an unbiased estimate of that over
+        the candidates as long as each of them can be drawn: finite logits, and none of top_k, top_p and min_p.  A filter's pixels are
+        never drawn, so their share is missing from the estimate, whatever the weights.  Where nothing can be drawn, pix is -1,
+        prob 0 and the ray NaN."""
         cand = self.crop_pixels(precrop_frac)
         n = self.H * self.W if cand is None else cand.numel()
         if logits.numel() != n:
