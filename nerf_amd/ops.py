@@ -183,6 +183,9 @@ def sample_pdf(bins, weights, n_samples, u=None):
     return out.reshape(*lead, n_samples)
 
 
+_COUNTS = {torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64}
+
+
 def _per_row(v, name, dtype, lead, device):
     """(scalar, per-row tensor or None) of a filter given as a number or as one value per row."""
     if not isinstance(v, torch.Tensor):
@@ -192,14 +195,17 @@ def _per_row(v, name, dtype, lead, device):
     if v.shape != lead:
         raise ValueError(f"{name}: expected one value per row {tuple(lead)}, got {tuple(v.shape)}")
     if dtype == torch.int32 and v.dtype != torch.int32:
-        v = v.clamp(0, 2 ** 31 - 1)
+        if v.dtype not in _COUNTS:
+            raise TypeError(f"{name}: expected whole numbers, got {v.dtype}")
+        v = v.to(torch.int64).clamp(0, 2 ** 31 - 1)
     return 0, v.to(dtype).contiguous()
 
 
 def sample_logits(logits, n_samples, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, u=None):
     """n_samples indices drawn from each row of `logits` [..., V] (f32 / bf16 / f16) -> (ids [..., n_samples] int64,
     prob [..., n_samples] f32, the probabilities they were drawn with).  u [..., n_samples]: the uniform numbers to draw by
-    (None: torch.rand).  temperature, top_k, top_p, min_p: numbers, or tensors with one value per row; see nrf_sample_logits."""
+    (None: torch.rand).  temperature, top_k, top_p, min_p: numbers, or tensors with one value per row (top_k: of a whole type); see
+    nrf_sample_logits."""
     _typed(logits, "logits")
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits: expected [..., V >= 1], got {tuple(logits.shape)}")
