@@ -6,6 +6,7 @@ render.run_network(..., codes=...) appends one code per ray to the direction cha
 each ray of a batch comes from.  The kernels are nrf_lookup_fwd and nrf_lookup_bwd."""
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -27,7 +28,10 @@ class _LookupFunction(torch.autograd.Function):
 
 
 def lookup(table, ids, scale=1.0, padding_idx=None, out_dtype=None):
-    """scale * table[ids] with the gradient w.r.t. `table`; see ops.lookup_fwd / ops.lookup_bwd for types and shapes."""
+    """scale * table[ids] with the gradient w.r.t. `table` (reverse mode; forward mode is refused); see ops.lookup_fwd / ops.lookup_bwd
+    for types and shapes."""
+    if forward_ad.unpack_dual(table).tangent is not None:       # the kernel's output would lose the tangent
+        raise NotImplementedError("lookup: no forward-mode derivative (jvp)")
     if table.requires_grad and torch.is_grad_enabled():
         return _LookupFunction.apply(table, ids, float(scale), padding_idx, out_dtype)
     return ops.lookup_fwd(table, ids, scale, out_dtype)
