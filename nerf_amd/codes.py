@@ -32,6 +32,8 @@ def lookup(table, ids, scale=1.0, padding_idx=None, out_dtype=None):
     for types and shapes."""
     if forward_ad.unpack_dual(table).tangent is not None:       # the kernel's output would lose the tangent
         raise NotImplementedError("lookup: no forward-mode derivative (jvp)")
+    if padding_idx is not None and not 0 <= padding_idx < table.shape[0]:
+        raise ValueError(f"padding_idx {padding_idx} is outside the table's {table.shape[0]} rows")
     if table.requires_grad and torch.is_grad_enabled():
         return _LookupFunction.apply(table, ids, float(scale), padding_idx, out_dtype)
     return ops.lookup_fwd(table, ids, scale, out_dtype)

@@ -42,3 +42,10 @@ def test_reverse_mode_and_none(plain):
     assert not codes.lookup(table.detach(), ids).requires_grad
     with fwd_ad.dual_level():                                   # a level alone makes no table a dual one
         assert torch.equal(codes.lookup(table, ids), table[ids])
+
+
+@pytest.mark.parametrize("padding_idx", [5, -1, 1 << 40])
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_padding_row_outside_the_table_is_refused_before_the_backward_pass(plain, padding_idx, grad):
+    with pytest.raises(ValueError, match="outside the table's 5 rows"):
+        codes.lookup(torch.randn(5, 3, requires_grad=grad), torch.tensor([1]), padding_idx=padding_idx)
