@@ -53,6 +53,12 @@ def _rows(t):
     return t, (row if n > 1 else dim)
 
 
+def _fits(v, what):
+    """ctypes takes a 32-bit argument modulo 2^32."""
+    if v > 2 ** 31 - 1:
+        raise ValueError(f"{what} {v}: more than 2^31 - 1")
+
+
 def _opt(t):
     return None if t is None else t.data_ptr()
 
@@ -212,6 +218,8 @@ def sample_logits(logits, n_samples, temperature=1.0, top_k=0, top_p=1.0, min_p=
     dev, lead, V, n = logits.device, logits.shape[:-1], logits.shape[-1], int(n_samples)
     if n < 0:
         raise ValueError(f"n_samples: {n}")
+    _fits(V, "logits: rows of")
+    _fits(n, "n_samples:")
     x = logits if logits.dim() == 2 else logits.reshape(-1, V)
     if V > 1 and x.stride(1) != 1:
         x = x.contiguous()
@@ -279,6 +287,7 @@ def lookup_fwd(table, ids, scale=1.0, out_dtype=None):
     _typed(table, "table")
     if table.dim() != 2 or table.shape[1] < 1:
         raise ValueError(f"table: expected [rows, dim >= 1], got {tuple(table.shape)}")
+    _fits(table.shape[1], "table: rows of")
     ids = _ids(ids, table.device)
     out_dtype = table.dtype if out_dtype is None else out_dtype
     if out_dtype != table.dtype and out_dtype != torch.float32:
@@ -298,6 +307,7 @@ def lookup_bwd(g_out, ids, n_rows, scale=1.0, padding_idx=None, dtype=None):
     ids = _ids(ids, g_out.device)
     if g_out.dim() < 1 or g_out.shape[:-1] != ids.shape or g_out.shape[-1] < 1:
         raise ValueError(f"g_out: expected [*{tuple(ids.shape)}, dim >= 1], got {tuple(g_out.shape)}")
+    _fits(g_out.shape[-1], "g_out: rows of")
     dtype = g_out.dtype if dtype is None else dtype
     if dtype not in _DTYPES or (g_out.dtype != dtype and g_out.dtype != torch.float32):
         raise TypeError(f"dtype {dtype} does not go with a gradient of {g_out.dtype}")
