@@ -928,7 +928,7 @@ __device__ __forceinline__ bool pick_entry(const double *e, double sum, double c
     const uint64_t over = __ballot(sum > 0.0 && before + cum > want), some = __ballot(sum > 0.0);
     if (some == 0) return false;
     const int src = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
-    double run = before + (cum - sum), m = 0.0;
+    double run = before + lane_before(cum), m = 0.0;
     int in = 0;
     bool found = false;
 #pragma unroll
@@ -1077,7 +1077,7 @@ __device__ __forceinline__ void draw_few(Shared<BLOCK> &s, const RowState &o, in
         m[j] = i0 + j < kept ? mass_or_zero(o, (uint32_t)c[j]) : 0.0;
         sum += m[j];
     }
-    double cum = wave_scan(sum) - sum;
+    double cum = lane_before(wave_scan(sum));          // (not a difference: a small mass before a large one would be lost)
 #pragma unroll
     for (int j = 0; j < P; ++j) {
         cum += m[j];

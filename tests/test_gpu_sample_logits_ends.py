@@ -72,3 +72,33 @@ def test_the_end_of_short_rows_and_of_lists(V):
     u = torch.tensor([ENDS] * 30).cuda()
     for f in (dict(), dict(k=200), dict(p=0.9), dict(m=0.02), dict(k=1000, p=0.99, m=1e-3)):
         check(x, u, **f)
+
+
+@pytest.mark.parametrize("R,V,n", [(6, 5, 3), (6, 700, 3), (6, 1500, 17), (6, 2048, 3), (6, 4483, 3), (200, 40000, 3), (2, 150000, 30)])
+def test_the_first_entry_with_mass_however_small(R, V, n):
+    """u = 0: a mass far below a rounding of the sums, at the row's first entry, with the largest close behind it or far."""
+    rng = np.random.RandomState(V)
+    u = rng.rand(R, n).astype(np.float32)
+    u[:, :2] = [0.0, -1.0]
+    u = torch.from_numpy(u).cuda()
+    for down in (40.0, 300.0, 650.0):
+        x = rng.uniform(-900.0, -800.0, (R, V)).astype(np.float32)       # no mass at all
+        for r in range(R):
+            peak = int(rng.randint(1, V)) if r % 3 == 2 else 1 + r % min(V - 1, 4)
+            x[r, peak] = 0.0
+            x[r, int(rng.randint(0, peak))] = -down
+        for f in (dict(), dict(k=2), dict(k=5), dict(k=V // 2), dict(k=min(V, 300))):
+            check(torch.from_numpy(x).cuda(), u, **f)
+
+
+@pytest.mark.parametrize("V", [12, 700, 3000])
+@pytest.mark.parametrize("L", [2, 3, 4, 5, 8, 12])
+def test_lists_that_begin_with_a_small_mass(V, L):
+    """All places of a small mass and the largest in a list of L entries, the others without mass."""
+    pairs = [(i, j) for j in range(1, L) for i in range(j)]
+    x = np.full((len(pairs), V), -900.0, np.float32)
+    x[:, :L] = -800.0
+    for r, (i, j) in enumerate(pairs):
+        x[r, i], x[r, j] = -200.0 - r, 0.0
+    u = torch.tensor([[0.0, -3.0, 2.0 ** -24, 0.5, 1.0]] * len(pairs)).cuda()
+    check(torch.from_numpy(x).cuda(), u, k=L)
