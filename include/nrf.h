@@ -402,7 +402,7 @@ int nrf_lookup_bwd(const void *g_out, int64_t g_stride, int32_t g_dtype, const v
  * (<= 0: all), of those the shortest prefix that holds top_p of their mass (>= 1: all), of those the ones with
  * e_i >= min_p (<= 0: all); the first entry always.  A draw is the first kept index whose running mass, in the order of the
  * index, exceeds u times the kept mass.  temperature 0: the first maximum.  Masses and sums are f64 (in rows above 2048 logits top-p
- * sees the mass of each to 2^-41 of itself, whatever the size).
+ * sees a mass to 2^-42 of the largest within temperature / 32, or 1/128, of its logit).
  * Each of the four can be given per row (a DEVICE array of n_rows values; NULL: the scalar).
  * -inf and NaN logits are never drawn; +inf logits share the whole mass.  id -1, prob 0: a row in which nothing can be drawn, a
  * row whose temperature is negative or not finite or whose top_p or min_p is NaN, a u that is NaN.  u outside [0, 1] is clamped;

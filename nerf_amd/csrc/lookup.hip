@@ -24,8 +24,8 @@ namespace {
 constexpr int kMaxDim = 32768;
 
 // Rows are taken in vectors of VW elements at any alignment (the hardware splits what crosses a line); where VW does not divide a row,
-// its last vector overlaps the one before and both give the shared elements the same bits.  786432 x 33 f32, the sums of tiles: 20.8 us against
-// 37 by single elements.
+// its last vector overlaps the one before and both give the shared elements the same bits.  The gradient of 786432 x 33 f32 over 200 rows:
+// 49 us a call against 58 by single elements.
 template <int VW>
 __device__ __forceinline__ int column(int vector, int dim) { return min(vector * VW, dim - VW); }
 
@@ -49,7 +49,7 @@ __device__ __forceinline__ void store_once(V *p, V v) {
 }
 
 // blockDim 256; chunk = VW elements of one row; `per_row` = dim / VW, up; magic = ceil(2^32 / per_row).  An output that the L2s could not
-// hold (32 MB) goes past them, which leaves them to rows that are met again: 16384 ids x 4096 bf16 34.5 us against 36.8.
+// hold (32 MB) goes past them, which leaves them to rows that are met again: 16384 ids x 4096 bf16 32.8 us against 34.9.
 template <typename T, typename O, int VW, typename I>
 __global__ void __launch_bounds__(256) lookup_fwd_kernel(const T *__restrict__ table, int64_t stride, int64_t n_rows,
                                                          const I *__restrict__ ids, int64_t chunks, int dim, uint32_t per_row,
@@ -680,8 +680,8 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const SumArgs a, const I 
 // lists its own tokens in order (ballots), ranks them by row in LDS, and writes the sums of its rows, zeros included.  Rows of up to
 // kLight tokens are a team's (several to a wave), up to kWaveTokens times a wave's teams a wave's, others the block's; the teams' sums
 // are added by halves, the waves' in order.  Its rows lie in groups of 64 bytes or more, 2^bits groups apart: neighbouring rows are
-// often met alike (frequent ids first), and 16384 such tokens x 4 bf16 over 74009 rows take 45 us in one range, 24 in groups of 256
-// bytes and 17.5 in groups of 64.  4096 x 10 bf16 over 12011 rows: 9.9 us a call (sorted 17); 16384 x 64 over 8000: 11.8 (24).
+// often met alike (frequent ids first), and 16384 such tokens x 4 bf16 over 74009 rows take 40.5 us in one range, 23.4 in groups of 256
+// bytes and 16.5 in groups of 64.  4096 x 10 bf16 over 12011 rows: 8.2 us a call (sorted 22); 16384 x 64 over 8000: 11.2 (24).
 constexpr int kLight = 16;
 constexpr int kWaveTokens = 64;
 constexpr int kMaxLow = 10;
@@ -875,7 +875,7 @@ __global__ void __launch_bounds__(1024, ITEMS > kTileItems ? 4 : 8) sum_ranges_k
 // pass, by the ids' high bits, into at most 1024 buckets of 2^low neighbouring table rows.  A block then takes up to `chunk` tokens
 // of a bucket, ranks them by their low bits (stable), lays their rows out in that order in LDS, and a thread adds each element of the
 // bucket's table rows, zeros included.  Buckets of more than a chunk leave their sums per chunk, added in order by a last launch.
-// 2^21 rows of two f32 into 524288: 64 us (5 count, 7 scan, 31 scatter, 22 sums, 5 join) against 111 by sorted pairs.
+// 2^21 rows of two f32 into 524288: 64 us (5 count, 7 scan, 31 scatter, 22 sums, 5 join) against 112 by sorted pairs.
 struct NarrowArgs {
     const void *g;
     int64_t g_stride, n;
@@ -1169,8 +1169,8 @@ struct BwdPlan {
 
 // Few rows, few tokens: without a sort (one or two launches against three or more).  The ids are read once a row or token, and a block may
 // meet all of g: each of its teams then 256 tokens at most, about 20 us.
-// Measured, us a call, against the sorted way: 4096 tokens x 32 over 100 rows 9.0 / 16.5, all on one row 10.2 / 17.7; 16384 x 8 over
-// 256 rows 11.7 / 31; 64 x 1024 over 1024 rows 9.2 / 16.2.
+// Measured, us a call, against the sorted way: 4096 tokens x 32 over 100 rows 8.3 / 16.8, all on one row 10.1 / 17.4; 16384 x 8 over
+// 256 rows 11.7 / 26.7; 64 x 1024 over 1024 rows 8.6 / 15.4.
 enum Few { kNotFew, kFewRows, kFewTokens };
 Few few_tokens(int64_t n, int64_t n_rows, int dim) {
     const int vw = dim >= 4 ? 4 : dim >= 2 ? 2 : 1, vectors = (dim + vw - 1) / vw, lanes = vectors < 256 ? vectors : 256;
@@ -1180,9 +1180,11 @@ Few few_tokens(int64_t n, int64_t n_rows, int dim) {
     return n <= 4096 ? kFewTokens : kNotFew;
 }
 
-// Ranges (what few rows leave): not for large gradients, whose zeros a launch of their own writes faster than blocks that wait for ids
-// (27442 rows x 263 f32: one token 22 us against 12, 4096 tokens 27 against 26; 9298 x 544: 10.5 against 12, 17 against 24), nor where
-// many blocks would read many ids (16384 tokens over 2^19 rows x 10: 25 against 29).
+// Ranges (what few rows leave): not for large gradients, whose zeros a launch of their own writes faster than blocks that wait for ids, nor
+// where many blocks would read many ids.  Us a call by ranges / otherwise, for one token; 4096; 16384 (f32):
+//   9298 rows x 544: 9.8 / 10.5, 16.3 / 24.3    50000 x 263: 15.0 / 13.0, 18.3 / 25.4, 43.3 / 35.3    100000 x 263: 23.4 / 18.9, 27.7 / 26.6,
+//   61.3 / 42.3    1500000 x 10: 20.8 / 15.0, 42.0 / 25.3, 108 / 38.8    2^19 x 10: 16384 tokens 30.9 / 31.1
+// The bound on the gradient's size is on the safe side: 4096 tokens x 263 over 27442 rows, just above it, take 14.8 by ranges, 24.4 otherwise.
 bool in_ranges(int64_t n, int64_t n_rows, int dim) {
     return n <= kSmall && n_rows * dim <= 6 << 20 && n_rows * n <= (int64_t)1 << 33;
 }
@@ -1369,7 +1371,7 @@ void pick_sums(int vw, const SumArgs &a, const BwdPlan &p, const void *ids, bool
     launch_sums<G, T, 1>(a, p, ids, i64, padding, s);
 }
 
-// Elements of a vector: 16 bytes of f32, or of 16-bit types where that divides a row (4096 x 420 bf16: 11 us a call by 4, 15 by 8)
+// Elements of a vector: 16 bytes of f32, or of 16-bit types where that divides a row (gradient of 4096 x 420 bf16 over 4096: 8.7 us a call by 4, 14.1 by 8)
 int width_of(int dim, int es_a, int es_b) {
     if (es_a == 2 && es_b == 2 && dim % 8 == 0) return 8;
     return dim >= 4 ? 4 : dim >= 2 ? 2 : 1;

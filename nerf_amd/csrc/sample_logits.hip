@@ -14,16 +14,18 @@
 //     largest entry from below.  The entries above that bound (a few more than k) go into a list in LDS.
 //   - else a histogram of the row, 2048 bins of equal width below the maximum, counts and masses.  Masses are added there as 64-bit
 //     integers, because these give the same sums in any order, in units that go down with the bin's masses, and are f64 from then on:
-//     what a bin holds is right to 2^-41 of itself, however small it is.  The bin of the cut, or all entries down to it, go into the
-//     list.  A bin that holds more than the list (many equal values, far outliers) is split again by the bits of its values until it
-//     does not, or holds one value only.
+//     an entry is right to 2^-42 of the largest mass its bin could hold, however small that is.  The bin of the cut, or all entries
+//     down to it, go into the list.  A bin that holds more than the list (many equal values, far outliers) is split again by the bits of
+//     its values until it does not, or holds one value only.
 // The list (up to 2048 entries) is sorted.  Where it holds everything that is kept, the draws come from it; else from the
 // masses of the row's tiles of 1024 entries.
 //
-// Three forms: short rows without a cut, a wave each (4096 rows of 1001 f32: 11 us); one block a row (256 rows of 131072 bf16, top-k
-// about 1000 and top-p: 40 us, instructions: two passes of some four a logit; top-p alone 117 us, an f64 exponential a logit); and,
-// for few long rows, 32 or 64 blocks a row over several launches (4096 draws from 640000 f32, top-p: 47 us in five; one of 131072 by
-// top-k: 16 us in two), where the block that arrives last at a stage's end does what needs the whole row.
+// Three forms: short rows without a cut, a wave each (4096 rows of 1001 f32: 11 us); one block a row; and, for few long rows, 32 or 64
+// blocks a row over several launches (4096 draws from 640000 f32, top-p: 48 us in five; one of 131072 by top-k: 16 us in two), where the
+// block that arrives last at a stage's end does what needs the whole row.
+// Of one block a row, 256 rows of 131072 bf16: by top-k 1000 and top-p 34 us, of which 15 are the pass for the maximum (4.5 TB/s), 3 the
+// bound, 6 the list and 11 its two sorts, cuts and the draw, with no other block on the CU and the vector units busy 30 % of the whole; by
+// top-p alone 127 us, vector units busy 66 %: 12 maximum, 45 histogram, 21 cut (bf16 ties overflow the list), 49 masses of the tiles and the draw.
 #include <algorithm>
 #include "nrf_types.h"
 
@@ -407,7 +409,8 @@ __device__ __forceinline__ RowState row_state(const SampleArgs &a, int r, float 
 
 // Masses of a histogram are added as 64-bit integers, which give the same sums in any order.  A bin's unit goes down with its masses:
 // the entries of bin b weigh at most 2^(-b lift) (but for some 1e-3 that f32 rounds into the bin), so e * 2^raise <= 2^shift * 1.001 and
-// the words of kSegment entries stay below 2^63.  An entry is held to half a unit, 2^-42 of its bin's largest at kSegment entries.
+// the words of kSegment entries stay below 2^63.  An entry is held to half a unit, 2^-42 of its bin's largest at kSegment entries
+// (the last bin has no lower end, but what begins there weighs e^-64 and less).
 __device__ __forceinline__ int raise(const RowState &o, int bin) { return o.shift + (int)((float)bin * o.lift); }
 // Nearest integer of 0 <= v < 2^52: the bits of 2^52 + v behind those of 2^52 (shift is at most 50: rows in a histogram have more than
 // 2048 entries)
@@ -1038,8 +1041,8 @@ __device__ __forceinline__ void wave_sort(uint64_t *list, int n, uint64_t *c) {
     for (int j = 0; j < P; ++j) c[j] = list[min(i0 + j, n - 1)];
 }
 
-// draw_top_k by one wave, for a list of at most 64 P entries and few draws: no barriers.  One row of 131072, top-k 50: 15.8 us a
-// call against 18.0 by the block's steps, 256 rows of 32768 11.7 against 14.0; lists of 200 with four entries a lane 23.6 against 21.6.
+// draw_top_k by one wave, for a list of at most 64 P entries and few draws: no barriers.  One row of 131072, top-k 50: 15.6 us a
+// call against 18.2 by the block's steps, 256 rows of 32768 11.8 against 13.5; lists of 200 with four entries a lane 23.6 against 21.6.
 template <int P, int BLOCK>
 __device__ __forceinline__ void draw_few(Shared<BLOCK> &s, const RowState &o, int n, const float *u, int draws, int64_t *ids, float *prob) {
     const int lane = threadIdx.x & 63, i0 = lane * P, last = min(o.f.k, n);
@@ -1578,7 +1581,7 @@ __device__ __forceinline__ RowState cut_state(const SampleArgs &a, int r, const 
     return o;
 }
 
-// Stage 5: masses of the tiles, a wave each (64 rows of 524288: 41 us); by the last block their running sums.
+// Stage 5: masses of the tiles, a wave each (64 rows of 524288: 44 us, vector units busy 66 %); by the last block their running sums.
 struct TileShared {
     double tab[16], wave_d[4];
     int32_t wave_last[4];
@@ -1633,9 +1636,9 @@ enum Cut { kNoCut, kListCut, kWideCut };       // kListCut: a top-k that the gro
 
 // Long rows: with many of them, a block each fills the chip and is done in one launch; few of them are split.  Measured, bf16, one block
 // a row against split rows, us a call (one draw; 64; 256):
-//   no cut  65536 x 64 rows: 28 / 26, 48 / 29, 116 / 46    131072 x 96: 47 / 40, 67 / 46, 134 / 71    524288 x 32: 157 / 39, 177 / 41, 245 / 49
-//   top-k 50  131072 x 4: 19 / 18  131072 x 16: 19 / 33  262144 x 4: 28 / 20  524288 x 16: 43 / 34  524288 x 32: 44 / 56
-//   top-p 0.9  32768 x 16: 42 / 64, 65 / 65, 147 / 67    131072 x 32: 117 / 110, 141 / 110, 223 / 119    524288 x 64: 440 / 308, 464 / 311, 546 / 329
+//   no cut  65536 x 64 rows: 26 / 24, 47 / 27, 116 / 43    131072 x 96: 45 / 38, 65 / 44, 135 / 67    524288 x 32: 155 / 36, 176 / 38, 245 / 45
+//   top-k 50  131072 x 4: 17 / 16  131072 x 16: 17 / 29  262144 x 4: 25 / 16  524288 x 16: 40 / 30  524288 x 32: 41 / 50
+//   top-p 0.9  32768 x 16: 41 / 61, 66 / 62, 149 / 65    131072 x 32: 117 / 109, 141 / 110, 224 / 119    524288 x 64: 439 / 302, 463 / 306, 546 / 323
 // Without a list that holds all that is kept, one block draws 16 at a time.
 Form form_of(int64_t rows, int size, int draws, Cut cut) {
     if (size <= kList) return cut == kNoCut && draws <= 16 ? kWaveForm : kShortForm;
@@ -1662,7 +1665,7 @@ void launch_sample(const SampleArgs &a, bool may_k, bool may_p, RowWork *work, h
         sample_short_kernel<T><<<a.rows, 256, 0, s>>>(a);
     } else if (form == kRowForm) {
         // 16 pieces of 1024 threads hold 131072 16-bit or 65536 f32 logits; they pay where top-k reads the row twice (256 rows of
-        // 131072: 40.0 us against 41.6)
+        // 131072, top-k 1000: 34.0 us against 36.7)
         if (may_k && a.size <= 16 * 1024 * Vec<T>::E) sample_row_kernel<T, 16><<<a.rows, 1024, 0, s>>>(a);
         else sample_row_kernel<T, 0><<<a.rows, 1024, 0, s>>>(a);
     } else {
@@ -1673,7 +1676,7 @@ void launch_sample(const SampleArgs &a, bool may_k, bool may_p, RowWork *work, h
         if (may_k) sample_groups_kernel<T><<<parts, 1024, 0, s>>>(a, work, alone);
         if (alone) return;
         if (may_k || may_p) {
-            // 4096 draws from one row of 640000 by top-p: 51.1 us with 32 blocks a row, 47.4 with 64, 48.8 with 128
+            // 4096 draws from one row of 640000 by top-p: 51.2 us with 32 blocks a row, 47.5 with 64, 48.7 with 128
             const dim3 more(std::clamp(128 / a.rows, kParts, 64), a.rows);
             sample_bins_kernel<T><<<more, 1024, 0, s>>>(a, work);
             sample_cut_kernel<T><<<more, 1024, 0, s>>>(a, work);
